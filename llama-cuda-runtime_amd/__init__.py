@@ -163,6 +163,15 @@ SIGNATURES = {
     "lcr_gemm_qkv_rope_ws": (_I, [_P, ctypes.POINTER(KvView), _P, _P, _P, _I, _I, _I, _I, _I, _P,
                                   ctypes.c_size_t, _P]),
     "lcr_prefill_attention": (_I, [_P, _P, ctypes.POINTER(KvView), _I, _I, _I, _I, _F, _I, _P]),
+    # lcr_batch.h
+    "lcr_batch_map": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "lcr_batch_norm_rope_write_kv": (_I, [_P, ctypes.POINTER(KvView), _P, _P, _P, _P, _P, _F, _P, _I, _P, _P, _I, _I,
+                                          _I, _I, _P]),
+    "lcr_batch_attention": (_I, [_P, _P, ctypes.POINTER(KvView), _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ,
+                                 _P]),
+    "lcr_batch_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "lcr_batch_verify": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P]),
+    "lcr_batch_verify_workspace_bytes": (_SZ, [_I, _I, _I]),
     # lcr_model.h
     "lcr_model_default_options": (None, [ctypes.POINTER(ModelOptions)]),
     "lcr_model_create": (_I, [ctypes.c_char_p, ctypes.POINTER(ModelOptions), ctypes.POINTER(_P)]),
