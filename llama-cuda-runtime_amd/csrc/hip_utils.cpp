@@ -100,6 +100,21 @@ DeviceInfo query_device(int index) {
   return d;
 }
 
+int device_compute_units() {
+  static int cached[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cached[dev] == 0) {
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        cus <= 0) {
+      cus = 256;
+    }
+    cached[dev] = cus;
+  }
+  return cached[dev];
+}
+
 GpuTimer::EventHandle GpuTimer::make_event() {
   hipEvent_t e = nullptr;
   HIP_CHECK(hipEventCreate(&e));

@@ -65,6 +65,9 @@ struct DeviceInfo {
 
 DeviceInfo query_device(int index);
 
+// Compute units of the current device (256 when the runtime does not say).
+int device_compute_units();
+
 // Times a region of a stream with two events; the host only waits in
 // elapsed_ms().
 class GpuTimer {
