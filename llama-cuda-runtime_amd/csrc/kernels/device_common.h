@@ -71,6 +71,11 @@ __device__ __forceinline__ void load_to_lds16(const void* src, uint32_t lds_addr
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds_address) : "memory");
 }
 
+// The same from a uniform address and a lane's byte offset from it.
+__device__ __forceinline__ void load_to_lds16(const void* base, uint32_t offset, uint32_t lds_address) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "{m0}"(lds_address) : "memory");
+}
+
 // Wait until at most kCount vector-memory operations of this wave are in
 // flight and every LDS access has returned (gfx9 encoding: vmcnt bits 3:0 and
 // 15:14, expcnt 6:4 left at its maximum, lgkmcnt 11:8 zero).

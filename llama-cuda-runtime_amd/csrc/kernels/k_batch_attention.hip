@@ -19,7 +19,7 @@
 // Arithmetic. S^T = K . Q^T on 16x16x32 matrix instructions: a lane holds one
 // packed row and four keys of each sixteen. One pass over the keys:
 //   p = exp2(c s + b), c = scale log2 e, b = -(c m) for a running maximum m
-//   l += p;  O^T += V^T . P^T
+//   l += 1 . P^T;  O^T += V^T . P^T
 // A new m is taken when some p would pass 2^8, and l and O then move to the new
 // base by exp2(b_new - b); a row's l and O always share one base, so its
 // rounding cancels in O / l. p is rounded to the element type for the value
@@ -62,6 +62,7 @@ struct BatchAttnArgs {
   int table_stride;
   int pool_pages;
   int q_row_stride;
+  int held;  // positions that a table has pages for
   float scale;
 };
 
@@ -69,42 +70,93 @@ struct BatchAttnArgs {
 // Work division
 // ---------------------------------------------------------------------------
 
-// What the matrix-core kernels need besides.
+// n / d for 0 <= n < 2^31: n * magic >> shift with magic = ceil(2^shift / d) and
+// 2^(shift - 31) >= d. magic * d is past 2^shift by less than d, so the error,
+// n / 2^shift of that, stays under 1 / d.
+struct FastDivide {
+  uint32_t magic;
+  uint32_t shift;
+
+  static FastDivide by(uint32_t d) {
+    uint32_t shift = 31;
+    while ((1ull << (shift - 31)) < d) ++shift;
+    return FastDivide{static_cast<uint32_t>(((1ull << shift) + d - 1) / d), shift};
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<uint32_t>(n)) * magic) >> shift);
+  }
+};
+
+// A unit that lies over a cut, for the join: written by the share it begins in.
+struct alignas(16) CutUnit {
+  int rows;             // packed rows; 0: the share leaves no unit unfinished
+  int last_share;
+  int first_row;        // of the buffer
+  int kv;
+  int position;         // of the first token
+};
+
+// A value that is the same in every lane, held once for the wave.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A kernel argument in registers of its own. Left in the sixteen that one load
+// brings, it is spilled and restored with all of them.
+template <typename T>
+__device__ __forceinline__ T own_register(T v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
+// What the matrix-core kernels need besides. Work is counted in steps of 64
+// keys.
 struct FlashPlan {
   uint32_t group_magic;   // r / group = r * group_magic >> 16 for r < 256
-  uint32_t page_magic;    // key / page_size = mulhi(key, page_magic) >> page_shift
-  int page_shift;
-  int whole_pages;        // page_size is a multiple of a load's rows
+  FastDivide by_page;     // by page_size
+  FastDivide by_tile;     // by tile_tokens
+  FastDivide by_shares;   // by shares
   int tile_tokens;        // tokens of a tile of many rows
-  int shares;             // blocks the keys are cut for; 0: a unit a block
-  int min_share;          // keys
+  int shares;             // of each kv head
+  int split;              // 0: a share is a unit
+  int min_share;          // steps
   float scale_log2e;
-  long long* starts;      // [batch + 2] keys before each sequence, their total, and the share
-  float* partials;        // [2 * shares][rows][head_dim], then [2 * shares][rows][2] bases and sums
+  CutUnit* cuts;          // [shares of all heads] the unit that each share leaves unfinished
+  float* partials;        // [2 * shares of all heads][rows][head_dim], then [...][rows][2] bases and sums
 };
 
 constexpr int kFewRows = 32;
-// Keys that a unit counts for besides its own: its queries, the join of the
+// Steps that a unit counts for besides its keys': its queries, the join of the
 // waves, the output.
-constexpr int kUnitKeys = 64;
-constexpr int kStepKeys = 64;  // shares are cut at multiples of this within a unit
+constexpr int kUnitSteps = 2;
+constexpr int kStepKeys = 64;
 
-// A sequence's share of the work, in tokens and keys of one kv head.
+// A sequence's share of the work, in tokens and steps of one kv head.
 struct Sequence {
   int row0;      // first row
   int rows;      // as row_starts says
   int tokens;    // at most max_new
   int tiles;
-  long long before;  // positions before its first row (may be negative)
+  int before;    // positions before its first row (may be negative)
   int visible;   // keys its last token sees
+  int steps;     // what it counts for
 };
 
 // Keys that token i of a sequence sees.
-__device__ __forceinline__ int keys_seen(const BatchAttnArgs& a, long long before, int i) {
-  const long long held = static_cast<long long>(a.table_stride) * a.view.page_size;
-  return static_cast<int>(max(0ll, min(before + i + 1, held)));
+__device__ __forceinline__ int keys_seen(const BatchAttnArgs& a, int before, int i) {
+  return max(0, min(before + i + 1, a.held));
 }
 
+// Steps the tiles before tile i count for: tile j sees up to
+// visible - tokens + (j + 1) tile_tokens keys. An estimate besides what is seen
+// (negative positions, the table's end) only makes a share longer or shorter.
+__device__ __forceinline__ int steps_before_tile(const FlashPlan& plan, const Sequence& s, int i) {
+  if (!plan.split) return i;
+  const long long tiles = i;
+  const long long keys = tiles * max(s.visible - s.tokens, 0) + plan.tile_tokens * (tiles * (tiles + 1) / 2);
+  return i * kUnitSteps + static_cast<int>(keys / kStepKeys);
+}
+
+// kMany: sequences may have more rows than a tile of few.
+template <bool kMany>
 __device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const FlashPlan& plan, int b) {
   const int lo = a.row_starts[b], hi = a.row_starts[b + 1];
   const int length = a.lengths[b];
@@ -113,87 +165,83 @@ __device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const 
   // starts that are no ascending rows of the buffer name no rows
   s.rows = lo >= 0 && hi > lo && hi <= a.tokens ? hi - lo : 0;
   s.tokens = min(s.rows, a.max_new);
-  s.tiles = s.tokens * a.group <= kFewRows ? (s.rows > 0 ? 1 : 0) : (s.tokens - 1) / plan.tile_tokens + 1;
-  s.before = static_cast<long long>(length) - s.rows;
+  s.tiles = s.rows > 0 ? 1 : 0;
+  if (kMany && s.tokens * a.group > kFewRows) s.tiles = plan.by_tile(s.tokens - 1) + 1;
+  // lengths below -2^30 see nothing, as -2^30 does; rows are at most 2^30
+  s.before = max(length, -(1 << 30)) - s.rows;
   s.visible = s.tokens > 0 ? keys_seen(a, s.before, s.tokens - 1) : 0;
+  // up to the last tile, and that
+  s.steps = s.tiles;
+  if (plan.split && s.tiles > 0) {
+    s.steps = kUnitSteps + max(s.visible, s.tokens) / kStepKeys;
+    if (kMany && s.tiles > 1) s.steps += steps_before_tile(plan, s, s.tiles - 1);
+  }
   return s;
 }
 
-// Keys the tiles before tile i count for: tile j sees up to
-// visible - tokens + (j + 1) tile_tokens keys. An estimate above the keys that
-// are seen (negative positions, the table's end) only leaves a share short.
-__device__ __forceinline__ long long keys_before_tile(const FlashPlan& plan, const Sequence& s, int i) {
-  if (plan.shares == 0) return i;
-  const long long first = max(s.visible - s.tokens, 0);
-  return i * (first + kUnitKeys) + static_cast<long long>(plan.tile_tokens) * i * (i + 1) / 2;
-}
-
-__device__ __forceinline__ long long sequence_keys(const FlashPlan& plan, const Sequence& s) {
-  if (plan.shares == 0 || s.tiles == 0) return s.tiles;
-  const int last = s.tiles - 1;
-  return keys_before_tile(plan, s, last) + max(s.visible - s.tokens, 0) + s.tokens + kUnitKeys;
-}
-
-__device__ __forceinline__ long long share_of(const FlashPlan& plan, long long total, int kv_heads) {
-  if (plan.shares == 0) return 1;
-  const long long even = (total * kv_heads + plan.shares - 1) / plan.shares;
-  return (max(even, static_cast<long long>(plan.min_share)) + kStepKeys - 1) / kStepKeys * kStepKeys;
+__device__ __forceinline__ Sequence uniform(const Sequence& s) {
+  return Sequence{uniform(s.row0),   uniform(s.rows),    uniform(s.tokens), uniform(s.tiles),
+                  uniform(s.before), uniform(s.visible), uniform(s.steps)};
 }
 
 struct ShareStart {
-  long long total;      // keys of one kv head
-  long long share;
-  long long before;     // keys before the sequence
-  int sequence;
+  int total;      // steps of a kv head
+  int share;
+  int before;     // steps before the sequence
+  int sequence;   // -1: there is nothing left for this share
+  Sequence seq;
 };
 
-// Where share `index` begins: the prefix sums of the sequences' keys, taken by
-// the whole block. With `starts` they are written out for the join.
-template <int kThreads>
-__device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const FlashPlan& plan, long long index,
-                                                 long long* starts, long long* lds_sums, ShareStart* lds_found) {
+// Where a kv head's share `index` begins: the prefix sums of the sequences'
+// steps, taken by the whole block.
+template <bool kMany, int kThreads>
+__device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const FlashPlan& plan, int index,
+                                                 int* lds_sums, ShareStart* lds_found) {
   constexpr int kWaves = kThreads / 64;
   const int t = threadIdx.x;
   const int per = (a.batch + kThreads - 1) / kThreads;
-  long long mine = 0;
+  int mine = 0;
+  Sequence seq{};
   for (int k = 0; k < per; ++k) {
     const int b = t * per + k;
-    if (b < a.batch) mine += sequence_keys(plan, load_sequence(a, plan, b));
+    if (b < a.batch) {
+      seq = load_sequence<kMany>(a, plan, b);
+      mine += seq.steps;
+    }
   }
-  long long to = mine;
+  int to = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const long long other = __shfl_up(to, o, 64);
+    const int other = __shfl_up(to, o, 64);
     if (lane_id() >= o) to += other;
   }
   if (lane_id() == 63) lds_sums[t >> 6] = to;
   if (t == 0) lds_found->sequence = -1;
   __syncthreads();
-  long long total = 0, before = to - mine;
+  int total = 0, before = to - mine;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     if (w < (t >> 6)) before += lds_sums[w];
     total += lds_sums[w];
   }
-  const long long share = share_of(plan, total, a.view.num_kv_heads);
-  const long long at = index * share;
-  const long long within = total > 0 && at < total * a.view.num_kv_heads ? at % total : -1;
-  if (starts != nullptr || (within >= before && within < before + mine)) {
+  const int share = plan.split ? max(plan.by_shares(total + plan.shares - 1), plan.min_share) : 1;
+  const int at = index * share;
+  if (at >= before && at < before + mine) {
     for (int k = 0; k < per; ++k) {
       const int b = t * per + k;
       if (b >= a.batch) break;
-      const long long keys = sequence_keys(plan, load_sequence(a, plan, b));
-      if (starts != nullptr) starts[b] = before;
-      if (within >= before && within < before + keys) *lds_found = ShareStart{total, share, before, b};
-      before += keys;
+      if (per > 1) seq = load_sequence<kMany>(a, plan, b);
+      if (at < before + seq.steps) {
+        *lds_found = ShareStart{total, share, before, b, seq};
+        break;
+      }
+      before += seq.steps;
     }
   }
-  if (starts != nullptr && t == 0) {
-    starts[a.batch] = total;
-    starts[a.batch + 1] = share;
-  }
   __syncthreads();
-  return *lds_found;
+  const ShareStart found = *lds_found;
+  return ShareStart{uniform(found.total), uniform(found.share), uniform(found.before), uniform(found.sequence),
+                    uniform(found.seq)};
 }
 
 // Waits for direct loads and for LDS reads, across which the compiler moves no
@@ -208,10 +256,12 @@ __device__ __forceinline__ void reads_returned() { loads_landed<63>(); }
 
 // One block's part of a unit.
 struct Piece {
-  Sequence seq;
   const int32_t* table;
+  const elem_t* keys;    // the kv head's, of page 0
+  const elem_t* values;
   int kv;
-  int token0;      // first token of the tile
+  int before;      // positions before the tile's first token
+  int row0;        // the tile's first row
   int rows;        // packed rows
   int seen_first;  // keys that the tile's first and last token see
   int seen_last;
@@ -224,13 +274,18 @@ struct Piece {
 // Matrix-core kernels
 // ---------------------------------------------------------------------------
 
+// Blocks a compute unit, and waves a SIMD, follow from LDS and registers. At
+// head_dim 64, three blocks of four waves (168 registers a lane); at 128, one of
+// eight (256).
 template <int kHeadDim>
 struct FlashShape {
   static constexpr int kWaves = kHeadDim == 64 ? 4 : 8;
+  static constexpr int kBlocks = kHeadDim == 64 ? 3 : 1;      // resident a compute unit
+  static constexpr int kSimdWaves = kWaves * kBlocks / 4;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kTileRows = 32 * kWaves;               // packed rows of a tile of many rows
-  static constexpr int kSlots = kHeadDim == 64 ? 2 : 1;       // few rows: steps in flight a wave
-  static constexpr int kStages = 4;                           // many rows: tiles staged
+  static constexpr int kSlots = 1;                            // few rows: steps in flight a wave
+  static constexpr int kStages = kHeadDim == 64 ? 3 : 4;      // many rows: tiles staged
   static constexpr int kRowChunks = kHeadDim / 8;             // 16-byte chunks of a key
   static constexpr int kLoadRows = 64 / kRowChunks;           // keys of one 1 KiB direct load
   static constexpr int kSteps = kHeadDim / 32;                // k-steps of a score
@@ -238,17 +293,23 @@ struct FlashShape {
   // elements of LDS: a wave's slots (few) or a block's stages (many)
   static constexpr int kWaveElems = kSlots * 2 * 32 * kHeadDim;
   static constexpr int kRingElems = kStages * 2 * 64 * kHeadDim;
-  static_assert(kRingElems == kWaves * kWaveElems, "both use the same LDS");
+  static_assert(kRingElems >= kWaves * kWaveElems, "both use the same LDS");
 };
 
 template <int kHeadDim>
 struct FlashLds {
   elem_t ring[FlashShape<kHeadDim>::kRingElems];
   float stats[FlashShape<kHeadDim>::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
-  long long sums[FlashShape<kHeadDim>::kWaves];
+  int sums[FlashShape<kHeadDim>::kWaves];
   ShareStart found;
   int bad;  // a page outside the pool was read
 };
+
+#if defined(LCR_ELEM_FP16)
+constexpr uint32_t kInfBits = 0x7c00u, kOneBits = 0x3c00u;
+#else
+constexpr uint32_t kInfBits = 0x7f80u, kOneBits = 0x3f80u;
+#endif
 
 // A packed-row fragment's accumulators: rows 16 rf + col, per lane.
 template <int kHeadDim, int kRF>
@@ -256,16 +317,34 @@ struct FlashRows {
   mfma_in8 q[kRF][FlashShape<kHeadDim>::kSteps];
   mfma_acc4 o[kRF][FlashShape<kHeadDim>::kDFrags];
   float base[kRF];  // +inf: no visible key yet
-  float sum[kRF];   // of this lane's keys
+  mfma_acc4 sum[kRF];  // of the row's weights, four times
   int seen[kRF];    // keys the row sees, at most key1
+  uint32_t up[kRF], down[kRF];  // bit 4 df + e: o[rf][df][e] sees +inf, -inf (both: NaN)
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int rf = 0; rf < kRF; ++rf) {
       base[rf] = __builtin_huge_valf();
-      sum[rf] = 0.0f;
+      sum[rf] = mfma_acc4{0.f, 0.f, 0.f, 0.f};
+      up[rf] = down[rf] = 0;
 #pragma unroll
       for (int df = 0; df < FlashShape<kHeadDim>::kDFrags; ++df) o[rf][df] = mfma_acc4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  __device__ __forceinline__ void add_special() {
+#pragma unroll
+    for (int rf = 0; rf < kRF; ++rf) {
+      if (!__any((up[rf] | down[rf]) != 0)) continue;
+#pragma unroll
+      for (int df = 0; df < FlashShape<kHeadDim>::kDFrags; ++df) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool plus = (up[rf] >> (4 * df + e) & 1) != 0, minus = (down[rf] >> (4 * df + e) & 1) != 0;
+          if (plus) o[rf][df][e] += __builtin_huge_valf();
+          if (minus) o[rf][df][e] -= __builtin_huge_valf();
+        }
+      }
     }
   }
 };
@@ -286,11 +365,23 @@ __device__ __forceinline__ void load_rows(FlashRows<kHeadDim, kRF>& rows, const 
     const int r = min(row0 + 16 * rf + col, p.rows - 1);
     const int token = packed_token(plan, r);
     const int head = p.kv * a.group + r - token * a.group;
-    const elem_t* q = a.q + static_cast<size_t>(p.seq.row0 + p.token0 + token) * a.q_row_stride +
+    const elem_t* q = a.q + static_cast<size_t>(p.row0 + token) * a.q_row_stride +
                       static_cast<size_t>(head) * kHeadDim + 8 * grp;
 #pragma unroll
     for (int ks = 0; ks < FlashShape<kHeadDim>::kSteps; ++ks) rows.q[rf][ks] = as_operand(load16(q + 32 * ks));
-    rows.seen[rf] = min(keys_seen(a, p.seq.before, p.token0 + token), p.key1);
+    rows.seen[rf] = min(keys_seen(a, p.before, token), p.key1);
+  }
+}
+
+// Waits for the queries here. Left to their first use, inside the loop over the
+// tiles, the compiler's wait for them there is one for every direct load in
+// flight, each time round.
+template <int kHeadDim, int kRF>
+__device__ __forceinline__ void hold_rows(FlashRows<kHeadDim, kRF>& rows) {
+#pragma unroll
+  for (int rf = 0; rf < kRF; ++rf) {
+#pragma unroll
+    for (int ks = 0; ks < FlashShape<kHeadDim>::kSteps; ++ks) asm volatile("" : "+v"(rows.q[rf][ks]));
   }
 }
 
@@ -362,19 +453,14 @@ struct TileWork {
       }
       // before the first visible key every score is -inf: against base 0
       const float base = rows.base[rf] == __builtin_huge_valf() ? 0.0f : rows.base[rf];
-      float sum = 0.0f;
 #pragma unroll
       for (int kf = 0; kf < kKF; ++kf) {
         float p[4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rf][kf][v], c, base));
-          sum += p[v];
-        }
+        for (int v = 0; v < 4; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rf][kf][v], c, base));
         packed[rf][kf][0] = pack_rounded(p[0], p[1]);
         packed[rf][kf][1] = pack_rounded(p[2], p[3]);
       }
-      rows.sum[rf] += sum;
     }
   }
 
@@ -383,93 +469,121 @@ struct TileWork {
                              packed[rf][2 * half + 1][1]}});
   }
 
-  __device__ __forceinline__ void products(FlashRows<kHeadDim, kRF>& rows, const elem_t* values, bool whole) {
+  // The weights' sum is a product with ones: of what the values are weighted
+  // with, rounded as they are, and off the vector units, which the exponentials
+  // keep busy.
+  __device__ __forceinline__ void products(FlashRows<kHeadDim, kRF>& rows, const elem_t* values) {
+    constexpr uint32_t kOnes = kOneBits << 16 | kOneBits;
+    const mfma_in8 ones = as_operand(vec16{{kOnes, kOnes, kOnes, kOnes}});
 #pragma unroll
     for (int half = 0; half < kKF / 2; ++half) {
 #pragma unroll
+      for (int rf = 0; rf < kRF; ++rf) rows.sum[rf] = mfma16x16x32(ones, weight_operand(rf, half), rows.sum[rf]);
+#pragma unroll
       for (int df = 0; df < Shape::kDFrags; ++df) {
-        mfma_in8 v = transposed_values<kHeadDim>(values, half, df, lane_id());
-        if (!whole) v = without_special(rows, v, half, df);
+        const mfma_in8 v = transposed_values<kHeadDim>(values, half, df, lane_id());
 #pragma unroll
         for (int rf = 0; rf < kRF; ++rf) rows.o[rf][df] = mfma16x16x32(v, weight_operand(rf, half), rows.o[rf][df]);
       }
     }
   }
 
-  // For a tile that some row does not see whole. An infinity or NaN among its
-  // values would reach, as 0 * inf in the matrix product, the rows that do not
-  // see it. It is taken as 0 there, and a product with 1 in its place shows the
-  // rows that do see it (weight above 0), which get it added; a NaN is added as
-  // both infinities.
-  __device__ __forceinline__ mfma_in8 without_special(FlashRows<kHeadDim, kRF>& rows, const mfma_in8& operand, int half,
-                                                      int df) {
-#if defined(LCR_ELEM_FP16)
-    constexpr uint32_t kInf = 0x7c00u, kOne = 0x3c00u;
-#else
-    constexpr uint32_t kInf = 0x7f80u, kOne = 0x3f80u;
-#endif
-    vec16 v = __builtin_bit_cast(vec16, operand);
-    bool special = false;
+  // Which rows see an infinity or NaN of the tile (with a weight above 0), by a
+  // product with 1 in its place; a NaN counts as both infinities.
+  __device__ __forceinline__ void mark_special(FlashRows<kHeadDim, kRF>& rows, const elem_t* values) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) special |= (v.w[i] & kInf) == kInf || ((v.w[i] >> 16) & kInf) == kInf;
-    if (!__any(special)) return operand;
-    vec16 up, down;
+    for (int half = 0; half < kKF / 2; ++half) {
+#pragma unroll 1
+      for (int df = 0; df < Shape::kDFrags; ++df) {
+        const vec16 v = __builtin_bit_cast(vec16, transposed_values<kHeadDim>(values, half, df, lane_id()));
+        vec16 up, down;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t kept = 0, plus = 0, minus = 0;
+        for (int i = 0; i < 4; ++i) {
+          uint32_t plus = 0, minus = 0;
 #pragma unroll
-      for (int h = 0; h < 32; h += 16) {
-        const uint32_t x = (v.w[i] >> h) & 0xffffu;
-        const bool out = (x & kInf) == kInf;
-        kept |= (out ? 0u : x) << h;
-        plus |= (out && x != (0x8000u | kInf) ? kOne : 0u) << h;
-        minus |= (out && x != kInf ? kOne : 0u) << h;
-      }
-      v.w[i] = kept;
-      up.w[i] = plus;
-      down.w[i] = minus;
-    }
+          for (int h = 0; h < 32; h += 16) {
+            const uint32_t x = (v.w[i] >> h) & 0xffffu;
+            const bool special = (x & kInfBits) == kInfBits;
+            plus |= (special && x != (0x8000u | kInfBits) ? kOneBits : 0u) << h;
+            minus |= (special && x != kInfBits ? kOneBits : 0u) << h;
+          }
+          up.w[i] = plus;
+          down.w[i] = minus;
+        }
 #pragma unroll
-    for (int rf = 0; rf < kRF; ++rf) {
-      const mfma_acc4 zero{0.f, 0.f, 0.f, 0.f};
-      const mfma_acc4 a = mfma16x16x32(as_operand(up), weight_operand(rf, half), zero);
-      const mfma_acc4 b = mfma16x16x32(as_operand(down), weight_operand(rf, half), zero);
+        for (int rf = 0; rf < kRF; ++rf) {
+          const mfma_acc4 zero{0.f, 0.f, 0.f, 0.f};
+          const mfma_acc4 a = mfma16x16x32(as_operand(up), weight_operand(rf, half), zero);
+          const mfma_acc4 b = mfma16x16x32(as_operand(down), weight_operand(rf, half), zero);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (a[e] > 0.0f) rows.o[rf][df][e] += __builtin_huge_valf();
-        if (b[e] > 0.0f) rows.o[rf][df][e] -= __builtin_huge_valf();
+          for (int e = 0; e < 4; ++e) {
+            rows.up[rf] |= (a[e] > 0.0f ? 1u : 0u) << (4 * df + e);
+            rows.down[rf] |= (b[e] > 0.0f ? 1u : 0u) << (4 * df + e);
+          }
+        }
       }
     }
-    return as_operand(v);
   }
 };
 
+// Infinities and NaN among the values of a tile that some row does not see
+// whole. In the matrix product they would reach, as 0 * inf, rows that do not
+// see them: such a tile's are marked in the rows that do, which get them added
+// at the end, and then cleared.
+__device__ __forceinline__ bool pair_special(uint32_t w) {
+  return (w & kInfBits) == kInfBits || ((w >> 16) & kInfBits) == kInfBits;
+}
+
+// Whether `chunks` groups of 64 16-byte chunks hold any.
+__device__ __forceinline__ bool any_special(const elem_t* values, int chunks) {
+  bool special = false;
+#pragma unroll 4
+  for (int n = 0; n < chunks; ++n) {
+    const vec16 v = load16(values + 8 * (64 * n + lane_id()));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) special |= pair_special(v.w[i]);
+  }
+  return __any(special);
+}
+
+__device__ __forceinline__ void clear_special(elem_t* values, int chunks) {
+#pragma unroll 1
+  for (int n = 0; n < chunks; ++n) {
+    elem_t* at = values + 8 * (64 * n + lane_id());
+    vec16 v = load16(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((v.w[i] & kInfBits) == kInfBits) v.w[i] &= 0xffff0000u;
+      if (((v.w[i] >> 16) & kInfBits) == kInfBits) v.w[i] &= 0xffffu;
+    }
+    store16(at, v);
+  }
+}
+
 // Direct loads of kLoads groups of kLoadRows keys: group n of a call holds
 // keys key_of(n) .. + kLoadRows - 1 (those past `last` repeat it). With whole
-// pages a group lies in one page, whose table entry is a scalar load; a vector
-// load of it would be waited for with every tile load in flight.
+// pages (page_size a multiple of kLoadRows) a group lies in one page, whose table
+// entry is a scalar load; otherwise each lane reads its own key's, and waits for
+// it with every tile load in flight.
 template <int kLoads>
 struct LoadPages {
   int page[kLoads];
   int slot[kLoads];  // of the group's first key, within its page
 };
 
-template <int kHeadDim, int kLoads, typename KeyOf>
+template <int kHeadDim, bool kWholePages, int kLoads, typename KeyOf>
 __device__ __forceinline__ LoadPages<kLoads> find_pages(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p,
-                                                        int last, bool& bad, KeyOf key_of) {
+                                                        int last, KeyOf key_of) {
   LoadPages<kLoads> pages;
   typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
   const constant_ptr table = (constant_ptr)(reinterpret_cast<uintptr_t>(p.table));
   constexpr int kLoadRows = FlashShape<kHeadDim>::kLoadRows;
 #pragma unroll
   for (int n = 0; n < kLoads; ++n) {
-    if (plan.whole_pages) {
-      const int key = __builtin_amdgcn_readfirstlane(min(key_of(n), last / kLoadRows * kLoadRows));
-      const int index = static_cast<int>(__umulhi(static_cast<uint32_t>(key), plan.page_magic) >> plan.page_shift);
-      const int page = table[index];
-      const bool inside = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool_pages);
-      bad |= !inside;
-      pages.page[n] = inside ? page : 0;
+    if constexpr (kWholePages) {
+      const int key = uniform(min(key_of(n), last / kLoadRows * kLoadRows));
+      const int index = plan.by_page(key);
+      pages.page[n] = table[index];
       pages.slot[n] = key - index * a.view.page_size;
     } else {
       pages.page[n] = pages.slot[n] = 0;
@@ -478,36 +592,40 @@ __device__ __forceinline__ LoadPages<kLoads> find_pages(const BatchAttnArgs& a, 
   return pages;
 }
 
-template <int kHeadDim, int kLoads, bool kKeys, typename KeyOf, typename RowOf>
+// A page outside the pool is read as page 0, and `bad` set.
+__device__ __forceinline__ int pool_page(const BatchAttnArgs& a, int page, int& bad) {
+  const bool inside = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pool_pages);
+  bad |= inside ? 0 : 1;
+  return inside ? page : 0;
+}
+
+template <int kHeadDim, bool kWholePages, int kLoads, bool kKeys, typename KeyOf, typename RowOf>
 __device__ __forceinline__ void issue_loads(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
-                                            const LoadPages<kLoads>& pages, bool& bad, elem_t* tile, KeyOf key_of,
+                                            const LoadPages<kLoads>& pages, int& bad, elem_t* tile, KeyOf key_of,
                                             RowOf row_of) {
   using Shape = FlashShape<kHeadDim>;
   const int load_row = lane_id() / Shape::kRowChunks;
   const int load_slot = lane_id() % Shape::kRowChunks;
-  const elem_t* pool = kKeys ? a.view.keys : a.view.values;
-  const size_t head_at = static_cast<size_t>(p.kv) * static_cast<size_t>(a.view.head_stride);
+  const elem_t* pool = kKeys ? p.keys : p.values;
 #pragma unroll
   for (int n = 0; n < kLoads; ++n) {
     const int row = row_of(n);  // of the tile, the group's first
     const int swizzle = kKeys ? key_swizzle<kHeadDim>(row + load_row) : value_swizzle<kHeadDim>(row + load_row);
-    size_t at;
-    if (plan.whole_pages) {
+    const uint32_t to = lds_address_of(tile + row * kHeadDim);
+    if constexpr (kWholePages) {
       const int first = min(key_of(n), last / Shape::kLoadRows * Shape::kLoadRows);
-      at = static_cast<size_t>(pages.page[n]) * static_cast<size_t>(a.view.page_stride) + head_at +
-           static_cast<size_t>((pages.slot[n] + min(load_row, last - first)) * kHeadDim);
+      const int page = pool_page(a, pages.page[n], bad);
+      const size_t from = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                          static_cast<size_t>(pages.slot[n] * kHeadDim);
+      load_to_lds16(pool + from, 2u * (min(load_row, last - first) * kHeadDim + 8 * (load_slot ^ swizzle)), to);
     } else {
       const int key = min(key_of(n) + load_row, last);
-      const int index = key / a.view.page_size;
-      int page = p.table[index];
-      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pool_pages)) {
-        bad = true;
-        page = 0;
-      }
-      at = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) + head_at +
-           static_cast<size_t>(key - index * a.view.page_size) * kHeadDim;
+      const int index = plan.by_page(key);
+      const int page = pool_page(a, p.table[index], bad);
+      const size_t at = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                        static_cast<size_t>(key - index * a.view.page_size) * kHeadDim;
+      load_to_lds16(pool + at + 8 * (load_slot ^ swizzle), to);
     }
-    load_to_lds16(pool + at + 8 * (load_slot ^ swizzle), lds_address_of(tile + row * kHeadDim));
   }
 }
 
@@ -515,17 +633,17 @@ __device__ __forceinline__ void issue_loads(const BatchAttnArgs& a, const FlashP
 template <int kHeadDim>
 __device__ __forceinline__ size_t out_at(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int r) {
   const int token = packed_token(plan, r);
-  return (static_cast<size_t>(p.seq.row0 + p.token0 + token) * a.num_heads + p.kv * a.group + (r - token * a.group)) *
+  return (static_cast<size_t>(p.row0 + token) * a.num_heads + p.kv * a.group + (r - token * a.group)) *
          kHeadDim;
 }
 
 template <int kHeadDim>
-__device__ __forceinline__ float* partial_stats(const FlashPlan& plan, int tile_rows) {
-  return plan.partials + static_cast<size_t>(2 * plan.shares) * tile_rows * kHeadDim;
+__device__ __forceinline__ float* partial_stats(const FlashPlan& plan, int kv_heads, int tile_rows) {
+  return plan.partials + static_cast<size_t>(2 * plan.shares) * kv_heads * tile_rows * kHeadDim;
 }
 
 // At most 32 rows: the waves split the keys.
-template <int kHeadDim, int kRF, int kTileRows>
+template <int kHeadDim, bool kWholePages, int kRF, int kTileRows>
 __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAttnArgs& a, const FlashPlan& plan,
                                          const Piece& p) {
   using Shape = FlashShape<kHeadDim>;
@@ -541,14 +659,14 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   const int tiles = (p.key1 - p.key0 + 31) / 32;
   const int count = tiles > wave ? (tiles - wave - 1) / Shape::kWaves + 1 : 0;
   const int last = p.key1 - 1;
-  bool bad = false;
+  int bad = 0;
   auto first_key = [&](int t) { return p.key0 + 32 * (wave + Shape::kWaves * t); };
   auto pages_of = [&](int t) {
-    return find_pages<kHeadDim, kLoads>(a, plan, p, last, bad, [&](int n) { return first_key(t) + Shape::kLoadRows * n; });
+    return find_pages<kHeadDim, kWholePages, kLoads>(a, plan, p, last, [&](int n) { return first_key(t) + Shape::kLoadRows * n; });
   };
   auto issue = [&](auto is_keys, int t, const LoadPages<kLoads>& pages) {
     constexpr bool kKeys = decltype(is_keys)::value;
-    issue_loads<kHeadDim, kLoads, kKeys>(a, plan, p, last, pages, bad, kKeys ? key_tile(t) : value_tile(t),
+    issue_loads<kHeadDim, kWholePages, kLoads, kKeys>(a, plan, p, last, pages, bad, kKeys ? key_tile(t) : value_tile(t),
                                          [&](int n) { return first_key(t) + Shape::kLoadRows * n; },
                                          [&](int n) { return Shape::kLoadRows * n; });
   };
@@ -559,15 +677,18 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   rows.clear();
   if (count > 0) {
     load_rows<kHeadDim, kRF>(rows, a, plan, p, 0);
+    LoadPages<kLoads> pages[kSlots];
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) pages[t] = pages_of(t);
 #pragma unroll
     for (int t = 0; t < kSlots; ++t) {
       if (t < count) {
-        const LoadPages<kLoads> pages = pages_of(t);
-        issue(Keys{}, t, pages);
-        issue(Values{}, t, pages);
+        issue(Keys{}, t, pages[t]);
+        issue(Values{}, t, pages[t]);
       }
     }
   }
+  hold_rows(rows);
   const int all_seen = min(p.seen_first, p.key1);
   for (int t = 0; t < count; ++t) {
     const int left = count - 1 - t;
@@ -596,23 +717,26 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
     } else {
       loads_landed<0>();
     }
-    work.products(rows, value_tile(t), whole);
+    if (!whole && any_special(value_tile(t), 32 * kHeadDim / 512)) {
+      work.mark_special(rows, value_tile(t));
+      clear_special(value_tile(t), 32 * kHeadDim / 512);
+    }
+    work.products(rows, value_tile(t));
     reads_returned();
     if (more) issue(Values{}, t + kSlots, pages);
   }
 
+  rows.add_special();
   // The waves' results meet in LDS, each in its own (now free) part.
-  if (__any(bad)) {
+  if (__any(bad != 0)) {
 #pragma unroll
-    for (int rf = 0; rf < kRF; ++rf) rows.sum[rf] = __builtin_nanf("");
+    for (int rf = 0; rf < kRF; ++rf) rows.sum[rf][0] = __builtin_nanf("");
   }
   float* outputs = reinterpret_cast<float*>(mine);
   static_assert(Shape::kWaveElems * sizeof(elem_t) >= kFewRows * kHeadDim * sizeof(float), "a wave's outputs fit");
 #pragma unroll
   for (int rf = 0; rf < kRF; ++rf) {
-    float sum = rows.sum[rf];
-    sum += xor_lane<16>(sum);
-    sum += xor_lane<32>(sum);
+    const float sum = rows.sum[rf][0];
     if (grp == 0) {
       lds.stats[wave][16 * rf + col][0] = rows.base[rf];
       lds.stats[wave][16 * rf + col][1] = sum;
@@ -646,13 +770,13 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
     if (p.slot >= 0) {
       *reinterpret_cast<mfma_acc4*>(plan.partials + (static_cast<size_t>(p.slot) * kTileRows + r) * kHeadDim + d) = o;
       if (d == 0) {
-        float* stats = partial_stats<kHeadDim>(plan, kTileRows) + (static_cast<size_t>(p.slot) * kTileRows + r) * 2;
+        float* stats = partial_stats<kHeadDim>(plan, a.view.num_kv_heads, kTileRows) + (static_cast<size_t>(p.slot) * kTileRows + r) * 2;
         stats[0] = base;
         stats[1] = sum;
       }
     } else {
       const int token = packed_token(plan, r);
-      const bool any = keys_seen(a, p.seq.before, p.token0 + token) > 0;
+      const bool any = keys_seen(a, p.before, token) > 0;
       const float inv = any ? 1.0f / sum : 0.0f;
       uint2 words;
       words.x = any ? pack_elems(o[0] * inv, o[1] * inv) : 0u;
@@ -664,7 +788,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
 }
 
 // Many rows: the waves split them, 32 each, and share the tiles.
-template <int kHeadDim>
+template <int kHeadDim, bool kWholePages>
 __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAttnArgs& a, const FlashPlan& plan,
                                           const Piece& p) {
   using Shape = FlashShape<kHeadDim>;
@@ -680,15 +804,15 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
   auto value_tile = [&](int t) { return key_tile(t) + 64 * kHeadDim; };
   const int tiles = (p.key1 - p.key0 + 63) / 64;
   const int last = p.key1 - 1;
-  bool bad = false;
+  int bad = 0;
   auto group_row = [&](int n) { return Shape::kLoadRows * (wave + Shape::kWaves * n); };
   auto pages_of = [&](int t) {
-    return find_pages<kHeadDim, kLoads>(a, plan, p, last, bad, [&](int n) { return p.key0 + 64 * t + group_row(n); });
+    return find_pages<kHeadDim, kWholePages, kLoads>(a, plan, p, last, [&](int n) { return p.key0 + 64 * t + group_row(n); });
   };
   auto issue = [&](int t, const LoadPages<kLoads>& pages) {
     auto key_of = [&](int n) { return p.key0 + 64 * t + group_row(n); };
-    issue_loads<kHeadDim, kLoads, true>(a, plan, p, last, pages, bad, key_tile(t), key_of, group_row);
-    issue_loads<kHeadDim, kLoads, false>(a, plan, p, last, pages, bad, value_tile(t), key_of, group_row);
+    issue_loads<kHeadDim, kWholePages, kLoads, true>(a, plan, p, last, pages, bad, key_tile(t), key_of, group_row);
+    issue_loads<kHeadDim, kWholePages, kLoads, false>(a, plan, p, last, pages, bad, value_tile(t), key_of, group_row);
   };
   if (threadIdx.x == 0) lds.bad = 0;
 
@@ -699,19 +823,23 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
   int all_seen = 0, any_seen = 0;
   if (active) {
     load_rows<kHeadDim, kRF>(rows, a, plan, p, row0);
-    all_seen = min(keys_seen(a, p.seq.before, p.token0 + packed_token(plan, row0)), p.key1);
-    any_seen = min(keys_seen(a, p.seq.before, p.token0 + packed_token(plan, min(row0 + 31, p.rows - 1))), p.key1);
+    all_seen = min(keys_seen(a, p.before, packed_token(plan, row0)), p.key1);
+    any_seen = min(keys_seen(a, p.before, packed_token(plan, min(row0 + 31, p.rows - 1))), p.key1);
   }
   constexpr int kAhead = Shape::kStages - 1;
   if (tiles > 0) {
+    LoadPages<kLoads> first[kAhead];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) first[t] = pages_of(t);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      if (t < tiles) issue(t, pages_of(t));
+      if (t < tiles) issue(t, first[t]);
     }
   }
-  LoadPages<kLoads> pages{};
-  if (kAhead < tiles) pages = pages_of(kAhead);
+  hold_rows(rows);
   for (int t = 0; t < tiles; ++t) {
+    LoadPages<kLoads> pages{};
+    if (t + kAhead < tiles) pages = pages_of(t + kAhead);
     // This wave's loads of the tile have landed (the later tiles' remain);
     // behind the barrier every wave's have, and the tile before is free.
     if (t + kAhead - 1 < tiles) {
@@ -721,27 +849,44 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
     }
     plain_barrier();
     if (t + kAhead < tiles) issue(t + kAhead, pages);
-    if (t + kAhead + 1 < tiles) pages = pages_of(t + kAhead + 1);
-    const int key0 = p.key0 + 64 * t;
-    if (key0 < any_seen) {
-      const bool whole = key0 + 64 <= all_seen;
-      TileWork<kHeadDim, kRF, 4> work;
-      work.scores(rows, key_tile(t));
-      if (!whole) work.mask(rows, key0);
-      work.weights(rows, plan.scale_log2e);
-      work.products(rows, value_tile(t), whole);
+    // A tile that some row of the unit does not see whole: every wave looks for
+    // infinities and NaN among its values, and finds the same.
+    const int tile0 = p.key0 + 64 * t;
+    const bool special = tile0 + 64 > p.seen_first && any_special(value_tile(t), kHeadDim / 8);
+    // 32 keys at a time: as many scores as registers allow with four waves a
+    // SIMD.
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const int key0 = tile0 + 32 * half;
+      const bool mine = key0 < any_seen;
+      elem_t* values = value_tile(t) + half * 32 * kHeadDim;
+      TileWork<kHeadDim, kRF, 2> work;
+      if (mine) {
+        work.scores(rows, key_tile(t) + half * 32 * kHeadDim);
+        if (key0 + 32 > all_seen) work.mask(rows, key0);
+        work.weights(rows, plan.scale_log2e);
+      }
+      if (special) {
+        if (mine) work.mark_special(rows, values);
+        wait_lds();
+        plain_barrier();
+        static_assert(kHeadDim / 16 <= Shape::kWaves, "a wave clears one group of chunks at most");
+        if (wave < kHeadDim / 16) clear_special(values + wave * 512, 1);
+        wait_lds();
+        plain_barrier();
+      }
+      if (mine) work.products(rows, values);
     }
   }
-  if (__any(bad) && lane == 0) lds.bad = 1;
+  if (__any(bad != 0) && lane == 0) lds.bad = 1;
   __syncthreads();  // every wave is done with the tiles; the flag is set
   if (!active) return;
+  rows.add_special();
   const bool spoilt = lds.bad != 0;
 #pragma unroll
   for (int rf = 0; rf < kRF; ++rf) {
     const int r = row0 + 16 * rf + col;
-    float sum = rows.sum[rf];
-    sum += xor_lane<16>(sum);
-    sum += xor_lane<32>(sum);
+    float sum = rows.sum[rf][0];
     if (spoilt) sum = __builtin_nanf("");
     if (r >= p.rows) continue;
     if (p.slot >= 0) {
@@ -751,12 +896,12 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
         *reinterpret_cast<mfma_acc4*>(plan.partials + at * kHeadDim + 16 * df + 4 * grp) = rows.o[rf][df];
       }
       if (grp == 0) {
-        float* stats = partial_stats<kHeadDim>(plan, kTileRows) + at * 2;
+        float* stats = partial_stats<kHeadDim>(plan, a.view.num_kv_heads, kTileRows) + at * 2;
         stats[0] = rows.base[rf];
         stats[1] = sum;
       }
     } else {
-      const bool any = keys_seen(a, p.seq.before, p.token0 + packed_token(plan, r)) > 0;
+      const bool any = keys_seen(a, p.before, packed_token(plan, r)) > 0;
       const float inv = any ? 1.0f / sum : 0.0f;
       elem_t* out = a.out + out_at<kHeadDim>(a, plan, p, r) + 4 * grp;
 #pragma unroll
@@ -770,170 +915,178 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
   }
 }
 
-// kMany: a sequence may have more than 32 packed rows.
-template <int kHeadDim, bool kMany>
-__global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, 2) void batch_attention_kernel(BatchAttnArgs a, FlashPlan plan) {
+// kMaxRows: packed rows a sequence may have, 16, 32 or any number (0).
+template <int kHeadDim, int kMaxRows, bool kWholePages>
+__global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim>::kSimdWaves) void batch_attention_kernel(
+    BatchAttnArgs args, FlashPlan flash_plan) {
   using Shape = FlashShape<kHeadDim>;
+  constexpr bool kMany = kMaxRows == 0;
   constexpr int kTileRows = kMany ? Shape::kTileRows : kFewRows;
   __shared__ __attribute__((aligned(1024))) FlashLds<kHeadDim> lds;
-  // Share: neighbours on one XCD (a grid of shares is a multiple of 8).
-  const long long index = plan.shares > 0
-      ? static_cast<long long>(blockIdx.x % 8u) * (gridDim.x / 8u) + blockIdx.x / 8u
-      : static_cast<long long>(blockIdx.x);
-  const ShareStart found = find_share<Shape::kThreads>(
-      a, plan, index, plan.shares > 0 && blockIdx.x == 0 ? plan.starts : nullptr, lds.sums, &lds.found);
+  BatchAttnArgs a = args;
+  a.view.page_size = own_register(a.view.page_size);
+  a.view.page_stride = own_register(a.view.page_stride);
+  a.pool_pages = own_register(a.pool_pages);
+  a.held = own_register(a.held);
+  a.group = own_register(a.group);
+  FlashPlan plan = flash_plan;
+  plan.by_page.magic = own_register(plan.by_page.magic);
+  plan.by_page.shift = own_register(plan.by_page.shift);
+  plan.group_magic = own_register(plan.group_magic);
+  plan.scale_log2e = own_register(plan.scale_log2e);
+
+  // Share: neighbours on one XCD where the grid is a multiple of 8.
+  const unsigned blocks = gridDim.x;
+  const int block = static_cast<int>(blocks % 8u == 0 ? blockIdx.x % 8u * (blocks / 8u) + blockIdx.x / 8u : blockIdx.x);
+  const int kv = plan.by_shares(block);
+  const ShareStart found =
+      find_share<kMany, Shape::kThreads>(a, plan, block - kv * plan.shares, lds.sums, &lds.found);
+  if (plan.split && threadIdx.x == 0) plan.cuts[block].rows = 0;
   if (found.sequence < 0) return;
-  const int kv_heads = a.view.num_kv_heads;
-  const long long end = min((index + 1) * found.share, found.total * kv_heads);
-  long long at = index * found.share;
-  int kv = __builtin_amdgcn_readfirstlane(static_cast<int>(at / found.total));
-  int b = __builtin_amdgcn_readfirstlane(found.sequence);
-  Sequence seq = load_sequence(a, plan, b);
-  long long before = kv * found.total + found.before;  // keys before the sequence
+  int b = found.sequence;
+  Sequence seq = found.seq;
+  int at = (block - kv * plan.shares) * found.share;
+  const int end = min(at + found.share, found.total);
+  int before = found.before;  // steps before the sequence
   // The tile that the share begins in: the last that starts at or before it.
   int tile = 0;
-  for (int lo = 0, hi = seq.tiles - 1; lo < hi;) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (before + keys_before_tile(plan, seq, mid) <= at) {
-      lo = mid;
-      tile = mid;
-    } else {
-      hi = mid - 1;
+  if constexpr (kMany) {
+    for (int lo = 0, hi = seq.tiles - 1; lo < hi;) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before + steps_before_tile(plan, seq, mid) <= at) {
+        lo = mid;
+        tile = mid;
+      } else {
+        hi = mid - 1;
+      }
     }
   }
-  while (at < end) {
-    const long long start = before + keys_before_tile(plan, seq, tile);
-    const long long keys = sequence_keys(plan, seq);
-    const long long stop = tile + 1 < seq.tiles ? before + keys_before_tile(plan, seq, tile + 1) : before + keys;
-    Piece p;
-    p.seq = seq;
+  Piece p;
+  p.kv = kv;
+  p.keys = a.view.keys + static_cast<size_t>(kv) * static_cast<size_t>(a.view.head_stride);
+  p.values = a.view.values + static_cast<size_t>(kv) * static_cast<size_t>(a.view.head_stride);
+  while (true) {
+    const int start = before + (kMany ? steps_before_tile(plan, seq, tile) : 0);
+    const int stop = before + (kMany && tile + 1 < seq.tiles ? steps_before_tile(plan, seq, tile + 1) : seq.steps);
+    const bool single = !kMany || seq.tokens * a.group <= kFewRows;
+    const int token0 = single ? 0 : tile * plan.tile_tokens;
+    const int tokens = single ? seq.tokens : min(plan.tile_tokens, seq.tokens - token0);
     p.table = a.view.page_table + static_cast<size_t>(b) * a.table_stride;
-    p.kv = kv;
-    const bool single = seq.tokens * a.group <= kFewRows;
-    p.token0 = tile * plan.tile_tokens;
-    const int tokens = single ? seq.tokens : min(plan.tile_tokens, seq.tokens - p.token0);
+    p.row0 = seq.row0 + token0;
+    p.before = seq.before + token0;
     p.rows = tokens * a.group;
-    p.seen_first = keys_seen(a, seq.before, p.token0);
-    p.seen_last = tokens > 0 ? keys_seen(a, seq.before, p.token0 + tokens - 1) : 0;
-    // Cuts within the unit round up to whole steps, both shares alike.
-    auto cut = [&](long long x) {
-      const long long k = x <= start ? 0 : (x - start + kStepKeys - 1) / kStepKeys * kStepKeys;
-      return static_cast<int>(min(k, static_cast<long long>(p.seen_last)));
-    };
+    p.seen_first = keys_seen(a, p.before, 0);
+    p.seen_last = tokens > 0 ? keys_seen(a, p.before, tokens - 1) : 0;
+    p.key0 = 0;
+    p.key1 = p.seen_last;
     p.slot = -1;
-    if (plan.shares > 0 && (start < at || stop > end)) {
-      p.slot = 2 * static_cast<int>(index) + (start < at ? 0 : 1);
-      p.key0 = cut(at);
-      p.key1 = stop > end ? cut(end) : p.seen_last;
-    } else {
-      p.key0 = 0;
-      p.key1 = p.seen_last;
+    if (plan.split && (start < at || stop > end)) {
+      // steps into the unit, in keys
+      auto cut = [&](int steps) { return steps >= (p.seen_last + kStepKeys - 1) / kStepKeys ? p.seen_last : steps * kStepKeys; };
+      p.slot = 2 * block + (start < at ? 0 : 1);
+      if (start < at) p.key0 = cut(at - start);
+      if (stop > end) p.key1 = cut(end - start);
+      if (start >= at && threadIdx.x == 0) {
+        plan.cuts[block] = CutUnit{p.rows, kv * plan.shares + static_cast<int>(static_cast<unsigned>(stop - 1) /
+                                                                               static_cast<unsigned>(found.share)),
+                                   p.row0, kv, p.before};
+      }
     }
-    // Rows past max_new are zeros, written with the sequence's first tile's
-    // first keys.
+    // Rows past max_new are zeros, written where the sequence begins.
     if (tile == 0 && start >= at && seq.rows > seq.tokens) {
-      const long long words = static_cast<long long>(seq.rows - seq.tokens) * a.group * (kHeadDim / 4);
-      for (long long i = threadIdx.x; i < words; i += Shape::kThreads) {
-        const long long r = i / (kHeadDim / 4);
-        const long long token = r / a.group;
-        const size_t row = static_cast<size_t>(seq.row0 + seq.tokens + token) * a.num_heads + kv * a.group +
-                           static_cast<size_t>(r - token * a.group);
-        *reinterpret_cast<uint2*>(a.out + row * kHeadDim + i % (kHeadDim / 4) * 4) = make_uint2(0u, 0u);
+      for (int i = seq.tokens; i < seq.rows; ++i) {
+        elem_t* row = a.out + (static_cast<size_t>(seq.row0 + i) * a.num_heads + kv * a.group) * kHeadDim;
+        for (int e = 4 * static_cast<int>(threadIdx.x); e < a.group * kHeadDim; e += 4 * Shape::kThreads) {
+          *reinterpret_cast<uint2*>(row + e) = make_uint2(0u, 0u);
+        }
       }
     }
     if (p.rows > 0) {
       if (!single) {
-        if constexpr (kMany) many_rows<kHeadDim>(lds, a, plan, p);
-      } else if (p.rows <= 16) {
-        few_rows<kHeadDim, 1, kTileRows>(lds, a, plan, p);
+        if constexpr (kMany) many_rows<kHeadDim, kWholePages>(lds, a, plan, p);
       } else {
-        few_rows<kHeadDim, 2, kTileRows>(lds, a, plan, p);
+        few_rows<kHeadDim, kWholePages, kMaxRows == 16 ? 1 : 2, kTileRows>(lds, a, plan, p);
       }
     }
     at = stop;
     if (at >= end) break;
-    if (++tile >= seq.tiles) {
+    if (!kMany || ++tile >= seq.tiles) {
       tile = 0;
-      before += keys;
-      do {  // the next sequence that has rows, in this kv head or the next
-        if (++b == a.batch) {
-          b = 0;
-          if (++kv == kv_heads) return;
-        }
-        seq = load_sequence(a, plan, b);
+      before += seq.steps;
+      do {  // the next sequence that has rows
+        if (++b == a.batch) return;
+        seq = uniform(load_sequence<kMany>(a, plan, b));
       } while (seq.tiles == 0);
     }
     if constexpr (kMany) __syncthreads();  // the tiles and the flag are free again
   }
 }
 
-// Joins the partials of each row whose unit lies over a cut: a block per token,
-// a wave per head.
+// Joins the partials of the units that lie over a cut: gridDim.y blocks for the
+// unit that share blockIdx.x leaves unfinished (most often none), four elements
+// of a packed row a lane, so that a wave has room for kGroups rows. Tiles of
+// many rows have few partials each, and the groups take a row each; few rows
+// have many, and the groups take the row's partials in turn.
 constexpr int kJoinThreads = 256;
 
-template <int kHeadDim>
+template <int kHeadDim, bool kRowEach>
 __global__ __launch_bounds__(kJoinThreads) void batch_attention_join_kernel(BatchAttnArgs a, FlashPlan plan,
                                                                            int tile_rows) {
-  __shared__ int lds_count[kJoinThreads / 64];
-  const int row = blockIdx.x;
+  constexpr int kRowLanes = kHeadDim / 4;
+  constexpr int kGroups = 64 / kRowLanes;
+  const CutUnit unit = plan.cuts[blockIdx.x];
+  if (unit.rows == 0) return;
   const int lane = lane_id();
-  const int wave = static_cast<int>(threadIdx.x) >> 6;
-  // The row's sequence: the starts at or before it, counted.
-  int below = 0;
-  for (int i = threadIdx.x; i <= a.batch; i += kJoinThreads) below += a.row_starts[i] <= row ? 1 : 0;
+  const int d = 4 * (lane % kRowLanes);
+  const int group = lane / kRowLanes;
+  const float* all_stats = partial_stats<kHeadDim>(plan, a.view.num_kv_heads, tile_rows);
+  const int waves = static_cast<int>(gridDim.y) * (kJoinThreads / 64);
+  const int wave = static_cast<int>(blockIdx.y) * (kJoinThreads / 64) + (static_cast<int>(threadIdx.x) >> 6);
+  constexpr int kWaveRows = kRowEach ? kGroups : 1;
+  const int first = static_cast<int>(blockIdx.x) + (kRowEach ? 0 : group);
+  for (int r0 = wave * kWaveRows; r0 < unit.rows; r0 += waves * kWaveRows) {
+    const int r = min(r0 + (kRowEach ? group : 0), unit.rows - 1);
+    float base = __builtin_huge_valf(), sum = 0.0f;
+    mfma_acc4 o{0.f, 0.f, 0.f, 0.f};
+    // (from, sum, x) joins (base, sum, o): both move to the smaller base. No
+    // keys: base +inf, nothing to add.
+    auto join = [&](float from, float part, const mfma_acc4& x) {
+      const float to = fminf(base, from);
+      const float keep = base == __builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(to - base);
+      const float move = from == __builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(to - from);
+      base = to;
+      sum = __builtin_fmaf(part, move, sum * keep);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
-  if (lane == 0) lds_count[wave] = below;
-  __syncthreads();
-  below = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 64; ++w) below += lds_count[w];
-  const int b = below - 1;
-  if (b < 0 || b >= a.batch) return;
-  const Sequence seq = load_sequence(a, plan, b);
-  const int i = row - seq.row0;
-  if (i < 0 || i >= seq.tokens) return;
-  const int seen = keys_seen(a, seq.before, i);
-  const bool single = seq.tokens * a.group <= kFewRows;
-  const int tile = single ? 0 : i / plan.tile_tokens;
-  const int in_tile = single ? i : i - tile * plan.tile_tokens;
-  const long long total = plan.starts[a.batch];
-  const long long share = plan.starts[a.batch + 1];
-  const long long first = plan.starts[b] + keys_before_tile(plan, seq, tile);
-  const long long next = tile + 1 < seq.tiles ? plan.starts[b] + keys_before_tile(plan, seq, tile + 1)
-                                              : plan.starts[b] + sequence_keys(plan, seq);
-  const float* all_stats = partial_stats<kHeadDim>(plan, tile_rows);
-  int last_kv = -1, from = 0, to = 0;
-  for (int head = wave; head < a.num_heads; head += kJoinThreads / 64) {
-    const int kv = head / a.group;
-    if (kv != last_kv) {
-      from = static_cast<int>((kv * total + first) / share);
-      to = static_cast<int>((kv * total + next - 1) / share);
-      last_kv = kv;
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], move, o[e] * keep);
+    };
+#pragma unroll 4
+    for (int s = first; s <= unit.last_share; s += kRowEach ? 1 : kGroups) {
+      // a share's first partial continues a unit, its second begins one
+      const size_t at = static_cast<size_t>(s == static_cast<int>(blockIdx.x) ? 2 * s + 1 : 2 * s) * tile_rows + r;
+      const float2 stats = *reinterpret_cast<const float2*>(all_stats + 2 * at);
+      join(stats.x, stats.y, *reinterpret_cast<const mfma_acc4*>(plan.partials + at * kHeadDim + d));
     }
-    if (from == to) continue;
-    const int r = in_tile * a.group + head - kv * a.group;
-    auto slot = [&](int s) { return static_cast<size_t>(s == from ? 2 * s + 1 : 2 * s) * tile_rows + r; };
-    float base = __builtin_huge_valf();
-    for (int s = from + lane; s <= to; s += 64) base = fminf(base, all_stats[2 * slot(s)]);
+    auto join_lane = [&](auto distance) {
+      constexpr int kDistance = decltype(distance)::value;
+      mfma_acc4 x;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) base = fminf(base, __shfl_xor(base, o, 64));
-    float sum = 0.0f;
-    float o[kHeadDim / 64] = {};
-    for (int s = from; s <= to; ++s) {
-      const float b_s = all_stats[2 * slot(s)], l_s = all_stats[2 * slot(s) + 1];
-      const float move = b_s == __builtin_huge_valf() ? 0.0f : __builtin_amdgcn_exp2f(base - b_s);
-      sum = __builtin_fmaf(l_s, move, sum);
-#pragma unroll
-      for (int j = 0; j < kHeadDim / 64; ++j) {
-        o[j] = __builtin_fmaf(plan.partials[slot(s) * kHeadDim + 64 * j + lane], move, o[j]);
-      }
+      for (int e = 0; e < 4; ++e) x[e] = xor_lane<kDistance>(o[e]);
+      join(xor_lane<kDistance>(base), xor_lane<kDistance>(sum), x);
+    };
+    if constexpr (!kRowEach) {
+      join_lane(std::integral_constant<int, 32>{});
+      if constexpr (kGroups == 4) join_lane(std::integral_constant<int, 16>{});
     }
-    const float inv = 1.0f / sum;
-#pragma unroll
-    for (int j = 0; j < kHeadDim / 64; ++j) {
-      a.out[(static_cast<size_t>(row) * a.num_heads + head) * kHeadDim + 64 * j + lane] =
-          float_to_elem(seen > 0 ? o[j] * inv : 0.0f);
+    if (kRowEach ? r0 + group < unit.rows : group == 0) {
+      const int token = packed_token(plan, r);
+      const bool any = unit.position + token >= 0;
+      const float inv = any ? 1.0f / sum : 0.0f;
+      uint2 words;
+      words.x = any ? pack_elems(o[0] * inv, o[1] * inv) : 0u;
+      words.y = any ? pack_elems(o[2] * inv, o[3] * inv) : 0u;
+      const size_t row = static_cast<size_t>(unit.first_row + token) * a.num_heads + unit.kv * a.group +
+                         (r - token * a.group);
+      *reinterpret_cast<uint2*>(a.out + row * kHeadDim + d) = words;
     }
   }
 }
@@ -974,8 +1127,7 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
   const int head_dim = a.view.head_dim;
   const int kv = head / a.group;
   const long long position = static_cast<long long>(a.lengths[b]) - (a.row_starts[b + 1] - row);
-  const long long held = static_cast<long long>(a.table_stride) * a.view.page_size;
-  const int limit = in_sequence < a.max_new ? static_cast<int>(max(0ll, min(position + 1, held))) : 0;
+  const int limit = in_sequence < a.max_new ? static_cast<int>(max(0ll, min(position + 1, static_cast<long long>(a.held)))) : 0;
   const int32_t* table = a.view.page_table + static_cast<size_t>(b) * a.table_stride;
   const elem_t* q = a.q + static_cast<size_t>(row) * a.q_row_stride + static_cast<size_t>(head) * head_dim;
   for (int i = lane; i < head_dim; i += 64) q_lds[wave][i] = elem_to_float(q[i]) * a.scale;
@@ -1039,65 +1191,68 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
   }
 }
 
-// The matrix-core kernels' shares: as many blocks as are resident at once.
+// A kv head's shares: all heads' together are the blocks resident at once.
 template <int kHeadDim>
-int flash_shares() {
-  constexpr int kBlocksPerUnit = kHeadDim == 64 ? 2 : 1;
-  return std::max(8, device_compute_units() * kBlocksPerUnit / 8 * 8);
+int flash_shares(int kv_heads) {
+  return std::max(1, device_compute_units() * FlashShape<kHeadDim>::kBlocks / kv_heads);
 }
 
-bool many_rows_possible(int max_new, int group) { return static_cast<long long>(max_new) * group > kFewRows; }
-
 template <int kHeadDim>
-size_t flash_workspace(int batch, int max_new, int group) {
-  const size_t rows = many_rows_possible(max_new, group) ? FlashShape<kHeadDim>::kTileRows : kFewRows;
-  const size_t starts = align_up((static_cast<size_t>(batch) + 2) * sizeof(long long), 256);
-  return starts + 2 * static_cast<size_t>(flash_shares<kHeadDim>()) * rows * (kHeadDim + 2) * sizeof(float);
+size_t flash_workspace(int max_new, int kv_heads, int group) {
+  const bool many = static_cast<long long>(max_new) * group > kFewRows;
+  const size_t rows = many ? FlashShape<kHeadDim>::kTileRows : kFewRows;
+  const size_t shares = static_cast<size_t>(flash_shares<kHeadDim>(kv_heads)) * static_cast<size_t>(kv_heads);
+  return shares * (sizeof(CutUnit) + 2 * rows * (kHeadDim + 2) * sizeof(float));
 }
 
-template <int kHeadDim, bool kMany>
-void launch_flash_kernels(const BatchAttnArgs& a, FlashPlan plan, hipStream_t s) {
+template <int kHeadDim, int kMaxRows, bool kWholePages>
+void launch_flash_kernels(const BatchAttnArgs& a, const FlashPlan& plan, hipStream_t s) {
   using Shape = FlashShape<kHeadDim>;
-  if (plan.shares > 0) {
-    batch_attention_kernel<kHeadDim, kMany><<<static_cast<unsigned>(plan.shares), Shape::kThreads, 0, s>>>(a, plan);
-    batch_attention_join_kernel<kHeadDim>
-        <<<static_cast<unsigned>(a.tokens), kJoinThreads, 0, s>>>(a, plan, kMany ? Shape::kTileRows : kFewRows);
-    return;
-  }
-  // A unit a block: at most one short tile a sequence beside the full ones.
-  const long long units = static_cast<long long>(a.tokens) / plan.tile_tokens + a.batch;
-  batch_attention_kernel<kHeadDim, kMany>
-      <<<static_cast<unsigned>(units * a.view.num_kv_heads), Shape::kThreads, 0, s>>>(a, plan);
+  constexpr int kTileRows = kMaxRows == 0 ? Shape::kTileRows : kFewRows;
+  const unsigned blocks = static_cast<unsigned>(plan.shares) * static_cast<unsigned>(a.view.num_kv_heads);
+  batch_attention_kernel<kHeadDim, kMaxRows, kWholePages><<<blocks, Shape::kThreads, 0, s>>>(a, plan);
+  if (!plan.split) return;
+  // A row is a chain of loads, so few follow each other: one time round for
+  // many rows, two for few.
+  constexpr bool kRowEach = kMaxRows == 0;
+  const dim3 join(blocks, kRowEach ? kTileRows / (4 * 256 / kHeadDim) : kTileRows / 8);
+  batch_attention_join_kernel<kHeadDim, kRowEach><<<join, kJoinThreads, 0, s>>>(a, plan, kTileRows);
 }
 
 template <int kHeadDim>
 void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
   using Shape = FlashShape<kHeadDim>;
   FlashPlan plan{};
+  const int kv_heads = a.view.num_kv_heads;
   plan.group_magic = static_cast<uint32_t>((65536 + a.group - 1) / a.group);
-  const uint32_t page = static_cast<uint32_t>(a.view.page_size);
-  plan.whole_pages = page % Shape::kLoadRows == 0 ? 1 : 0;
-  if (plan.whole_pages) {
-    // ceil(2^(31 + l) / page) with 2^l >= page: exact for keys below 2^31
-    int l = 0;
-    while ((1ull << l) < page) ++l;
-    plan.page_magic = static_cast<uint32_t>(((1ull << (31 + l)) + page - 1) / page);
-    plan.page_shift = l - 1;
-  }
   plan.tile_tokens = std::max(1, Shape::kTileRows / a.group);
+  plan.by_page = FastDivide::by(static_cast<uint32_t>(a.view.page_size));
+  plan.by_tile = FastDivide::by(static_cast<uint32_t>(plan.tile_tokens));
   plan.scale_log2e = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
-  plan.min_share = 256;
-  const bool many = many_rows_possible(a.max_new, a.group);
-  if (workspace != nullptr && workspace_bytes >= flash_workspace<kHeadDim>(a.batch, a.max_new, a.group)) {
-    plan.shares = flash_shares<kHeadDim>();
-    plan.starts = static_cast<long long*>(workspace);
-    plan.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                             align_up((static_cast<size_t>(a.batch) + 2) * sizeof(long long), 256));
-  }
-  if (many) {
-    launch_flash_kernels<kHeadDim, true>(a, plan, s);
+  plan.min_share = 4;
+  if (workspace != nullptr && workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
+    plan.split = 1;
+    plan.shares = flash_shares<kHeadDim>(kv_heads);
+    plan.cuts = static_cast<CutUnit*>(workspace);
+    plan.partials = reinterpret_cast<float*>(plan.cuts + static_cast<size_t>(plan.shares) * kv_heads);
   } else {
-    launch_flash_kernels<kHeadDim, false>(a, plan, s);
+    // A unit a block: at most one short tile a sequence beside the full ones.
+    plan.shares = a.tokens / plan.tile_tokens + a.batch;
+  }
+  plan.by_shares = FastDivide::by(static_cast<uint32_t>(plan.shares));
+  const long long most = static_cast<long long>(a.max_new) * a.group;
+  if (a.view.page_size % Shape::kLoadRows == 0) {
+    if (most <= 16) {
+      launch_flash_kernels<kHeadDim, 16, true>(a, plan, s);
+    } else if (most <= kFewRows) {
+      launch_flash_kernels<kHeadDim, 32, true>(a, plan, s);
+    } else {
+      launch_flash_kernels<kHeadDim, 0, true>(a, plan, s);
+    }
+  } else if (most <= kFewRows) {
+    launch_flash_kernels<kHeadDim, 32, false>(a, plan, s);
+  } else {
+    launch_flash_kernels<kHeadDim, 0, false>(a, plan, s);
   }
 }
 
@@ -1121,8 +1276,9 @@ using namespace lcr;
 extern "C" size_t lcr_batch_attention_workspace_bytes(int batch, int tokens, int max_new, int num_heads,
                                                       int heads_per_kv, int head_dim) {
   if (batch <= 0 || tokens <= 0 || max_new <= 0 || num_heads <= 0 || heads_per_kv <= 0) return 0;
-  if (head_dim == 64) return flash_workspace<64>(batch, max_new, heads_per_kv);
-  if (head_dim == 128) return flash_workspace<128>(batch, max_new, heads_per_kv);
+  const int kv_heads = std::max(1, num_heads / heads_per_kv);
+  if (head_dim == 64) return flash_workspace<64>(max_new, kv_heads, heads_per_kv);
+  if (head_dim == 128) return flash_workspace<128>(max_new, kv_heads, heads_per_kv);
   return 0;
 }
 
@@ -1148,8 +1304,8 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
   CAPI_CHECK(view->page_stride >= 0 && view->head_stride >= 0, "batch attention needs non-negative cache strides");
   CAPI_CHECK(q_row_stride >= static_cast<long long>(num_heads) * view->head_dim,
              "query rows of " << num_heads << " heads cannot lie " << q_row_stride << " elements apart");
-  CAPI_CHECK(static_cast<long long>(tokens) * num_heads <= INT32_MAX,
-             "batch attention takes up to 2^31 - 1 query heads in all");
+  CAPI_CHECK(tokens <= (1 << 30) && static_cast<long long>(tokens) * num_heads <= INT32_MAX,
+             "batch attention takes up to 2^30 rows and 2^31 - 1 query heads in all");
   CAPI_CHECK(out != nullptr && q != nullptr && view->keys != nullptr && view->values != nullptr &&
                  row_starts != nullptr && lengths != nullptr,
              "batch attention needs its arrays");
@@ -1157,7 +1313,8 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
              "batch attention workspace of " << workspace_bytes << " bytes has no pointer");
   CAPI_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "batch attention workspace must be 16-byte aligned");
   BatchAttnArgs a{static_cast<elem_t*>(out), static_cast<const elem_t*>(q), KvCacheView::from_c(*view), row_starts,
-                  lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride, scale};
+                  lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride,
+                  table_stride * view->page_size, scale};
   auto s = static_cast<hipStream_t>(stream);
   if (flash_takes(a)) {
     if (view->head_dim == 64) {
