@@ -1,23 +1,23 @@
 // lcr_batch_verify: drafted tokens kept or not, and the token behind them.
 //
 // Three launches:
-//   verify_stats    a slice of one row of target or draft logits a block: its
-//                   largest logit (with its index, as argmax's 64-bit key) and
-//                   the sum of exp((l - largest) / T) against it
-//   verify_residual a slice of the vocabulary of one sequence a block: the
-//                   row's slices joined, the drafts kept or not in order, and
+//   verify_stats    1024 logits of a row of target or draft a wave: the largest
+//                   and the sum of exp((l - largest) / T) against it
+//   verify_residual a slice of the vocabulary of one sequence a block: a
+//                   row's waves joined, the drafts kept or not in order, and
 //                   the slice's sum of the weights the last token is drawn
 //                   with: max(p - q, 0) in the row of the first draft not
 //                   kept, or p in the last row
 //   verify_pick     one block a sequence: the slice, then the index, at which
 //                   the running sum of those weights passes the draw
 // Every logit is read once in the first launch, and one row of each sequence
-// again in the second: bound by memory. The exponentials and sums are fp64. The
-// running sum over 128256 weights has intervals of 1e-5 and less, of which fp32
-// weights (6e-8 each, and as much in p's and q's normalisers) would give some
-// draws to a neighbour. gfx950 runs fp64 fma at the fp32 rate, so a logit's 20
-// fp64 operations stay under its 4 bytes of traffic.
+// again in the second. The exponentials and sums are fp64: the running sum over
+// 128256 weights has intervals of 1e-5 and less, of which fp32 weights (6e-8
+// each, and as much in p's and q's normalisers) would give some draws to a
+// neighbour. gfx950 runs fp64 fma at the fp32 rate, so that a logit's 13 fp64
+// operations take about as long as its 4 bytes.
 #include <algorithm>
+#include <climits>
 #include <cstdint>
 
 #include "../../../include/lcr_batch.h"
@@ -29,16 +29,20 @@ namespace {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
-constexpr int kSlice = 4096;                        // logits of a block
-constexpr int kPerThread = kSlice / kVerifyThreads;  // 16
+constexpr int kPart = 1024;                         // logits of a wave of verify_stats
+constexpr int kPerLane = kPart / 64;
+constexpr int kSlice = 4096;                        // logits of a block of verify_residual
+constexpr int kPerThread = kSlice / kVerifyThreads;
 constexpr int kPickThreads = 1024;
 constexpr int kPickPer = kSlice / kPickThreads;
 
-// A row's slice: its sum of exp((l - max) / T), and its argmax key (the maximum
-// is the key's value half).
-struct SliceStats {
+// A part of a row: its largest logit, its sum of exp((l - max) / T), and the
+// lowest index of the largest logit (only of greedy rows and where it is not
+// finite).
+struct alignas(16) PartStats {
   double sum;
-  unsigned long long key;
+  float max;
+  int index;
 };
 
 // What a row's distribution is: exp((l - max) / T) / sum where max is finite,
@@ -70,42 +74,76 @@ struct VerifyArgs {
   const float* sample_uniforms;
   int32_t* out_ids;
   int32_t* out_counts;
-  SliceStats* stats;    // [rows][2][slices]
+  PartStats* stats;     // [rows][2][parts]
   double2* totals;      // [batch][slices]: sum of max(p - q, 0), sum of p
   SequencePlan* plans;  // [batch]
   int batch;
   int rows;
   int max_draft;
   int vocab;
+  int parts;
   int slices;
   int logits_stride;
   bool vectors;         // rows on 16-byte boundaries
 };
 
-// exp(x) for x <= 0 in fp64: x = k ln2 + r (ln2 in two parts, the high one with
-// 32 significant bits so that k ln2_hi is exact), the Taylor polynomial of
-// degree 12 (|r| <= 0.347: truncated by 2e-16), scaled by 2^k. 0 below -708,
-// where the result leaves the normal range.
-__device__ __forceinline__ double exp_negative(double x) {
-  const double y = fmax(x, -708.0);
-  const double k = __builtin_rint(y * 1.44269504088896340736);
-  double r = __builtin_fma(k, -6.93147180369123816490e-01, y);
-  r = __builtin_fma(k, -1.90821492927058770002e-10, r);
-  double p = 2.08767569878680989792e-09;
-  p = __builtin_fma(p, r, 2.50521083854417187751e-08);
-  p = __builtin_fma(p, r, 2.75573192239858906526e-07);
-  p = __builtin_fma(p, r, 2.75573192239858906526e-06);
-  p = __builtin_fma(p, r, 2.48015873015873015873e-05);
-  p = __builtin_fma(p, r, 1.98412698412698412698e-04);
-  p = __builtin_fma(p, r, 1.38888888888888888889e-03);
-  p = __builtin_fma(p, r, 8.33333333333333333333e-03);
-  p = __builtin_fma(p, r, 4.16666666666666666667e-02);
-  p = __builtin_fma(p, r, 1.66666666666666666667e-01);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return x < -708.0 ? 0.0 : __builtin_ldexp(p, static_cast<int>(k));
+// 2^(j / 64), by a thread of the table's 64: 2^x on [-1/2, 1/2] by its Chebyshev
+// interpolation of degree 10 (off by 3e-16), doubled for j of 32 and more.
+constexpr int kExp2Entries = 64;
+
+__device__ __forceinline__ double exp2_entry(int j) {
+  const double x = (j < 32 ? j : j - 64) * (1.0 / 64.0);
+  double p = 7.072585949269223e-09;
+  p = __builtin_fma(p, x, 1.0208690299958306e-07);
+  p = __builtin_fma(p, x, 1.321544258792169e-06);
+  p = __builtin_fma(p, x, 1.5252657260200837e-05);
+  p = __builtin_fma(p, x, 0.0001540353044173605);
+  p = __builtin_fma(p, x, 0.0013333558230164974);
+  p = __builtin_fma(p, x, 0.009618129107606888);
+  p = __builtin_fma(p, x, 0.05550410866444772);
+  p = __builtin_fma(p, x, 0.24022650695910097);
+  p = __builtin_fma(p, x, 0.69314718055995);
+  p = __builtin_fma(p, x, 1.0);
+  return j < 32 ? p : 2.0 * p;
 }
+
+// 2^z for z <= 0 in fp64: z = k / 64 + f with k whole, by adding and taking off
+// 1.5 * 2^46 (k then also stands in the sum's low word); 2^f = 1 + f Q(f) on
+// [-1/128, 1/128], Q by Chebyshev interpolation (off by 5e-15), times the
+// table's 2^((k mod 64) / 64), and k / 64 added to the exponent. 0 below -1020,
+// where the result would leave the normal range, and for NaN (a logit of -inf at
+// an infinite temperature). A polynomial over [-1/2, 1/2] instead of the table
+// takes six more fp64 operations a logit: 48 us against 42 for the statistics
+// of 332 rows of 128256.
+// The coefficients are kept in scalar registers: left to the compiler, each is
+// moved into vector registers before each use.
+struct Exp2 {
+  double c0, c1, c2, c3;
+  const double* table;
+
+  __device__ __forceinline__ explicit Exp2(const double* table_lds)
+      : c0(0.6931471805593244), c1(0.24022650695902897), c2(0.05550419004645178), c3(0.009618138509201629),
+        table(table_lds) {
+    asm volatile("" : "+s"(c0), "+s"(c1), "+s"(c2), "+s"(c3));
+  }
+
+  __device__ __forceinline__ double operator()(double z) const {
+    const double shifted = z + 105553116266496.0;
+    const double f = z - (shifted - 105553116266496.0);
+    const uint32_t k = static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, shifted));
+    const double t = table[k & (kExp2Entries - 1)];
+    double q = __builtin_fma(c3, f, c2);
+    q = __builtin_fma(q, f, c1);
+    q = __builtin_fma(q, f, c0);
+    const unsigned long long bits = __builtin_bit_cast(unsigned long long, __builtin_fma(t * f, q, t));
+    const uint32_t high = static_cast<uint32_t>(bits >> 32) + ((k >> 6) << 20);
+    const bool inside = z >= -1020.0;
+    const uint32_t lo = inside ? static_cast<uint32_t>(bits) : 0u, hi = inside ? high : 0u;
+    return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
+  }
+};
+
+constexpr double kLog2e = 1.44269504088896340736;
 
 template <int kMask>
 __device__ __forceinline__ double xor_lane_f64(double v) {
@@ -124,40 +162,54 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return v + xor_lane_f64<1>(v);
 }
 
+// v of another lane by DPP, 0 in lanes that get none.
+template <int kControl, int kRowMask, bool kBoundZero>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const int lo = static_cast<int>(static_cast<uint32_t>(bits)), hi = static_cast<int>(static_cast<uint32_t>(bits >> 32));
+  const uint32_t l = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, lo, kControl, kRowMask, 0xF, kBoundZero));
+  const uint32_t h = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, hi, kControl, kRowMask, 0xF, kBoundZero));
+  return __builtin_bit_cast(double, (static_cast<unsigned long long>(h) << 32) | l);
+}
+
+// Inclusive sums over the wave: within rows of 16 lanes by shifts, then the
+// total of row 0 into row 1 and of row 2 into row 3, then of rows 0-1 into 2-3.
 __device__ __forceinline__ double wave_inclusive_scan_f64(double v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double other = __shfl_up(v, o, 64);
-    if (lane_id() >= o) v += other;
-  }
+  v += dpp_f64<0x111, 0xF, true>(v);   // row_shr:1
+  v += dpp_f64<0x112, 0xF, true>(v);   // row_shr:2
+  v += dpp_f64<0x114, 0xF, true>(v);   // row_shr:4
+  v += dpp_f64<0x118, 0xF, true>(v);   // row_shr:8
+  v += dpp_f64<0x142, 0xA, false>(v);  // row_bcast:15
+  v += dpp_f64<0x143, 0xC, false>(v);  // row_bcast:31
   return v;
 }
 
-__device__ __forceinline__ float key_logit(unsigned long long key) {
-  const uint32_t k = static_cast<uint32_t>(key >> 32);
-  return u32_as_f32((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+__device__ __forceinline__ double read_lane_f64(double v, int lane) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t l = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(bits)), lane));
+  const uint32_t h =
+      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(bits >> 32)), lane));
+  return __builtin_bit_cast(double, (static_cast<unsigned long long>(h) << 32) | l);
 }
 
-// A logit's key: NaN as -inf, -0 as 0 (equal logits tie on the index alone).
-__device__ __forceinline__ float clean_logit(float l) { return l != l ? -__builtin_huge_valf() : l + 0.0f; }
+// A logit as it counts: NaN as -inf, -0 as 0 (equal logits tie on the index).
+__device__ __forceinline__ float clean_logit(float l) { return fmaxf(l, -__builtin_huge_valf()) + 0.0f; }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
-// Weight of a logit against a row's maximum.
-__device__ __forceinline__ double logit_weight(float l, double max, double inv_t) {
-  return l == -__builtin_huge_valf() ? 0.0 : exp_negative((static_cast<double>(l) - max) * inv_t);
+// exp((l - max) / T) of a logit, c = log2(e) / T.
+__device__ __forceinline__ double logit_weight(const Exp2& exp2, float l, double max, double c) {
+  return exp2((static_cast<double>(l) - max) * c);
 }
 
 // Probability of index i with logit l in a row's distribution.
-__device__ __forceinline__ double probability(const RowStats& r, double inv_sum, float l, int i, double inv_t) {
-  return r.sum > 0.0 ? logit_weight(clean_logit(l), r.max, inv_t) * inv_sum : (i == r.hot ? 1.0 : 0.0);
+__device__ __forceinline__ double probability(const Exp2& exp2, const RowStats& r, double inv_sum, float l, int i,
+                                              double c) {
+  return r.sum > 0.0 ? logit_weight(exp2, clean_logit(l), r.max, c) * inv_sum : (i == r.hot ? 1.0 : 0.0);
 }
 
-// kCount logits of a row from index `first` (all of the block's at once, so
-// they arrive together); -inf behind the vocabulary's end.
-template <int kCount>
+// Four logits of a row from index `first`; -inf behind the vocabulary's end.
 __device__ __forceinline__ void load_logits(float* out, const float* row, int first, int vocab, bool vectors) {
-  static_assert(kCount == 4, "one 16-byte load");
   if (vectors && first + 4 <= vocab) {
     const float4 v = *reinterpret_cast<const float4*>(row + first);
     out[0] = v.x;
@@ -170,21 +222,41 @@ __device__ __forceinline__ void load_logits(float* out, const float* row, int fi
   }
 }
 
-// The sequence of a row (the batch's size for a row behind the last), and its
-// first row and row count. Every thread of the block reads its share of the
-// starts; a bisection would be a chain of as many loads. `lds` holds 4 ints.
-__device__ __forceinline__ int sequence_of(const VerifyArgs& a, int row, int* lds) {
-  int below = 0;
-  for (int b = threadIdx.x; b <= a.batch; b += kVerifyThreads) below += a.row_starts[b] <= row ? 1 : 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
-  if (lane_id() == 0) lds[threadIdx.x >> 6] = below;
-  __syncthreads();
-  below = 0;
-#pragma unroll
-  for (int w = 0; w < kVerifyWaves; ++w) below += lds[w];
-  __syncthreads();
-  return below - 1;
+// A row's sequence: its first row, the next sequence's, its temperature.
+struct RowPlace {
+  int start;     // -1: the row is behind the last sequence
+  int next;
+  float temperature;
+};
+
+// 64 starts and temperatures at once, each wave for itself: the last start at
+// or before the row, and the one behind it. A bisection would be a chain of
+// loads.
+__device__ __forceinline__ RowPlace place_row(const VerifyArgs& a, int row, int starts, float temperatures) {
+  RowPlace place{-1, 0, 0.0f};
+  for (int base = 0;; base += 64) {
+    const int b = base + lane_id();
+    const unsigned long long below = __ballot(b <= a.batch && starts <= row);
+    const int count = __popcll(below);
+    if (count > 0) {
+      place.start = __builtin_amdgcn_readlane(starts, count - 1);
+      place.temperature = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(temperatures), count - 1));
+    }
+    if (count < 64 || base + 64 > a.batch) {
+      // count - 1 is the last start at or before the row: batch's own says that
+      // the row is behind the last sequence
+      if (base + count > a.batch || place.start < 0) return RowPlace{-1, 0, 0.0f};
+      place.next = __builtin_amdgcn_readlane(starts, min(count, 63));
+      return place;
+    }
+    starts = a.row_starts[min(b + 64, a.batch)];
+    temperatures = a.temperatures[min(b + 64, a.batch - 1)];
+    // the next 64 may begin behind the row
+    if (__builtin_amdgcn_readfirstlane(starts) > row) {
+      place.next = __builtin_amdgcn_readfirstlane(starts);
+      return place;
+    }
+  }
 }
 
 __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
@@ -199,77 +271,108 @@ __device__ __forceinline__ double block_sum_f64(double v, double* lds) {
 }
 
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ int lds_count[kVerifyWaves];
-  __shared__ unsigned long long lds_key[16];
-  __shared__ double lds_sum[kVerifyWaves];
-  const int slice = blockIdx.x;
+  __shared__ double lds_table[kExp2Entries];
+  const int part = static_cast<int>(blockIdx.x) * kVerifyWaves + (static_cast<int>(threadIdx.x) >> 6);
   const int row = blockIdx.y;
   const bool is_draft = blockIdx.z != 0;
+  const int lane = lane_id();
   const float* logits = (is_draft ? a.draft : a.target) + static_cast<size_t>(row) * a.logits_stride;
-  float l[kPerThread];
+  // Four of each 256 neighbouring logits a lane.
+  const int first = min(part, a.parts - 1) * kPart + 4 * lane;
+  const int starts = a.row_starts[min(lane, a.batch)];
+  const float temperatures = a.temperatures[min(lane, a.batch - 1)];
+  float l[kPerLane];
   auto load = [&] {
 #pragma unroll
-    for (int j = 0; j < kPerThread / 4; ++j) {
-      load_logits<4>(l + 4 * j, logits, slice * kSlice + 4 * (j * kVerifyThreads + static_cast<int>(threadIdx.x)),
-                     a.vocab, a.vectors);
-    }
+    for (int j = 0; j < kPerLane / 4; ++j) load_logits(l + 4 * j, logits, first + 256 * j, a.vocab, a.vectors);
   };
-  // Nearly every target row counts: its logits are requested before the block
-  // knows. Every sequence has a draft row that does not.
+  // Nearly every target row counts: its logits are requested before the wave
+  // knows (and behind what it has to know, as loads return in order). Every
+  // sequence has a draft row that does not.
   if (!is_draft) load();
-  const int b = sequence_of(a, row, lds_count);
-  if (b < 0 || b >= a.batch) return;
-  const int in_sequence = row - a.row_starts[b];
-  const int drafts = min(a.row_starts[b + 1] - a.row_starts[b] - 1, a.max_draft);
-  const float t = a.temperatures[b];
+  if (threadIdx.x < kExp2Entries) lds_table[threadIdx.x] = exp2_entry(static_cast<int>(threadIdx.x));
+  __syncthreads();
+  if (part >= a.parts) return;  // the waves have no more to do with each other
+  const RowPlace place = place_row(a, row, starts, temperatures);
+  if (place.start < 0) return;
+  const int in_sequence = row - place.start;
+  const int drafts = min(place.next - place.start - 1, a.max_draft);
+  const float t = place.temperature;
   const bool greedy = !(t > 0.0f);
   if (in_sequence > drafts || (is_draft && (greedy || in_sequence == drafts))) return;
   if (is_draft) load();
-  unsigned long long key = 0;
+  float max = -__builtin_huge_valf();
 #pragma unroll
-  for (int j = 0; j < kPerThread; ++j) {
-    const int i = slice * kSlice + 4 * ((j / 4) * kVerifyThreads + static_cast<int>(threadIdx.x)) + (j & 3);
+  for (int j = 0; j < kPerLane; ++j) {
     l[j] = clean_logit(l[j]);
-    if (i < a.vocab) key = umax64(key, argmax_key(l[j], static_cast<uint32_t>(i)));
+    max = fmaxf(max, l[j]);
   }
-  key = block_max_u64(key, lds_key);
+  max = wave_max(max);
   double sum = 0.0;
-  const float max = key_logit(key);
-  if (!greedy && finite(max)) {
-    const double inv_t = 1.0 / static_cast<double>(t);
-    const double m = max;
+  int index = INT_MAX;
+  if (greedy || !finite(max)) {
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) sum += logit_weight(l[j], m, inv_t);
-    sum = block_sum_f64(sum, lds_sum);
-  }
-  if (threadIdx.x == 0) a.stats[(static_cast<size_t>(row) * 2 + (is_draft ? 1 : 0)) * a.slices + slice] = SliceStats{sum, key};
-}
-
-// A row's slices joined, by one wave; every lane gets the result.
-__device__ __forceinline__ RowStats join_slices(const SliceStats* s, int slices, double inv_t) {
-  unsigned long long key = 0;
-  for (int i = lane_id(); i < slices; i += 64) key = umax64(key, s[i].key);
-  key = wave_max_u64(key);
-  const float max = key_logit(key);
-  double sum = 0.0;
-  if (finite(max)) {
-    for (int i = lane_id(); i < slices; i += 64) {
-      const float m = key_logit(s[i].key);
-      if (finite(m)) sum += s[i].sum * exp_negative((static_cast<double>(m) - max) * inv_t);
+    for (int j = kPerLane - 1; j >= 0; --j) {
+      const int i = first + 256 * (j / 4) + (j & 3);
+      if (l[j] == max && i < a.vocab) index = i;
     }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) index = min(index, __shfl_xor(index, o, 64));
+  } else {
+    const double c = kLog2e / static_cast<double>(t);
+    const double m = max;
+    const Exp2 exp2(lds_table);
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) sum += logit_weight(exp2, l[j], m, c);
     sum = wave_sum_f64(sum);
   }
-  return RowStats{max, sum, argmax_id(key)};
+  if (lane == 0) {
+    a.stats[(static_cast<size_t>(row) * 2 + (is_draft ? 1 : 0)) * a.parts + part] = PartStats{sum, max, index};
+  }
+}
+
+// A row's parts joined, by one wave; every lane gets the result.
+__device__ __forceinline__ RowStats join_row(const Exp2& exp2, const PartStats* stats, int parts, double c) {
+  // Two parts a lane at once, which is all of a vocabulary up to 131072.
+  PartStats s[2];
+  float max = -__builtin_huge_valf();
+  double sum = 0.0;
+  int index = INT_MAX;
+  for (int base = 0; base < parts; base += 128) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = base + 64 * k + lane_id();
+      s[k] = i < parts ? stats[i] : PartStats{0.0, -__builtin_huge_valf(), INT_MAX};
+    }
+    const float to = fmaxf(max, wave_max(fmaxf(s[0].max, s[1].max)));
+    index = max == to ? index : INT_MAX;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) index = s[k].max == to ? min(index, s[k].index) : index;
+    if (finite(to)) {
+      if (max != to) sum = finite(max) ? sum * exp2((static_cast<double>(max) - to) * c) : 0.0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (finite(s[k].max)) sum += s[k].sum * exp2((static_cast<double>(s[k].max) - to) * c);
+      }
+    }
+    max = to;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) index = min(index, __shfl_xor(index, o, 64));
+  return RowStats{max, finite(max) ? wave_sum_f64(sum) : 0.0, index};
 }
 
 __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyArgs a) {
-  __shared__ int shared_kept;
-  __shared__ RowStats shared_target, shared_draft;
-  __shared__ int shared_subtract;
+  __shared__ int lds_stop[kVerifyWaves];
+  __shared__ RowStats lds_target[kVerifyWaves], lds_draft[kVerifyWaves];
   __shared__ double lds_sum[kVerifyWaves];
+  __shared__ double lds_table[kExp2Entries];
   const int slice = blockIdx.x;
   const int b = blockIdx.y;
   const int lane = lane_id();
+  const int wave = static_cast<int>(threadIdx.x) >> 6;
+  if (threadIdx.x < kExp2Entries) lds_table[threadIdx.x] = exp2_entry(static_cast<int>(threadIdx.x));
+  __syncthreads();
   const int first = a.row_starts[b];
   const int count = a.row_starts[b + 1] - first;
   SequencePlan& plan = a.plans[b];
@@ -281,63 +384,75 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyA
   const int drafts = min(count - 1, a.max_draft);
   const float t = a.temperatures[b];
   const bool greedy = !(t > 0.0f);
-  const double inv_t = greedy ? 0.0 : 1.0 / static_cast<double>(t);
-  // Drafts kept, in order, by wave 0.
-  if (threadIdx.x < 64) {
-    int kept = 0;
-    RowStats target{}, draft{};
-    for (;; ++kept) {
-      const int row = first + kept;
-      target = join_slices(a.stats + static_cast<size_t>(row) * 2 * a.slices, a.slices, inv_t);
-      if (kept == drafts) break;
-      const int x = a.draft_ids[row];
-      if (greedy) {
-        if (x != target.hot) break;
-        continue;
-      }
-      draft = RowStats{0.0, 0.0, x};
-      if (a.draft != nullptr) {
-        const RowStats d = join_slices(a.stats + (static_cast<size_t>(row) * 2 + 1) * a.slices, a.slices, inv_t);
+  const double c = greedy ? 0.0 : kLog2e / static_cast<double>(t);
+  const Exp2 exp2(lds_table);
+  // The first row that stops: its draft is not kept, or it is the last. A wave
+  // a row, so that rows do not wait for each other's reads.
+  int kept = 0;
+  int at = -1;
+  for (int base = 0; at < 0; base += kVerifyWaves) {
+    const int i = base + wave;
+    bool stop = true;
+    if (i <= drafts) {
+      const int row = first + i;
+      const PartStats* stats = a.stats + static_cast<size_t>(row) * 2 * a.parts;
+      const bool sampled = i < drafts && !greedy;
+      const int x = i < drafts ? a.draft_ids[row] : 0;
+      const bool inside = x >= 0 && x < a.vocab;
+      const size_t place = static_cast<size_t>(row) * a.logits_stride + (inside ? x : 0);
+      const float target_logit = sampled ? a.target[place] : 0.0f;
+      const float draft_logit = sampled && a.draft != nullptr ? a.draft[place] : 0.0f;
+      const float u = sampled ? a.accept_uniforms[row] : 0.0f;
+      RowStats draft{0.0, 0.0, x};
+      if (sampled && a.draft != nullptr) {
+        const RowStats d = join_row(exp2, stats + a.parts, a.parts, c);
         draft.max = d.max;
         draft.sum = d.sum;
       }
-      if (x < 0 || x >= a.vocab) break;
-      const size_t at = static_cast<size_t>(row) * a.logits_stride + x;
-      const double p = probability(target, 1.0 / target.sum, a.target[at], x, inv_t);
-      const double q = draft.sum > 0.0 ? probability(draft, 1.0 / draft.sum, a.draft[at], x, inv_t) : 1.0;
-      if (!(static_cast<double>(a.accept_uniforms[row]) * q < p)) break;
+      const RowStats target = join_row(exp2, stats, a.parts, c);
+      if (sampled) {
+        const double p = probability(exp2, target, 1.0 / target.sum, target_logit, x, c);
+        const double q = draft.sum > 0.0 ? probability(exp2, draft, 1.0 / draft.sum, draft_logit, x, c) : 1.0;
+        stop = !(inside && static_cast<double>(u) * q < p);
+      } else {
+        stop = i == drafts || x != target.hot;
+      }
+      if (lane == 0) {
+        lds_target[wave] = target;
+        lds_draft[wave] = draft;
+      }
     }
-    if (lane == 0) {
-      shared_kept = kept;
-      shared_target = target;
-      shared_draft = draft;
-      shared_subtract = kept < drafts ? 1 : 0;
+    if (lane == 0) lds_stop[wave] = stop ? 1 : 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = kVerifyWaves - 1; w >= 0; --w) {
+      if (lds_stop[w] != 0) at = w;
     }
+    kept = base + at;
+    if (at < 0) __syncthreads();  // read before the next rows are written
   }
-  __syncthreads();
-  const int kept = shared_kept;
-  const RowStats target = shared_target, draft = shared_draft;
-  const int subtract = shared_subtract;
+  const RowStats target = lds_target[at], draft = lds_draft[at];
+  const int subtract = kept < drafts ? 1 : 0;
   const int row = first + kept;
   if (slice == 0 && threadIdx.x == 0) {
     plan = SequencePlan{kept, row, greedy ? target.hot : -1, subtract, target, draft};
   }
   if (greedy) return;
-  const size_t at = static_cast<size_t>(row) * a.logits_stride;
+  const size_t row_at = static_cast<size_t>(row) * a.logits_stride;
   const double inv_p = 1.0 / target.sum, inv_q = 1.0 / draft.sum;
   double rest = 0.0, whole = 0.0;
 #pragma unroll
   for (int j = 0; j < kPerThread / 4; ++j) {
     const int i0 = slice * kSlice + 4 * (j * kVerifyThreads + static_cast<int>(threadIdx.x));
     float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    load_logits<4>(lp, a.target + at, i0, a.vocab, a.vectors);
-    if (subtract && draft.sum > 0.0) load_logits<4>(lq, a.draft + at, i0, a.vocab, a.vectors);
+    load_logits(lp, a.target + row_at, i0, a.vocab, a.vectors);
+    if (subtract && draft.sum > 0.0) load_logits(lq, a.draft + row_at, i0, a.vocab, a.vectors);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (i0 + e >= a.vocab) continue;
-      const double p = probability(target, inv_p, lp[e], i0 + e, inv_t);
+      const double p = probability(exp2, target, inv_p, lp[e], i0 + e, c);
       whole += p;
-      if (subtract) rest += fmax(p - probability(draft, inv_q, lq[e], i0 + e, inv_t), 0.0);
+      if (subtract) rest += fmax(p - probability(exp2, draft, inv_q, lq[e], i0 + e, c), 0.0);
     }
   }
   rest = block_sum_f64(rest, lds_sum);
@@ -350,6 +465,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   __shared__ double shared_before, shared_goal;
   __shared__ double wave_total[kPickThreads / 64];
   __shared__ int wave_first[kPickThreads / 64], wave_last[kPickThreads / 64];
+  __shared__ double lds_table[kExp2Entries];
   const int b = blockIdx.x;
   const int lane = lane_id();
   const int wave = static_cast<int>(threadIdx.x) >> 6;
@@ -365,6 +481,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
     if (plan.row >= 0 && plan.greedy_id >= 0) ids[kept] = plan.greedy_id;
   }
   if (plan.row < 0 || plan.greedy_id >= 0) return;  // the whole block
+  if (wave == 1) lds_table[lane] = exp2_entry(lane);
   // The slice: the first whose running sum passes the draw. Rounding may leave
   // none: then the last slice with a weight.
   if (wave == 0) {
@@ -377,7 +494,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
     for (int base = 0; base < a.slices; base += 64) {
       const int s = base + lane;
       const double v = s < a.slices ? (subtract ? totals[s].x : totals[s].y) : 0.0;
-      whole += __shfl(wave_inclusive_scan_f64(v), 63, 64);
+      whole += read_lane_f64(wave_inclusive_scan_f64(v), 63);
     }
     const double goal = static_cast<double>(a.sample_uniforms[b]) * whole;
     double before = 0.0, last_before = 0.0;
@@ -391,10 +508,10 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
       const int pick = hit != 0 ? __ffsll(hit) - 1 : (weighty != 0 ? 63 - __clzll(weighty) : -1);
       if (pick >= 0) {
         last = base + pick;
-        last_before = before + __shfl(incl - v, pick, 64);
+        last_before = before + read_lane_f64(incl - v, pick);
         if (hit != 0) found = last;
       }
-      before += __shfl(incl, 63, 64);
+      before += read_lane_f64(incl, 63);
     }
     if (lane == 0) {
       shared_slice = last;
@@ -406,15 +523,16 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   __syncthreads();
   const int slice = shared_slice;
   const bool subtract = shared_subtract != 0;
-  const double inv_t = 1.0 / static_cast<double>(a.temperatures[b]);
+  const double c = kLog2e / static_cast<double>(a.temperatures[b]);
+  const Exp2 exp2(lds_table);
   const double inv_p = 1.0 / plan.target.sum, inv_q = 1.0 / plan.draft.sum;
   const size_t at = static_cast<size_t>(plan.row) * a.logits_stride;
   // Four neighbouring weights a thread, their running sum within the slice.
   static_assert(kPickPer == 4, "one 16-byte load a thread");
   const int i0 = slice * kSlice + 4 * static_cast<int>(threadIdx.x);
   float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  load_logits<4>(lp, a.target + at, i0, a.vocab, a.vectors);
-  if (subtract && plan.draft.sum > 0.0) load_logits<4>(lq, a.draft + at, i0, a.vocab, a.vectors);
+  load_logits(lp, a.target + at, i0, a.vocab, a.vectors);
+  if (subtract && plan.draft.sum > 0.0) load_logits(lq, a.draft + at, i0, a.vocab, a.vectors);
   double run[4];
   double sum = 0.0;
   bool weighty[4];
@@ -422,8 +540,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   for (int e = 0; e < 4; ++e) {
     double w = 0.0;
     if (i0 + e < a.vocab) {
-      w = probability(plan.target, inv_p, lp[e], i0 + e, inv_t);
-      if (subtract) w = fmax(w - probability(plan.draft, inv_q, lq[e], i0 + e, inv_t), 0.0);
+      w = probability(exp2, plan.target, inv_p, lp[e], i0 + e, c);
+      if (subtract) w = fmax(w - probability(exp2, plan.draft, inv_q, lq[e], i0 + e, c), 0.0);
     }
     sum += w;
     run[e] = sum;
@@ -462,6 +580,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a)
   }
 }
 
+int parts_for(int vocab) { return (vocab + kPart - 1) / kPart; }
 int slices_for(int vocab) { return (vocab + kSlice - 1) / kSlice; }
 
 struct VerifyLayout {
@@ -471,7 +590,7 @@ struct VerifyLayout {
 VerifyLayout layout_for(int batch, int rows, int vocab) {
   const size_t slices = static_cast<size_t>(slices_for(vocab));
   VerifyLayout l;
-  l.totals_at = static_cast<size_t>(rows) * 2 * slices * sizeof(SliceStats);
+  l.totals_at = static_cast<size_t>(rows) * 2 * static_cast<size_t>(parts_for(vocab)) * sizeof(PartStats);
   l.plans_at = l.totals_at + static_cast<size_t>(batch) * slices * sizeof(double2);
   l.bytes = l.plans_at + static_cast<size_t>(batch) * sizeof(SequencePlan);
   return l;
@@ -521,20 +640,22 @@ extern "C" int lcr_batch_verify(int32_t* out_ids, int32_t* out_counts, const flo
   a.sample_uniforms = sample_uniforms;
   a.out_ids = out_ids;
   a.out_counts = out_counts;
-  a.stats = reinterpret_cast<SliceStats*>(ws);
+  a.stats = reinterpret_cast<PartStats*>(ws);
   a.totals = reinterpret_cast<double2*>(ws + layout.totals_at);
   a.plans = reinterpret_cast<SequencePlan*>(ws + layout.plans_at);
   a.batch = batch;
   a.rows = rows;
   a.max_draft = max_draft;
   a.vocab = vocab;
+  a.parts = parts_for(vocab);
   a.slices = slices_for(vocab);
   a.logits_stride = logits_stride;
   a.vectors = logits_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(target_logits) & 15u) == 0 &&
               (reinterpret_cast<uintptr_t>(draft_logits) & 15u) == 0;
   auto s = static_cast<hipStream_t>(stream);
   if (rows > 0) {
-    const dim3 grid(static_cast<unsigned>(a.slices), static_cast<unsigned>(rows), a.draft != nullptr ? 2u : 1u);
+    const dim3 grid(static_cast<unsigned>((a.parts + kVerifyWaves - 1) / kVerifyWaves), static_cast<unsigned>(rows),
+                    a.draft != nullptr ? 2u : 1u);
     verify_stats_kernel<<<grid, kVerifyThreads, 0, s>>>(a);
     CAPI_LAUNCHED();
   }
