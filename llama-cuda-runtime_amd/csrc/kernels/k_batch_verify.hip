@@ -1,21 +1,24 @@
 // lcr_batch_verify: drafted tokens kept or not, and the token behind them.
 //
-// Three launches:
-//   verify_stats    1024 logits of a row of target or draft a wave: the largest
-//                   and the sum of exp((l - largest) / T) against it
-//   verify_residual a slice of the vocabulary of one sequence a block: a
-//                   row's waves joined, the drafts kept or not in order, and
-//                   the slice's sum of the weights the last token is drawn
-//                   with: max(p - q, 0) in the row of the first draft not
-//                   kept, or p in the last row
-//   verify_pick     one block a sequence: the slice, then the index, at which
-//                   the running sum of those weights passes the draw
-// Every logit is read once in the first launch, and one row of each sequence
+// Two launches:
+//   verify_stats  1024 logits (a part) of a row of target or draft a wave: the
+//                 largest and the sum of exp((l - largest) / T) against it
+//   verify_draw   four parts of the vocabulary of one sequence a block: the
+//                 parts of its rows joined, the drafts kept or not in order, and
+//                 the id behind them. Behind drafts that were all kept it is
+//                 drawn from the last row's p, whose parts' sums are there
+//                 already: the first block finds the part, then the index, at
+//                 which the running sum passes the draw. Behind a draft not
+//                 kept, the blocks sum max(p - q, 0) over their parts of its
+//                 row, and the block whose sum arrives last finds them.
+// Every logit is read once in the first launch, and the row of a draft not kept
 // again in the second. The exponentials and sums are fp64: the running sum over
 // 128256 weights has intervals of 1e-5 and less, of which fp32 weights (6e-8
 // each, and as much in p's and q's normalisers) would give some draws to a
 // neighbour. gfx950 runs fp64 fma at the fp32 rate, so that a logit's 13 fp64
 // operations take about as long as its 4 bytes.
+// Which block arrives last decides who computes, not what: all sums have a fixed
+// order.
 #include <algorithm>
 #include <climits>
 #include <cstdint>
@@ -29,12 +32,8 @@ namespace {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
-constexpr int kPart = 1024;                         // logits of a wave of verify_stats
+constexpr int kPart = 1024;                         // logits of a wave
 constexpr int kPerLane = kPart / 64;
-constexpr int kSlice = 4096;                        // logits of a block of verify_residual
-constexpr int kPerThread = kSlice / kVerifyThreads;
-constexpr int kPickThreads = 1024;
-constexpr int kPickPer = kSlice / kPickThreads;
 
 // A part of a row: its largest logit, its sum of exp((l - max) / T), and the
 // lowest index of the largest logit (only of greedy rows and where it is not
@@ -53,17 +52,6 @@ struct RowStats {
   int hot;
 };
 
-// What verify_pick needs of a sequence: `kept` drafts, the row and its
-// distribution, and whether there is a draft's row to take off.
-struct SequencePlan {
-  int kept;
-  int row;           // -1: the sequence has no rows
-  int greedy_id;     // >= 0: the id itself
-  int subtract;      // 1: weights max(p - q, 0)
-  RowStats target;
-  RowStats draft;    // sum = 0: one at the index `hot`
-};
-
 struct VerifyArgs {
   const float* target;
   const float* draft;
@@ -75,14 +63,13 @@ struct VerifyArgs {
   int32_t* out_ids;
   int32_t* out_counts;
   PartStats* stats;     // [rows][2][parts]
-  double2* totals;      // [batch][slices]: sum of max(p - q, 0), sum of p
-  SequencePlan* plans;  // [batch]
+  double* totals;       // [batch][parts]: sums of max(p - q, 0)
+  int* arrived;         // [batch] parts of `totals` that are there
   int batch;
   int rows;
   int max_draft;
   int vocab;
   int parts;
-  int slices;
   int logits_stride;
   bool vectors;         // rows on 16-byte boundaries
 };
@@ -259,17 +246,6 @@ __device__ __forceinline__ RowPlace place_row(const VerifyArgs& a, int row, int 
   }
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double* lds) {
-  v = wave_sum_f64(v);
-  if (lane_id() == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double sum = lds[0];
-#pragma unroll
-  for (int w = 1; w < kVerifyWaves; ++w) sum += lds[w];
-  __syncthreads();
-  return sum;
-}
-
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
   __shared__ double lds_table[kExp2Entries];
   const int part = static_cast<int>(blockIdx.x) * kVerifyWaves + (static_cast<int>(threadIdx.x) >> 6);
@@ -279,6 +255,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
   const float* logits = (is_draft ? a.draft : a.target) + static_cast<size_t>(row) * a.logits_stride;
   // Four of each 256 neighbouring logits a lane.
   const int first = min(part, a.parts - 1) * kPart + 4 * lane;
+  if (blockIdx.x == 0 && row == 0 && !is_draft) {
+    for (int b = threadIdx.x; b < a.batch; b += kVerifyThreads) a.arrived[b] = 0;
+  }
   const int starts = a.row_starts[min(lane, a.batch)];
   const float temperatures = a.temperatures[min(lane, a.batch - 1)];
   float l[kPerLane];
@@ -362,30 +341,149 @@ __device__ __forceinline__ RowStats join_row(const Exp2& exp2, const PartStats* 
   return RowStats{max, finite(max) ? wave_sum_f64(sum) : 0.0, index};
 }
 
-__global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyArgs a) {
-  __shared__ int lds_stop[kVerifyWaves];
-  __shared__ RowStats lds_target[kVerifyWaves], lds_draft[kVerifyWaves];
-  __shared__ double lds_sum[kVerifyWaves];
-  __shared__ double lds_table[kExp2Entries];
-  const int slice = blockIdx.x;
+struct DrawLds {
+  int stop[kVerifyWaves];
+  RowStats target[kVerifyWaves], draft[kVerifyWaves];
+  double table[kExp2Entries];
+  int last;          // this block's sum was the last
+  int part;          // of the drawn index; -1: no part has a weight
+  double before;     // running sum before that part
+  double goal;
+  double wave_total[kVerifyWaves];
+  int wave_first[kVerifyWaves], wave_last[kVerifyWaves];
+};
+
+// The first index whose running sum of weights passes u times their whole sum,
+// by the block: the part by its parts' sums total_of(part), then the index by
+// the weights weight_of(logits of target, logits of draft, index) in it.
+// Rounding may leave no sum past the goal: then the last index with a weight.
+// -1 where there is no weight.
+template <typename TotalOf, typename WeightOf>
+__device__ __forceinline__ int draw_index(DrawLds& lds, const VerifyArgs& a, float u, const float* target_row,
+                                          const float* draft_row, TotalOf total_of, WeightOf weight_of) {
+  const int lane = lane_id();
+  const int wave = static_cast<int>(threadIdx.x) >> 6;
+  if (wave == 0) {
+    double whole = 0.0;
+    for (int base = 0; base < a.parts; base += 64) {
+      const double v = base + lane < a.parts ? total_of(base + lane) : 0.0;
+      whole += read_lane_f64(wave_inclusive_scan_f64(v), 63);
+    }
+    const double goal = static_cast<double>(u) * whole;
+    double before = 0.0, part_before = 0.0;
+    int part = -1;
+    for (int base = 0, hit = 0; base < a.parts && hit == 0; base += 64) {
+      const double v = base + lane < a.parts ? total_of(base + lane) : 0.0;
+      const double incl = wave_inclusive_scan_f64(v);
+      const unsigned long long past = __ballot(v > 0.0 && before + incl > goal);
+      const unsigned long long weighty = __ballot(v > 0.0);
+      const int at = past != 0 ? __ffsll(past) - 1 : (weighty != 0 ? 63 - __clzll(weighty) : -1);
+      if (at >= 0) {
+        part = base + at;
+        part_before = before + read_lane_f64(incl - v, at);
+        hit = past != 0 ? 1 : 0;
+      }
+      before += read_lane_f64(incl, 63);
+    }
+    if (lane == 0) {
+      lds.part = part;
+      lds.before = part_before;
+      lds.goal = goal;
+    }
+  }
+  __syncthreads();
+  const int part = lds.part;
+  if (part < 0) return -1;
+  // Four neighbouring weights a thread.
+  static_assert(kPart == 4 * kVerifyThreads, "one 16-byte load a thread");
+  const int i0 = part * kPart + 4 * static_cast<int>(threadIdx.x);
+  float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  load_logits(lp, target_row, i0, a.vocab, a.vectors);
+  if (draft_row != nullptr) load_logits(lq, draft_row, i0, a.vocab, a.vectors);
+  double run[4];
+  double sum = 0.0;
+  bool weighty[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const double w = i0 + e < a.vocab ? weight_of(lp[e], lq[e], i0 + e) : 0.0;
+    sum += w;
+    run[e] = sum;
+    weighty[e] = w > 0.0;
+  }
+  const double incl = wave_inclusive_scan_f64(sum);
+  if (lane == 63) lds.wave_total[wave] = incl;
+  __syncthreads();
+  double before = lds.before;
+  for (int w = 0; w < wave; ++w) before += lds.wave_total[w];
+  before += incl - sum;
+  int first = INT_MAX, last = -1;
+#pragma unroll
+  for (int e = 3; e >= 0; --e) {
+    if (weighty[e]) {
+      last = max(last, i0 + e);
+      if (before + run[e] > lds.goal) first = i0 + e;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    first = min(first, __shfl_xor(first, o, 64));
+    last = max(last, __shfl_xor(last, o, 64));
+  }
+  if (lane == 0) {
+    lds.wave_first[wave] = first;
+    lds.wave_last[wave] = last;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kVerifyWaves; ++w) {
+    first = min(first, lds.wave_first[w]);
+    last = max(last, lds.wave_last[w]);
+  }
+  __syncthreads();  // `lds` may be drawn with again
+  return first != INT_MAX ? first : max(last, 0);
+}
+
+// A sum handed to other blocks of the grid. Atomic accesses of device scope go
+// past the caches of one XCD; that the exchange has returned says that its value
+// is where they all look, so that a count taken after it counts it. (Releasing
+// and acquiring with the count instead writes back and drops the whole L2, once
+// a block: 68 us against 24 for 64
+// sequences of 128256 logits.)
+__device__ __forceinline__ void publish(double* at, double value) {
+  const unsigned long long before =
+      __hip_atomic_exchange(reinterpret_cast<unsigned long long*>(at), __builtin_bit_cast(unsigned long long, value),
+                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("" : : "v"(before) : "memory");  // waits for it
+}
+__device__ __forceinline__ double published(const double* at) {
+  return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(at), __ATOMIC_RELAXED,
+                                                      __HIP_MEMORY_SCOPE_AGENT));
+}
+
+__global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ DrawLds lds;
   const int b = blockIdx.y;
   const int lane = lane_id();
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  if (threadIdx.x < kExp2Entries) lds_table[threadIdx.x] = exp2_entry(static_cast<int>(threadIdx.x));
-  __syncthreads();
   const int first = a.row_starts[b];
   const int count = a.row_starts[b + 1] - first;
-  SequencePlan& plan = a.plans[b];
+  const float t = a.temperatures[b];
+  if (threadIdx.x < kExp2Entries) lds.table[threadIdx.x] = exp2_entry(static_cast<int>(threadIdx.x));
+  if (threadIdx.x == 0) lds.last = 0;
+  __syncthreads();
+  int32_t* ids = a.out_ids + static_cast<size_t>(b) * (a.max_draft + 1);
   // Rows of a table that is no ascending list of rows are not read.
   if (count <= 0 || first < 0 || first > a.rows - count) {
-    if (slice == 0 && threadIdx.x == 0) plan.row = -1;
+    if (blockIdx.x == 0) {
+      for (int i = threadIdx.x; i <= a.max_draft; i += kVerifyThreads) ids[i] = -1;
+      if (threadIdx.x == 0) a.out_counts[b] = 0;
+    }
     return;
   }
   const int drafts = min(count - 1, a.max_draft);
-  const float t = a.temperatures[b];
   const bool greedy = !(t > 0.0f);
   const double c = greedy ? 0.0 : kLog2e / static_cast<double>(t);
-  const Exp2 exp2(lds_table);
+  const Exp2 exp2(lds.table);
   // The first row that stops: its draft is not kept, or it is the last. A wave
   // a row, so that rows do not wait for each other's reads.
   int kept = 0;
@@ -398,18 +496,18 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyA
       const PartStats* stats = a.stats + static_cast<size_t>(row) * 2 * a.parts;
       const bool sampled = i < drafts && !greedy;
       const int x = i < drafts ? a.draft_ids[row] : 0;
+      const float u = sampled ? a.accept_uniforms[row] : 0.0f;
       const bool inside = x >= 0 && x < a.vocab;
       const size_t place = static_cast<size_t>(row) * a.logits_stride + (inside ? x : 0);
       const float target_logit = sampled ? a.target[place] : 0.0f;
       const float draft_logit = sampled && a.draft != nullptr ? a.draft[place] : 0.0f;
-      const float u = sampled ? a.accept_uniforms[row] : 0.0f;
+      const RowStats target = join_row(exp2, stats, a.parts, c);
       RowStats draft{0.0, 0.0, x};
       if (sampled && a.draft != nullptr) {
         const RowStats d = join_row(exp2, stats + a.parts, a.parts, c);
         draft.max = d.max;
         draft.sum = d.sum;
       }
-      const RowStats target = join_row(exp2, stats, a.parts, c);
       if (sampled) {
         const double p = probability(exp2, target, 1.0 / target.sum, target_logit, x, c);
         const double q = draft.sum > 0.0 ? probability(exp2, draft, 1.0 / draft.sum, draft_logit, x, c) : 1.0;
@@ -418,181 +516,91 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyA
         stop = i == drafts || x != target.hot;
       }
       if (lane == 0) {
-        lds_target[wave] = target;
-        lds_draft[wave] = draft;
+        lds.target[wave] = target;
+        lds.draft[wave] = draft;
       }
     }
-    if (lane == 0) lds_stop[wave] = stop ? 1 : 0;
+    if (lane == 0) lds.stop[wave] = stop ? 1 : 0;
     __syncthreads();
 #pragma unroll
     for (int w = kVerifyWaves - 1; w >= 0; --w) {
-      if (lds_stop[w] != 0) at = w;
+      if (lds.stop[w] != 0) at = w;
     }
     kept = base + at;
     if (at < 0) __syncthreads();  // read before the next rows are written
   }
-  const RowStats target = lds_target[at], draft = lds_draft[at];
-  const int subtract = kept < drafts ? 1 : 0;
+  const RowStats target = lds.target[at], draft = lds.draft[at];
+  const bool subtract = kept < drafts && !greedy;
+  if (!subtract && blockIdx.x != 0) return;
   const int row = first + kept;
-  if (slice == 0 && threadIdx.x == 0) {
-    plan = SequencePlan{kept, row, greedy ? target.hot : -1, subtract, target, draft};
-  }
-  if (greedy) return;
-  const size_t row_at = static_cast<size_t>(row) * a.logits_stride;
-  const double inv_p = 1.0 / target.sum, inv_q = 1.0 / draft.sum;
-  double rest = 0.0, whole = 0.0;
+  const float* target_row = a.target + static_cast<size_t>(row) * a.logits_stride;
+  const float* draft_row =
+      subtract && draft.sum > 0.0 ? a.draft + static_cast<size_t>(row) * a.logits_stride : nullptr;
+  int id = -1;
+  if (subtract) {
+    const double inv_p = 1.0 / target.sum, inv_q = 1.0 / draft.sum;
+    auto weight_of = [&](float p, float q, int i) {
+      return fmax(probability(exp2, target, inv_p, p, i, c) - probability(exp2, draft, inv_q, q, i, c), 0.0);
+    };
+    double* totals = a.totals + static_cast<size_t>(b) * a.parts;
+    const int part = static_cast<int>(blockIdx.x) * kVerifyWaves + wave;
+    if (part < a.parts) {
+      double rest = 0.0;
 #pragma unroll
-  for (int j = 0; j < kPerThread / 4; ++j) {
-    const int i0 = slice * kSlice + 4 * (j * kVerifyThreads + static_cast<int>(threadIdx.x));
-    float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    load_logits(lp, a.target + row_at, i0, a.vocab, a.vectors);
-    if (subtract && draft.sum > 0.0) load_logits(lq, a.draft + row_at, i0, a.vocab, a.vectors);
+      for (int j = 0; j < kPerLane / 4; ++j) {
+        const int i0 = part * kPart + 256 * j + 4 * lane;
+        float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        load_logits(lp, target_row, i0, a.vocab, a.vectors);
+        if (draft_row != nullptr) load_logits(lq, draft_row, i0, a.vocab, a.vectors);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (i0 + e >= a.vocab) continue;
-      const double p = probability(exp2, target, inv_p, lp[e], i0 + e, c);
-      whole += p;
-      if (subtract) rest += fmax(p - probability(exp2, draft, inv_q, lq[e], i0 + e, c), 0.0);
-    }
-  }
-  rest = block_sum_f64(rest, lds_sum);
-  whole = block_sum_f64(whole, lds_sum);
-  if (threadIdx.x == 0) a.totals[static_cast<size_t>(b) * a.slices + slice] = make_double2(rest, whole);
-}
-
-__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ int shared_slice, shared_subtract;
-  __shared__ double shared_before, shared_goal;
-  __shared__ double wave_total[kPickThreads / 64];
-  __shared__ int wave_first[kPickThreads / 64], wave_last[kPickThreads / 64];
-  __shared__ double lds_table[kExp2Entries];
-  const int b = blockIdx.x;
-  const int lane = lane_id();
-  const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const SequencePlan plan = a.plans[b];
-  int32_t* ids = a.out_ids + static_cast<size_t>(b) * (a.max_draft + 1);
-  const int kept = plan.row < 0 ? 0 : plan.kept;
-  // The kept drafts, and -1 behind the drawn token, which is written last.
-  for (int i = threadIdx.x; i <= a.max_draft; i += kPickThreads) {
-    if (plan.row < 0 || i != kept) ids[i] = i < kept ? a.draft_ids[plan.row - kept + i] : -1;
-  }
-  if (threadIdx.x == 0) {
-    a.out_counts[b] = plan.row < 0 ? 0 : kept + 1;
-    if (plan.row >= 0 && plan.greedy_id >= 0) ids[kept] = plan.greedy_id;
-  }
-  if (plan.row < 0 || plan.greedy_id >= 0) return;  // the whole block
-  if (wave == 1) lds_table[lane] = exp2_entry(lane);
-  // The slice: the first whose running sum passes the draw. Rounding may leave
-  // none: then the last slice with a weight.
-  if (wave == 0) {
-    const double2* totals = a.totals + static_cast<size_t>(b) * a.slices;
-    double rest = 0.0;
-    for (int s = lane; s < a.slices; s += 64) rest += totals[s].x;
-    rest = wave_sum_f64(rest);
-    const bool subtract = plan.subtract != 0 && rest > 0.0;
-    double whole = 0.0;
-    for (int base = 0; base < a.slices; base += 64) {
-      const int s = base + lane;
-      const double v = s < a.slices ? (subtract ? totals[s].x : totals[s].y) : 0.0;
-      whole += read_lane_f64(wave_inclusive_scan_f64(v), 63);
-    }
-    const double goal = static_cast<double>(a.sample_uniforms[b]) * whole;
-    double before = 0.0, last_before = 0.0;
-    int found = -1, last = 0;
-    for (int base = 0; base < a.slices && found < 0; base += 64) {
-      const int s = base + lane;
-      const double v = s < a.slices ? (subtract ? totals[s].x : totals[s].y) : 0.0;
-      const double incl = wave_inclusive_scan_f64(v);
-      const unsigned long long weighty = __ballot(v > 0.0);
-      const unsigned long long hit = __ballot(v > 0.0 && before + incl > goal);
-      const int pick = hit != 0 ? __ffsll(hit) - 1 : (weighty != 0 ? 63 - __clzll(weighty) : -1);
-      if (pick >= 0) {
-        last = base + pick;
-        last_before = before + read_lane_f64(incl - v, pick);
-        if (hit != 0) found = last;
+        for (int e = 0; e < 4; ++e) {
+          if (i0 + e < a.vocab) rest += weight_of(lp[e], lq[e], i0 + e);
+        }
       }
-      before += read_lane_f64(incl, 63);
+      rest = wave_sum_f64(rest);
+      if (lane == 0) publish(totals + part, rest);
     }
-    if (lane == 0) {
-      shared_slice = last;
-      shared_before = last_before;
-      shared_goal = goal;
-      shared_subtract = subtract ? 1 : 0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int before = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (before == static_cast<int>(gridDim.x) - 1) lds.last = 1;
     }
+    __syncthreads();
+    if (lds.last == 0) return;
+    id = draw_index(lds, a, a.sample_uniforms[b], target_row, draft_row, [&](int i) { return published(totals + i); }, weight_of);
   }
-  __syncthreads();
-  const int slice = shared_slice;
-  const bool subtract = shared_subtract != 0;
-  const double c = kLog2e / static_cast<double>(a.temperatures[b]);
-  const Exp2 exp2(lds_table);
-  const double inv_p = 1.0 / plan.target.sum, inv_q = 1.0 / plan.draft.sum;
-  const size_t at = static_cast<size_t>(plan.row) * a.logits_stride;
-  // Four neighbouring weights a thread, their running sum within the slice.
-  static_assert(kPickPer == 4, "one 16-byte load a thread");
-  const int i0 = slice * kSlice + 4 * static_cast<int>(threadIdx.x);
-  float lp[4], lq[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  load_logits(lp, a.target + at, i0, a.vocab, a.vectors);
-  if (subtract && plan.draft.sum > 0.0) load_logits(lq, a.draft + at, i0, a.vocab, a.vectors);
-  double run[4];
-  double sum = 0.0;
-  bool weighty[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    double w = 0.0;
-    if (i0 + e < a.vocab) {
-      w = probability(exp2, plan.target, inv_p, lp[e], i0 + e, c);
-      if (subtract) w = fmax(w - probability(exp2, plan.draft, inv_q, lq[e], i0 + e, c), 0.0);
-    }
-    sum += w;
-    run[e] = sum;
-    weighty[e] = w > 0.0;
+  if (greedy) {
+    id = target.hot;
+  } else if (id < 0) {
+    // from p: unnormalised, as the parts' sums are
+    const PartStats* stats = a.stats + static_cast<size_t>(row) * 2 * a.parts;
+    id = draw_index(
+        lds, a, a.sample_uniforms[b], target_row, nullptr,
+        [&](int i) {
+          if (!(target.sum > 0.0)) return target.hot / kPart == i ? 1.0 : 0.0;
+          const PartStats s = stats[i];
+          return finite(s.max) ? s.sum * exp2((static_cast<double>(s.max) - target.max) * c) : 0.0;
+        },
+        [&](float p, float, int i) { return probability(exp2, target, 1.0, p, i, c); });
   }
-  const double incl = wave_inclusive_scan_f64(sum);
-  if (lane == 63) wave_total[wave] = incl;
-  __syncthreads();
-  double before = shared_before;
-  for (int w = 0; w < wave; ++w) before += wave_total[w];
-  before += incl - sum;
-  int hit = INT32_MAX, last = -1;
-#pragma unroll
-  for (int e = 3; e >= 0; --e) {
-    if (weighty[e]) {
-      last = max(last, i0 + e);
-      if (before + run[e] > shared_goal) hit = i0 + e;
-    }
+  for (int i = threadIdx.x; i <= a.max_draft; i += kVerifyThreads) {
+    ids[i] = i < kept ? a.draft_ids[first + i] : (i == kept ? id : -1);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    hit = min(hit, __shfl_xor(hit, o, 64));
-    last = max(last, __shfl_xor(last, o, 64));
-  }
-  if (lane == 0) {
-    wave_first[wave] = hit;
-    wave_last[wave] = last;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < kPickThreads / 64; ++w) {
-      hit = min(hit, wave_first[w]);
-      last = max(last, wave_last[w]);
-    }
-    ids[kept] = hit != INT32_MAX ? hit : max(last, 0);
-  }
+  if (threadIdx.x == 0) a.out_counts[b] = kept + 1;
 }
 
 int parts_for(int vocab) { return (vocab + kPart - 1) / kPart; }
-int slices_for(int vocab) { return (vocab + kSlice - 1) / kSlice; }
 
 struct VerifyLayout {
-  size_t totals_at, plans_at, bytes;
+  size_t totals_at, arrived_at, bytes;
 };
 
 VerifyLayout layout_for(int batch, int rows, int vocab) {
-  const size_t slices = static_cast<size_t>(slices_for(vocab));
+  const size_t parts = static_cast<size_t>(parts_for(vocab));
   VerifyLayout l;
-  l.totals_at = static_cast<size_t>(rows) * 2 * static_cast<size_t>(parts_for(vocab)) * sizeof(PartStats);
-  l.plans_at = l.totals_at + static_cast<size_t>(batch) * slices * sizeof(double2);
-  l.bytes = l.plans_at + static_cast<size_t>(batch) * sizeof(SequencePlan);
+  l.totals_at = static_cast<size_t>(rows) * 2 * parts * sizeof(PartStats);
+  l.arrived_at = l.totals_at + static_cast<size_t>(batch) * parts * sizeof(double);
+  l.bytes = l.arrived_at + static_cast<size_t>(batch) * sizeof(int);
   return l;
 }
 
@@ -641,14 +649,13 @@ extern "C" int lcr_batch_verify(int32_t* out_ids, int32_t* out_counts, const flo
   a.out_ids = out_ids;
   a.out_counts = out_counts;
   a.stats = reinterpret_cast<PartStats*>(ws);
-  a.totals = reinterpret_cast<double2*>(ws + layout.totals_at);
-  a.plans = reinterpret_cast<SequencePlan*>(ws + layout.plans_at);
+  a.totals = reinterpret_cast<double*>(ws + layout.totals_at);
+  a.arrived = reinterpret_cast<int*>(ws + layout.arrived_at);
   a.batch = batch;
   a.rows = rows;
   a.max_draft = max_draft;
   a.vocab = vocab;
   a.parts = parts_for(vocab);
-  a.slices = slices_for(vocab);
   a.logits_stride = logits_stride;
   a.vectors = logits_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(target_logits) & 15u) == 0 &&
               (reinterpret_cast<uintptr_t>(draft_logits) & 15u) == 0;
@@ -659,10 +666,8 @@ extern "C" int lcr_batch_verify(int32_t* out_ids, int32_t* out_counts, const flo
     verify_stats_kernel<<<grid, kVerifyThreads, 0, s>>>(a);
     CAPI_LAUNCHED();
   }
-  const dim3 grid(static_cast<unsigned>(a.slices), static_cast<unsigned>(batch));
-  verify_residual_kernel<<<grid, kVerifyThreads, 0, s>>>(a);
-  CAPI_LAUNCHED();
-  verify_pick_kernel<<<static_cast<unsigned>(batch), kPickThreads, 0, s>>>(a);
+  const dim3 grid(static_cast<unsigned>((a.parts + kVerifyWaves - 1) / kVerifyWaves), static_cast<unsigned>(batch));
+  verify_draw_kernel<<<grid, kVerifyThreads, 0, s>>>(a);
   CAPI_LAUNCHED();
   return LCR_OK;
 }
