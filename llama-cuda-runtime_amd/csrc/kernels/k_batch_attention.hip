@@ -560,36 +560,33 @@ __device__ __forceinline__ void clear_special(elem_t* values, int chunks) {
   }
 }
 
-// Direct loads of kLoads groups of kLoadRows keys: group n of a call holds
-// keys key_of(n) .. + kLoadRows - 1 (those past `last` repeat it). With whole
-// pages (page_size a multiple of kLoadRows) a group lies in one page, whose table
-// entry is a scalar load; otherwise each lane reads its own key's, and waits for
-// it with every tile load in flight.
-template <int kLoads>
-struct LoadPages {
-  int page[kLoads];
-  int slot[kLoads];  // of the group's first key, within its page
+// Keys are loaded in runs: kRun keys from a multiple of kRun on, by direct loads
+// of kLoadRows keys each. With whole pages (page_size a multiple of 16) a run
+// lies in one page, whose table entry is a scalar load; otherwise each lane reads
+// its own key's, and waits for it with every tile load in flight. Keys past the
+// last repeat it.
+struct RunPage {
+  int page;
+  int slot;  // of the run's first key, within its page
 };
 
-template <int kHeadDim, bool kWholePages, int kLoads, typename KeyOf>
-__device__ __forceinline__ LoadPages<kLoads> find_pages(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p,
-                                                        int last, KeyOf key_of) {
-  LoadPages<kLoads> pages;
-  typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
-  const constant_ptr table = (constant_ptr)(reinterpret_cast<uintptr_t>(p.table));
-  constexpr int kLoadRows = FlashShape<kHeadDim>::kLoadRows;
-#pragma unroll
-  for (int n = 0; n < kLoads; ++n) {
-    if constexpr (kWholePages) {
-      const int key = uniform(min(key_of(n), last / kLoadRows * kLoadRows));
-      const int index = plan.by_page(key);
-      pages.page[n] = table[index];
-      pages.slot[n] = key - index * a.view.page_size;
-    } else {
-      pages.page[n] = pages.slot[n] = 0;
-    }
+template <int kRun>
+__device__ __forceinline__ int run_start(int key, int last) {
+  return min(key, last / kRun * kRun);
+}
+
+template <bool kWholePages, int kRun>
+__device__ __forceinline__ RunPage find_run(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
+                                            int key) {
+  if constexpr (kWholePages) {
+    typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
+    const constant_ptr table = (constant_ptr)(reinterpret_cast<uintptr_t>(p.table));
+    const int first = uniform(run_start<kRun>(key, last));
+    const int index = plan.by_page(first);
+    return RunPage{table[index], first - index * a.view.page_size};
+  } else {
+    return RunPage{0, 0};
   }
-  return pages;
 }
 
 // A page outside the pool is read as page 0, and `bad` set.
@@ -599,32 +596,51 @@ __device__ __forceinline__ int pool_page(const BatchAttnArgs& a, int page, int& 
   return inside ? page : 0;
 }
 
-template <int kHeadDim, bool kWholePages, int kLoads, bool kKeys, typename KeyOf, typename RowOf>
-__device__ __forceinline__ void issue_loads(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
-                                            const LoadPages<kLoads>& pages, int& bad, elem_t* tile, KeyOf key_of,
-                                            RowOf row_of) {
+// The run of keys (or values) from key `key` on into rows row0 .. of a tile. Row
+// r of LDS starts r rows behind the tile, in memory as in LDS, so the loads of a
+// run differ by one offset that counts in both.
+template <int kHeadDim, bool kWholePages, int kRun, bool kKeys>
+__device__ __forceinline__ void load_run(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
+                                         const RunPage& run, int& bad, elem_t* tile, int key, int row0) {
   using Shape = FlashShape<kHeadDim>;
+  constexpr int kLoads = kRun / Shape::kLoadRows;
+  constexpr int kLoadBytes = Shape::kLoadRows * kHeadDim * 2;
+  static_assert(kLoadBytes == 1024 && kLoads <= 4, "offsets of 12 bits");
   const int load_row = lane_id() / Shape::kRowChunks;
   const int load_slot = lane_id() % Shape::kRowChunks;
   const elem_t* pool = kKeys ? p.keys : p.values;
-#pragma unroll
-  for (int n = 0; n < kLoads; ++n) {
-    const int row = row_of(n);  // of the tile, the group's first
-    const int swizzle = kKeys ? key_swizzle<kHeadDim>(row + load_row) : value_swizzle<kHeadDim>(row + load_row);
-    const uint32_t to = lds_address_of(tile + row * kHeadDim);
-    if constexpr (kWholePages) {
-      const int first = min(key_of(n), last / Shape::kLoadRows * Shape::kLoadRows);
-      const int page = pool_page(a, pages.page[n], bad);
-      const size_t from = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                          static_cast<size_t>(pages.slot[n] * kHeadDim);
-      load_to_lds16(pool + from, 2u * (min(load_row, last - first) * kHeadDim + 8 * (load_slot ^ swizzle)), to);
+  auto chunk = [&](int n) {
+    const int row = row0 + n * Shape::kLoadRows + load_row;
+    return 16u * static_cast<uint32_t>(load_slot ^ (kKeys ? key_swizzle<kHeadDim>(row) : value_swizzle<kHeadDim>(row)));
+  };
+  const uint32_t to = lds_address_of(tile + row0 * kHeadDim);
+  if constexpr (kWholePages) {
+    const int first = run_start<kRun>(key, last);
+    const int page = pool_page(a, run.page, bad);
+    const elem_t* from = pool + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                         static_cast<size_t>(run.slot * kHeadDim);
+    if (last - first >= kRun - 1) {
+      const uint32_t row_at = static_cast<uint32_t>(load_row * kHeadDim * 2);
+      load_to_lds16<0>(from, row_at + chunk(0), to);
+      if constexpr (kLoads > 1) load_to_lds16<kLoadBytes>(from, row_at + chunk(1), to);
+      if constexpr (kLoads > 2) load_to_lds16<2 * kLoadBytes>(from, row_at + chunk(2), to);
+      if constexpr (kLoads > 3) load_to_lds16<3 * kLoadBytes>(from, row_at + chunk(3), to);
     } else {
-      const int key = min(key_of(n) + load_row, last);
-      const int index = plan.by_page(key);
+#pragma unroll 1
+      for (int n = 0; n < kLoads; ++n) {
+        const int row = min(n * Shape::kLoadRows + load_row, last - first);
+        load_to_lds16<0>(from, static_cast<uint32_t>(row * kHeadDim * 2) + chunk(n), to + n * kLoadBytes);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int n = 0; n < kLoads; ++n) {
+      const int at_key = min(key + n * Shape::kLoadRows + load_row, last);
+      const int index = plan.by_page(at_key);
       const int page = pool_page(a, p.table[index], bad);
       const size_t at = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                        static_cast<size_t>(key - index * a.view.page_size) * kHeadDim;
-      load_to_lds16(pool + at + 8 * (load_slot ^ swizzle), to);
+                        static_cast<size_t>(at_key - index * a.view.page_size) * kHeadDim;
+      load_to_lds16(reinterpret_cast<const char*>(pool + at) + chunk(n), to + n * kLoadBytes);
     }
   }
 }
@@ -661,14 +677,20 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   const int last = p.key1 - 1;
   int bad = 0;
   auto first_key = [&](int t) { return p.key0 + 32 * (wave + Shape::kWaves * t); };
-  auto pages_of = [&](int t) {
-    return find_pages<kHeadDim, kWholePages, kLoads>(a, plan, p, last, [&](int n) { return first_key(t) + Shape::kLoadRows * n; });
+  struct StepPages {
+    RunPage run[2];
   };
-  auto issue = [&](auto is_keys, int t, const LoadPages<kLoads>& pages) {
+  auto pages_of = [&](int t) {
+    return StepPages{{find_run<kWholePages, 16>(a, plan, p, last, first_key(t)),
+                      find_run<kWholePages, 16>(a, plan, p, last, first_key(t) + 16)}};
+  };
+  auto issue = [&](auto is_keys, int t, const StepPages& pages) {
     constexpr bool kKeys = decltype(is_keys)::value;
-    issue_loads<kHeadDim, kWholePages, kLoads, kKeys>(a, plan, p, last, pages, bad, kKeys ? key_tile(t) : value_tile(t),
-                                         [&](int n) { return first_key(t) + Shape::kLoadRows * n; },
-                                         [&](int n) { return Shape::kLoadRows * n; });
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      load_run<kHeadDim, kWholePages, 16, kKeys>(a, plan, p, last, pages.run[n], bad, kKeys ? key_tile(t) : value_tile(t),
+                                                 first_key(t) + 16 * n, 16 * n);
+    }
   };
   using Keys = std::integral_constant<bool, true>;
   using Values = std::integral_constant<bool, false>;
@@ -677,7 +699,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   rows.clear();
   if (count > 0) {
     load_rows<kHeadDim, kRF>(rows, a, plan, p, 0);
-    LoadPages<kLoads> pages[kSlots];
+    StepPages pages[kSlots];
 #pragma unroll
     for (int t = 0; t < kSlots; ++t) pages[t] = pages_of(t);
 #pragma unroll
@@ -693,7 +715,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   for (int t = 0; t < count; ++t) {
     const int left = count - 1 - t;
     const bool more = left >= kSlots;
-    LoadPages<kLoads> pages{};
+    StepPages pages{};
     if (more) pages = pages_of(t + kSlots);
     // In flight behind step t's keys: its values, and the later steps' both.
     if (kSlots > 1 && left > 0) {
@@ -793,26 +815,24 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
                                           const Piece& p) {
   using Shape = FlashShape<kHeadDim>;
   constexpr int kRF = 2;
-  constexpr int kLoads = 64 / Shape::kLoadRows / Shape::kWaves;  // a wave's, of keys or of values
-  static_assert(kLoads * Shape::kLoadRows * Shape::kWaves == 64, "a tile splits over the waves");
+  constexpr int kRun = 64 / Shape::kWaves;          // a wave's keys of a tile
+  constexpr int kLoads = kRun / Shape::kLoadRows;
   constexpr int kTileRows = Shape::kTileRows;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int lane = lane_id();
   const int col = lane & 15;
   const int grp = lane >> 4;
-  auto key_tile = [&](int t) { return lds.ring + (t % Shape::kStages) * (2 * 64 * kHeadDim); };
-  auto value_tile = [&](int t) { return key_tile(t) + 64 * kHeadDim; };
+  constexpr int kStageElems = 2 * 64 * kHeadDim;    // a tile's keys, then its values
   const int tiles = (p.key1 - p.key0 + 63) / 64;
   const int last = p.key1 - 1;
   int bad = 0;
-  auto group_row = [&](int n) { return Shape::kLoadRows * (wave + Shape::kWaves * n); };
-  auto pages_of = [&](int t) {
-    return find_pages<kHeadDim, kWholePages, kLoads>(a, plan, p, last, [&](int n) { return p.key0 + 64 * t + group_row(n); });
+  auto page_of = [&](int t) {
+    return find_run<kWholePages, kRun>(a, plan, p, last, p.key0 + 64 * t + kRun * wave);
   };
-  auto issue = [&](int t, const LoadPages<kLoads>& pages) {
-    auto key_of = [&](int n) { return p.key0 + 64 * t + group_row(n); };
-    issue_loads<kHeadDim, kWholePages, kLoads, true>(a, plan, p, last, pages, bad, key_tile(t), key_of, group_row);
-    issue_loads<kHeadDim, kWholePages, kLoads, false>(a, plan, p, last, pages, bad, value_tile(t), key_of, group_row);
+  auto issue = [&](int t, elem_t* stage, const RunPage& page) {
+    const int key = p.key0 + 64 * t + kRun * wave;
+    load_run<kHeadDim, kWholePages, kRun, true>(a, plan, p, last, page, bad, stage, key, kRun * wave);
+    load_run<kHeadDim, kWholePages, kRun, false>(a, plan, p, last, page, bad, stage + 64 * kHeadDim, key, kRun * wave);
   };
   if (threadIdx.x == 0) lds.bad = 0;
 
@@ -828,18 +848,21 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
   }
   constexpr int kAhead = Shape::kStages - 1;
   if (tiles > 0) {
-    LoadPages<kLoads> first[kAhead];
+    RunPage first[kAhead];
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) first[t] = pages_of(t);
+    for (int t = 0; t < kAhead; ++t) first[t] = page_of(t);
 #pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      if (t < tiles) issue(t, first[t]);
+      if (t < tiles) issue(t, lds.ring + t * kStageElems, first[t]);
     }
   }
   hold_rows(rows);
-  for (int t = 0; t < tiles; ++t) {
-    LoadPages<kLoads> pages{};
-    if (t + kAhead < tiles) pages = pages_of(t + kAhead);
+  elem_t* stage = lds.ring;                            // tile t's
+  elem_t* next_stage = lds.ring + kAhead * kStageElems;  // tile t + kAhead's: the one before tile t's
+  auto step = [&](elem_t* at) { return at == lds.ring + kAhead * kStageElems ? lds.ring : at + kStageElems; };
+  for (int t = 0; t < tiles; ++t, stage = step(stage), next_stage = step(next_stage)) {
+    RunPage page{0, 0};
+    if (t + kAhead < tiles) page = page_of(t + kAhead);
     // This wave's loads of the tile have landed (the later tiles' remain);
     // behind the barrier every wave's have, and the tile before is free.
     if (t + kAhead - 1 < tiles) {
@@ -848,21 +871,21 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
       wait_stage_landed<0>();
     }
     plain_barrier();
-    if (t + kAhead < tiles) issue(t + kAhead, pages);
+    if (t + kAhead < tiles) issue(t + kAhead, next_stage, page);
     // A tile that some row of the unit does not see whole: every wave looks for
     // infinities and NaN among its values, and finds the same.
     const int tile0 = p.key0 + 64 * t;
-    const bool special = tile0 + 64 > p.seen_first && any_special(value_tile(t), kHeadDim / 8);
+    const bool special = tile0 + 64 > p.seen_first && any_special(stage + 64 * kHeadDim, kHeadDim / 8);
     // 32 keys at a time: as many scores as registers allow with four waves a
     // SIMD.
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       const int key0 = tile0 + 32 * half;
       const bool mine = key0 < any_seen;
-      elem_t* values = value_tile(t) + half * 32 * kHeadDim;
+      elem_t* values = stage + (64 + 32 * half) * kHeadDim;
       TileWork<kHeadDim, kRF, 2> work;
       if (mine) {
-        work.scores(rows, key_tile(t) + half * 32 * kHeadDim);
+        work.scores(rows, stage + half * 32 * kHeadDim);
         if (key0 + 32 > all_seen) work.mask(rows, key0);
         work.weights(rows, plan.scale_log2e);
       }
@@ -1241,7 +1264,7 @@ void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   }
   plan.by_shares = FastDivide::by(static_cast<uint32_t>(plan.shares));
   const long long most = static_cast<long long>(a.max_new) * a.group;
-  if (a.view.page_size % Shape::kLoadRows == 0) {
+  if (a.view.page_size % 16 == 0) {
     if (most <= 16) {
       launch_flash_kernels<kHeadDim, 16, true>(a, plan, s);
     } else if (most <= kFewRows) {
