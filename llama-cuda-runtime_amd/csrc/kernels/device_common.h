@@ -77,16 +77,24 @@ __device__ __forceinline__ void load_to_lds16(const void* src, uint32_t lds_addr
 // instruction wrote them (v_readfirstlane, v_readlane) and not sooner. The
 // compiler keeps that distance for its own instructions, not for these, so they
 // bring their own wait.
-template <int kOffset>
+// kStream marks data that is read once (non-temporal).
+template <int kOffset, bool kStream>
 __device__ __forceinline__ void load_to_lds16(const void* base, uint32_t offset, uint32_t lds_address) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(base);
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits));
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits >> 32));
   const unsigned long long uniform_base = (static_cast<unsigned long long>(hi) << 32) | lo;
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
-               :
-               : "v"(offset), "s"(uniform_base), "{m0}"(lds_address), "i"(kOffset)
-               : "memory");
+  if constexpr (kStream) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3 nt"
+                 :
+                 : "v"(offset), "s"(uniform_base), "{m0}"(lds_address), "i"(kOffset)
+                 : "memory");
+  } else {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3"
+                 :
+                 : "v"(offset), "s"(uniform_base), "{m0}"(lds_address), "i"(kOffset)
+                 : "memory");
+  }
 }
 
 // Wait until at most kCount vector-memory operations of this wave are in

@@ -126,8 +126,13 @@ struct FlashPlan {
 constexpr int kFewRows = 32;
 // Steps that a unit counts for besides its keys': its queries, the join of the
 // waves, the output.
-constexpr int kUnitSteps = 2;
+constexpr int kUnitSteps = 3;
 constexpr int kStepKeys = 64;
+// A unit of at most so many steps is not cut: its partials and their join cost
+// more than the share it lengthens. Eight prompts of 256 tokens 20 us, cut 27; one
+// of 2048 50, cut 51. With 16 steps 64 sequences of 600 positions took 20 us for
+// 18, and a prompt of 1024 tokens 37 for 30.
+constexpr int kWholeSteps = 8;
 
 // A sequence's share of the work, in tokens and steps of one kv head.
 struct Sequence {
@@ -281,6 +286,9 @@ template <int kHeadDim>
 struct FlashShape {
   static constexpr int kWaves = kHeadDim == 64 ? 4 : 8;
   static constexpr int kBlocks = kHeadDim == 64 ? 3 : 1;      // resident a compute unit
+  // Of few rows, two: 64 sequences of 8000 positions 115 us, with three 116, and
+  // shorter caches have fewer cuts (32 of 1000 in 16.0, 16.1).
+  static constexpr int kFewBlocks = kHeadDim == 64 ? 2 : 1;
   static constexpr int kSimdWaves = kWaves * kBlocks / 4;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kTileRows = 32 * kWaves;               // packed rows of a tile of many rows
@@ -599,7 +607,7 @@ __device__ __forceinline__ int pool_page(const BatchAttnArgs& a, int page, int& 
 // The run of keys (or values) from key `key` on into rows row0 .. of a tile. Row
 // r of LDS starts r rows behind the tile, in memory as in LDS, so the loads of a
 // run differ by one offset that counts in both.
-template <int kHeadDim, bool kWholePages, int kRun, bool kKeys>
+template <int kHeadDim, bool kWholePages, int kRun, bool kKeys, bool kStream>
 __device__ __forceinline__ void load_run(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
                                          const RunPage& run, int& bad, elem_t* tile, int key, int row0) {
   using Shape = FlashShape<kHeadDim>;
@@ -621,15 +629,15 @@ __device__ __forceinline__ void load_run(const BatchAttnArgs& a, const FlashPlan
                          static_cast<size_t>(run.slot * kHeadDim);
     if (last - first >= kRun - 1) {
       const uint32_t row_at = static_cast<uint32_t>(load_row * kHeadDim * 2);
-      load_to_lds16<0>(from, row_at + chunk(0), to);
-      if constexpr (kLoads > 1) load_to_lds16<kLoadBytes>(from, row_at + chunk(1), to);
-      if constexpr (kLoads > 2) load_to_lds16<2 * kLoadBytes>(from, row_at + chunk(2), to);
-      if constexpr (kLoads > 3) load_to_lds16<3 * kLoadBytes>(from, row_at + chunk(3), to);
+      load_to_lds16<0, kStream>(from, row_at + chunk(0), to);
+      if constexpr (kLoads > 1) load_to_lds16<kLoadBytes, kStream>(from, row_at + chunk(1), to);
+      if constexpr (kLoads > 2) load_to_lds16<2 * kLoadBytes, kStream>(from, row_at + chunk(2), to);
+      if constexpr (kLoads > 3) load_to_lds16<3 * kLoadBytes, kStream>(from, row_at + chunk(3), to);
     } else {
 #pragma unroll 1
       for (int n = 0; n < kLoads; ++n) {
         const int row = min(n * Shape::kLoadRows + load_row, last - first);
-        load_to_lds16<0>(from, static_cast<uint32_t>(row * kHeadDim * 2) + chunk(n), to + n * kLoadBytes);
+        load_to_lds16<0, kStream>(from, static_cast<uint32_t>(row * kHeadDim * 2) + chunk(n), to + n * kLoadBytes);
       }
     }
   } else {
@@ -688,7 +696,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
     constexpr bool kKeys = decltype(is_keys)::value;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      load_run<kHeadDim, kWholePages, 16, kKeys>(a, plan, p, last, pages.run[n], bad, kKeys ? key_tile(t) : value_tile(t),
+      load_run<kHeadDim, kWholePages, 16, kKeys, true>(a, plan, p, last, pages.run[n], bad, kKeys ? key_tile(t) : value_tile(t),
                                                  first_key(t) + 16 * n, 16 * n);
     }
   };
@@ -831,8 +839,8 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
   };
   auto issue = [&](int t, elem_t* stage, const RunPage& page) {
     const int key = p.key0 + 64 * t + kRun * wave;
-    load_run<kHeadDim, kWholePages, kRun, true>(a, plan, p, last, page, bad, stage, key, kRun * wave);
-    load_run<kHeadDim, kWholePages, kRun, false>(a, plan, p, last, page, bad, stage + 64 * kHeadDim, key, kRun * wave);
+    load_run<kHeadDim, kWholePages, kRun, true, false>(a, plan, p, last, page, bad, stage, key, kRun * wave);
+    load_run<kHeadDim, kWholePages, kRun, false, false>(a, plan, p, last, page, bad, stage + 64 * kHeadDim, key, kRun * wave);
   };
   if (threadIdx.x == 0) lds.bad = 0;
 
@@ -1003,7 +1011,9 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
     p.key0 = 0;
     p.key1 = p.seen_last;
     p.slot = -1;
-    if (plan.split && (start < at || stop > end)) {
+    // A short unit is not cut: it goes to the share that it begins in.
+    const bool whole = !plan.split || stop - start <= kWholeSteps;
+    if (!whole && (start < at || stop > end)) {
       // steps into the unit, in keys
       auto cut = [&](int steps) { return steps >= (p.seen_last + kStepKeys - 1) / kStepKeys ? p.seen_last : steps * kStepKeys; };
       p.slot = 2 * block + (start < at ? 0 : 1);
@@ -1024,7 +1034,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
         }
       }
     }
-    if (p.rows > 0) {
+    if (p.rows > 0 && !(whole && start < at)) {
       if (!single) {
         if constexpr (kMany) many_rows<kHeadDim, kWholePages>(lds, a, plan, p);
       } else {
@@ -1216,15 +1226,18 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
 
 // A kv head's shares: all heads' together are the blocks resident at once.
 template <int kHeadDim>
-int flash_shares(int kv_heads) {
-  return std::max(1, device_compute_units() * FlashShape<kHeadDim>::kBlocks / kv_heads);
+int flash_shares(int kv_heads, bool many) {
+  const int blocks = many ? FlashShape<kHeadDim>::kBlocks : FlashShape<kHeadDim>::kFewBlocks;
+  return std::max(1, device_compute_units() * blocks / kv_heads);
 }
+
+bool many_rows_possible(int max_new, int group) { return static_cast<long long>(max_new) * group > kFewRows; }
 
 template <int kHeadDim>
 size_t flash_workspace(int max_new, int kv_heads, int group) {
-  const bool many = static_cast<long long>(max_new) * group > kFewRows;
+  const bool many = many_rows_possible(max_new, group);
   const size_t rows = many ? FlashShape<kHeadDim>::kTileRows : kFewRows;
-  const size_t shares = static_cast<size_t>(flash_shares<kHeadDim>(kv_heads)) * static_cast<size_t>(kv_heads);
+  const size_t shares = static_cast<size_t>(flash_shares<kHeadDim>(kv_heads, many)) * static_cast<size_t>(kv_heads);
   return shares * (sizeof(CutUnit) + 2 * rows * (kHeadDim + 2) * sizeof(float));
 }
 
@@ -1253,9 +1266,15 @@ void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   plan.by_tile = FastDivide::by(static_cast<uint32_t>(plan.tile_tokens));
   plan.scale_log2e = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
   plan.min_share = 4;
-  if (workspace != nullptr && workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
+  // Tables of at most 1024 positions: no unit is long enough for a cut and its
+  // second launch to pay. By the number of sequences and positions, one token
+  // each, cut and not: 8 of 1000 14.4 and 11.7 us, 64 of 600 18.2 and 13.1, 128 of
+  // 1000 36.4 and 35.0; 8 of 2000 14.3 and 18.0.
+  constexpr int kCutPositions = 1024;
+  if (a.held > kCutPositions && workspace != nullptr &&
+      workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
     plan.split = 1;
-    plan.shares = flash_shares<kHeadDim>(kv_heads);
+    plan.shares = flash_shares<kHeadDim>(kv_heads, many_rows_possible(a.max_new, a.group));
     plan.cuts = static_cast<CutUnit*>(workspace);
     plan.partials = reinterpret_cast<float*>(plan.cuts + static_cast<size_t>(plan.shares) * kv_heads);
   } else {
