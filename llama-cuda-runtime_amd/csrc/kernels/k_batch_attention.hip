@@ -435,34 +435,46 @@ struct TileWork {
     }
   }
 
-  // The running statistics, and the weights rounded to the element type.
-  __device__ __forceinline__ void weights(FlashRows<kHeadDim, kRF>& rows, float c) {
+  // The running statistics: a larger base where a score needs one.
+  __device__ __forceinline__ void raise_base(FlashRows<kHeadDim, kRF>& rows, float c) {
+    float top[kRF];
+    bool raise = false;
 #pragma unroll
     for (int rf = 0; rf < kRF; ++rf) {
-      float top = s[rf][0][0];
+      top[rf] = s[rf][0][0];
 #pragma unroll
       for (int kf = 0; kf < kKF; ++kf) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) top = fmaxf(top, s[rf][kf][v]);
+        for (int v = 0; v < 4; ++v) top[rf] = fmaxf(top[rf], s[rf][kf][v]);
       }
       // c top + base: the largest weight's exponent (inf for a first visible
       // key, NaN, which compares false, while there is none)
-      if (__any(__builtin_fmaf(top, c, rows.base[rf]) > 8.0f)) {
-        top = fmaxf(top, xor_lane<16>(top));
-        top = fmaxf(top, xor_lane<32>(top));
-        if (__builtin_fmaf(top, c, rows.base[rf]) > 0.0f) {
-          const float base = -(top * c);
-          const float move = __builtin_amdgcn_exp2f(base - rows.base[rf]);
-          rows.base[rf] = base;
-          rows.sum[rf] *= move;
+      raise |= __builtin_fmaf(top[rf], c, rows.base[rf]) > 8.0f;
+    }
+    if (!__any(raise)) return;
 #pragma unroll
-          for (int df = 0; df < Shape::kDFrags; ++df) rows.o[rf][df] *= move;
-        }
+    for (int rf = 0; rf < kRF; ++rf) {
+      float most = fmaxf(top[rf], xor_lane<16>(top[rf]));
+      most = fmaxf(most, xor_lane<32>(most));
+      if (__builtin_fmaf(most, c, rows.base[rf]) > 0.0f) {
+        const float base = -(most * c);
+        const float move = __builtin_amdgcn_exp2f(base - rows.base[rf]);
+        rows.base[rf] = base;
+        rows.sum[rf] *= move;
+#pragma unroll
+        for (int df = 0; df < Shape::kDFrags; ++df) rows.o[rf][df] *= move;
       }
+    }
+  }
+
+  // The weights of the scores of 32 keys, rounded to the element type.
+  __device__ __forceinline__ void weights(const FlashRows<kHeadDim, kRF>& rows, float c, int half) {
+#pragma unroll
+    for (int rf = 0; rf < kRF; ++rf) {
       // before the first visible key every score is -inf: against base 0
       const float base = rows.base[rf] == __builtin_huge_valf() ? 0.0f : rows.base[rf];
 #pragma unroll
-      for (int kf = 0; kf < kKF; ++kf) {
+      for (int kf = 2 * half; kf < 2 * half + 2; ++kf) {
         float p[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rf][kf][v], c, base));
@@ -480,19 +492,16 @@ struct TileWork {
   // The weights' sum is a product with ones: of what the values are weighted
   // with, rounded as they are, and off the vector units, which the exponentials
   // keep busy.
-  __device__ __forceinline__ void products(FlashRows<kHeadDim, kRF>& rows, const elem_t* values) {
+  __device__ __forceinline__ void products(FlashRows<kHeadDim, kRF>& rows, const elem_t* values, int half) {
     constexpr uint32_t kOnes = kOneBits << 16 | kOneBits;
     const mfma_in8 ones = as_operand(vec16{{kOnes, kOnes, kOnes, kOnes}});
 #pragma unroll
-    for (int half = 0; half < kKF / 2; ++half) {
+    for (int rf = 0; rf < kRF; ++rf) rows.sum[rf] = mfma16x16x32(ones, weight_operand(rf, half), rows.sum[rf]);
 #pragma unroll
-      for (int rf = 0; rf < kRF; ++rf) rows.sum[rf] = mfma16x16x32(ones, weight_operand(rf, half), rows.sum[rf]);
+    for (int df = 0; df < Shape::kDFrags; ++df) {
+      const mfma_in8 v = transposed_values<kHeadDim>(values, half, df, lane_id());
 #pragma unroll
-      for (int df = 0; df < Shape::kDFrags; ++df) {
-        const mfma_in8 v = transposed_values<kHeadDim>(values, half, df, lane_id());
-#pragma unroll
-        for (int rf = 0; rf < kRF; ++rf) rows.o[rf][df] = mfma16x16x32(v, weight_operand(rf, half), rows.o[rf][df]);
-      }
+      for (int rf = 0; rf < kRF; ++rf) rows.o[rf][df] = mfma16x16x32(v, weight_operand(rf, half), rows.o[rf][df]);
     }
   }
 
@@ -738,7 +747,8 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
     reads_returned();  // the keys have been read
     if (more) issue(Keys{}, t + kSlots, pages);
     if (!whole) work.mask(rows, key0);
-    work.weights(rows, plan.scale_log2e);
+    work.raise_base(rows, plan.scale_log2e);
+    work.weights(rows, plan.scale_log2e, 0);
     // Behind step t's values: the later steps' keys and values.
     if (more) {
       loads_landed<(2 * (kSlots - 1) + 1) * kLoads>();
@@ -751,7 +761,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
       work.mark_special(rows, value_tile(t));
       clear_special(value_tile(t), 32 * kHeadDim / 512);
     }
-    work.products(rows, value_tile(t));
+    work.products(rows, value_tile(t), 0);
     reads_returned();
     if (more) issue(Values{}, t + kSlots, pages);
   }
@@ -884,29 +894,40 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
     // infinities and NaN among its values, and finds the same.
     const int tile0 = p.key0 + 64 * t;
     const bool special = tile0 + 64 > p.seen_first && any_special(stage + 64 * kHeadDim, kHeadDim / 8);
-    // 32 keys at a time: as many scores as registers allow with four waves a
-    // SIMD.
+    const bool mine = tile0 < any_seen;
+    const bool whole = tile0 + 64 <= all_seen;
+    elem_t* values = stage + 64 * kHeadDim;
+    if (mine) {
+      TileWork<kHeadDim, kRF, 4> work;
+      work.scores(rows, stage);
+      if (!whole) work.mask(rows, tile0);
+      work.raise_base(rows, plan.scale_log2e);
+      if (!special) {
+        work.weights(rows, plan.scale_log2e, 0);
+        work.products(rows, values, 0);
+        work.weights(rows, plan.scale_log2e, 1);
+        work.products(rows, values, 1);
+      }
+    }
+    if (!special) continue;
+    // Half a tile at a time, its scores once more: registers for the marks.
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
-      const int key0 = tile0 + 32 * half;
-      const bool mine = key0 < any_seen;
-      elem_t* values = stage + (64 + 32 * half) * kHeadDim;
+      elem_t* at = values + half * 32 * kHeadDim;
       TileWork<kHeadDim, kRF, 2> work;
       if (mine) {
         work.scores(rows, stage + half * 32 * kHeadDim);
-        if (key0 + 32 > all_seen) work.mask(rows, key0);
-        work.weights(rows, plan.scale_log2e);
+        if (!whole) work.mask(rows, tile0 + 32 * half);
+        work.weights(rows, plan.scale_log2e, 0);
+        work.mark_special(rows, at);
       }
-      if (special) {
-        if (mine) work.mark_special(rows, values);
-        wait_lds();
-        plain_barrier();
-        static_assert(kHeadDim / 16 <= Shape::kWaves, "a wave clears one group of chunks at most");
-        if (wave < kHeadDim / 16) clear_special(values + wave * 512, 1);
-        wait_lds();
-        plain_barrier();
-      }
-      if (mine) work.products(rows, values);
+      wait_lds();
+      plain_barrier();
+      static_assert(kHeadDim / 16 <= Shape::kWaves, "a wave clears one group of chunks at most");
+      if (wave < kHeadDim / 16) clear_special(at + wave * 512, 1);
+      wait_lds();
+      plain_barrier();
+      if (mine) work.products(rows, at, 0);
     }
   }
   if (__any(bad != 0) && lane == 0) lds.bad = 1;

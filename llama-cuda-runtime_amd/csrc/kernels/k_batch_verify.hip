@@ -20,6 +20,7 @@
 // Which block arrives last decides who computes, not what: all sums have a fixed
 // order.
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cstdint>
 
@@ -47,8 +48,8 @@ struct alignas(16) PartStats {
 // What a row's distribution is: exp((l - max) / T) / sum where max is finite,
 // else (sum = 0) one at the index `hot`.
 struct RowStats {
-  double max;
   double sum;
+  float max;
   int hot;
 };
 
@@ -74,12 +75,14 @@ struct VerifyArgs {
   bool vectors;         // rows on 16-byte boundaries
 };
 
-// 2^(j / 64), by a thread of the table's 64: 2^x on [-1/2, 1/2] by its Chebyshev
-// interpolation of degree 10 (off by 3e-16), doubled for j of 32 and more.
-constexpr int kExp2Entries = 64;
+// 2^(j / 32), by a thread of the table's 32: 2^x on [-1/2, 1/2] by its Chebyshev
+// interpolation of degree 10 (off by 3e-16), doubled for j of 16 and more. The
+// table holds it with j << 15 taken off the high word, which the exponent's
+// addition below puts back.
+constexpr int kExp2Entries = 32;
 
-__device__ __forceinline__ double exp2_entry(int j) {
-  const double x = (j < 32 ? j : j - 64) * (1.0 / 64.0);
+__device__ __forceinline__ uint2 exp2_entry(int j) {
+  const double x = (j < 16 ? j : j - 32) * (1.0 / 32.0);
   double p = 7.072585949269223e-09;
   p = __builtin_fma(p, x, 1.0208690299958306e-07);
   p = __builtin_fma(p, x, 1.321544258792169e-06);
@@ -91,46 +94,80 @@ __device__ __forceinline__ double exp2_entry(int j) {
   p = __builtin_fma(p, x, 0.24022650695910097);
   p = __builtin_fma(p, x, 0.69314718055995);
   p = __builtin_fma(p, x, 1.0);
-  return j < 32 ? p : 2.0 * p;
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, j < 16 ? p : 2.0 * p);
+  return make_uint2(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32) - (static_cast<uint32_t>(j) << 15));
 }
 
-// 2^z for z <= 0 in fp64: z = k / 64 + f with k whole, by adding and taking off
-// 1.5 * 2^46 (k then also stands in the sum's low word); 2^f = 1 + f Q(f) on
-// [-1/128, 1/128], Q by Chebyshev interpolation (off by 5e-15), times the
-// table's 2^((k mod 64) / 64), and k / 64 added to the exponent. 0 below -1020,
-// where the result would leave the normal range, and for NaN (a logit of -inf at
-// an infinite temperature). A polynomial over [-1/2, 1/2] instead of the table
-// takes six more fp64 operations a logit: 48 us against 42 for the statistics
-// of 332 rows of 128256.
-// The coefficients are kept in scalar registers: left to the compiler, each is
-// moved into vector registers before each use.
+constexpr double kLog2e = 1.44269504088896340736;
+
+// The scale of a temperature: z = (l - max) c is the power of two that a logit
+// weighs, and logits more than `span` below the largest weigh nothing: z below
+// -1020 would leave the normal range.
+struct Scale {
+  double c, span;
+};
+
+__device__ __forceinline__ Scale scale_of(float temperature) {
+  const double t = temperature;
+  return Scale{kLog2e / t, t * (1020.0 / kLog2e)};
+}
+
+// The lowest logit that weighs anything beside `max`.
+__device__ __forceinline__ double lowest_of(float max, const Scale& scale) {
+  return static_cast<double>(max) - scale.span;
+}
+
+// The next float at or above a double, -FLT_MAX at least.
+__device__ __forceinline__ float float_above(double v) {
+  const float f = fmaxf(static_cast<float>(v), -FLT_MAX);
+  if (static_cast<double>(f) >= v) return f;
+  const int bits = __float_as_int(f);
+  return f == 0.0f ? __int_as_float(1) : __int_as_float(bits + (bits < 0 ? -1 : 1));
+}
+
+// exp((l - max) / T) = 2^z in fp64: z = k / 32 + f with k whole, by adding and
+// taking off 1.5 * 2^47 (k then also stands in the sum's low word); 2^f = 1 + f
+// Q(f) on [-1/64, 1/64], Q by Chebyshev interpolation (off by 1.6e-13, of which
+// a running sum over a vocabulary hands a draw of 1e-8 to a neighbour), times the
+// table's 2^((k mod 32) / 32), and k / 32 added to the exponent. 32 entries of 8
+// bytes lie on banks of their own, so that 64 lanes with an entry each read them
+// without conflicts. MEASURED
+// The coefficients are kept in registers, scalar but for one (an instruction
+// takes one scalar): left to the compiler, each is moved before each use.
 struct Exp2 {
   double c0, c1, c2, c3;
-  const double* table;
+  const uint2* table;
 
-  __device__ __forceinline__ explicit Exp2(const double* table_lds)
-      : c0(0.6931471805593244), c1(0.24022650695902897), c2(0.05550419004645178), c3(0.009618138509201629),
+  __device__ __forceinline__ explicit Exp2(const uint2* table_lds)
+      : c0(0.693147180550011), c1(0.24022650695795306), c2(0.055504434191939005), c3(0.009618166713972776),
         table(table_lds) {
-    asm volatile("" : "+s"(c0), "+s"(c1), "+s"(c2), "+s"(c3));
+    asm volatile("" : "+s"(c0), "+s"(c1), "+v"(c2), "+s"(c3));
   }
 
-  __device__ __forceinline__ double operator()(double z) const {
-    const double shifted = z + 105553116266496.0;
-    const double f = z - (shifted - 105553116266496.0);
+  // Of a logit no lower than lowest_of(max).
+  __device__ __forceinline__ double inside(float l, double max, const Scale& scale) const {
+    constexpr double kRound = 211106232532992.0;
+    const double below = static_cast<double>(l) - max;
+    const double shifted = __builtin_fma(below, scale.c, kRound);
+    const double f = __builtin_fma(below, scale.c, kRound - shifted);
     const uint32_t k = static_cast<uint32_t>(__builtin_bit_cast(unsigned long long, shifted));
-    const double t = table[k & (kExp2Entries - 1)];
+    const uint2 entry = table[k & (kExp2Entries - 1)];
+    const uint32_t high = entry.y + (k << 15);
+    const double t = __builtin_bit_cast(double, (static_cast<unsigned long long>(high) << 32) | entry.x);
     double q = __builtin_fma(c3, f, c2);
     q = __builtin_fma(q, f, c1);
     q = __builtin_fma(q, f, c0);
-    const unsigned long long bits = __builtin_bit_cast(unsigned long long, __builtin_fma(t * f, q, t));
-    const uint32_t high = static_cast<uint32_t>(bits >> 32) + ((k >> 6) << 20);
-    const bool inside = z >= -1020.0;
-    const uint32_t lo = inside ? static_cast<uint32_t>(bits) : 0u, hi = inside ? high : 0u;
-    return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
+    return __builtin_fma(t * f, q, t);
+  }
+
+  // Of any logit but infinity: 0 below the lowest and for NaN.
+  __device__ __forceinline__ double operator()(float l, float max, const Scale& scale) const {
+    const double lowest = fmax(lowest_of(max, scale), -static_cast<double>(FLT_MAX));
+    const bool weighs = static_cast<double>(l) >= lowest;
+    const double w = inside(weighs ? l : max, max, scale);
+    return weighs ? w : 0.0;
   }
 };
-
-constexpr double kLog2e = 1.44269504088896340736;
 
 template <int kMask>
 __device__ __forceinline__ double xor_lane_f64(double v) {
@@ -179,25 +216,17 @@ __device__ __forceinline__ double read_lane_f64(double v, int lane) {
   return __builtin_bit_cast(double, (static_cast<unsigned long long>(h) << 32) | l);
 }
 
-// A logit as it counts: NaN as -inf, -0 as 0 (equal logits tie on the index).
-__device__ __forceinline__ float clean_logit(float l) { return fmaxf(l, -__builtin_huge_valf()) + 0.0f; }
-
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
-
-// exp((l - max) / T) of a logit, c = log2(e) / T.
-__device__ __forceinline__ double logit_weight(const Exp2& exp2, float l, double max, double c) {
-  return exp2((static_cast<double>(l) - max) * c);
-}
 
 // Probability of index i with logit l in a row's distribution.
 __device__ __forceinline__ double probability(const Exp2& exp2, const RowStats& r, double inv_sum, float l, int i,
-                                              double c) {
-  return r.sum > 0.0 ? logit_weight(exp2, clean_logit(l), r.max, c) * inv_sum : (i == r.hot ? 1.0 : 0.0);
+                                              const Scale& scale) {
+  return r.sum > 0.0 ? exp2(l, r.max, scale) * inv_sum : (i == r.hot ? 1.0 : 0.0);
 }
 
 // Four logits of a row from index `first`; -inf behind the vocabulary's end.
 __device__ __forceinline__ void load_logits(float* out, const float* row, int first, int vocab, bool vectors) {
-  if (vectors && first + 4 <= vocab) {
+  if (vectors && first <= vocab - 4) {
     const float4 v = *reinterpret_cast<const float4*>(row + first);
     out[0] = v.x;
     out[1] = v.y;
@@ -205,7 +234,7 @@ __device__ __forceinline__ void load_logits(float* out, const float* row, int fi
     out[3] = v.w;
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = first + j < vocab ? row[first + j] : -__builtin_huge_valf();
+    for (int j = 0; j < 4; ++j) out[j] = j < vocab - first ? row[first + j] : -__builtin_huge_valf();
   }
 }
 
@@ -247,7 +276,7 @@ __device__ __forceinline__ RowPlace place_row(const VerifyArgs& a, int row, int 
 }
 
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ double lds_table[kExp2Entries];
+  __shared__ uint2 lds_table[kExp2Entries];
   const int part = static_cast<int>(blockIdx.x) * kVerifyWaves + (static_cast<int>(threadIdx.x) >> 6);
   const int row = blockIdx.y;
   const bool is_draft = blockIdx.z != 0;
@@ -282,10 +311,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
   if (is_draft) load();
   float max = -__builtin_huge_valf();
 #pragma unroll
-  for (int j = 0; j < kPerLane; ++j) {
-    l[j] = clean_logit(l[j]);
-    max = fmaxf(max, l[j]);
-  }
+  for (int j = 0; j < kPerLane; ++j) max = fmaxf(max, l[j]);  // NaN counts as -inf
   max = wave_max(max);
   double sum = 0.0;
   int index = INT_MAX;
@@ -293,16 +319,29 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
 #pragma unroll
     for (int j = kPerLane - 1; j >= 0; --j) {
       const int i = first + 256 * (j / 4) + (j & 3);
-      if (l[j] == max && i < a.vocab) index = i;
+      if (fmaxf(l[j], -__builtin_huge_valf()) == max && i < a.vocab) index = i;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) index = min(index, __shfl_xor(index, o, 64));
   } else {
-    const double c = kLog2e / static_cast<double>(t);
+    const Scale scale = scale_of(t);
     const double m = max;
+    const double lowest = lowest_of(max, scale);
     const Exp2 exp2(lds_table);
+    if (lowest >= -static_cast<double>(FLT_MAX)) {
+      // Beside the 1 of the largest, 2^-1020 for a logit below the lowest is
+      // nothing: one operation, where a choice of 0 takes three.
+      const float low = float_above(lowest);
 #pragma unroll
-    for (int j = 0; j < kPerLane; ++j) sum += logit_weight(exp2, l[j], m, c);
+      for (int j = 0; j < kPerLane; ++j) {
+        sum += exp2.inside(__builtin_amdgcn_fmed3f(l[j], low, max), m, scale);  // NaN is the lowest
+      }
+    } else {
+      // A temperature so high that every finite logit weighs something, and
+      // -inf nothing.
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) sum += exp2(l[j], max, scale);
+    }
     sum = wave_sum_f64(sum);
   }
   if (lane == 0) {
@@ -311,7 +350,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
 }
 
 // A row's parts joined, by one wave; every lane gets the result.
-__device__ __forceinline__ RowStats join_row(const Exp2& exp2, const PartStats* stats, int parts, double c) {
+__device__ __forceinline__ RowStats join_row(const Exp2& exp2, const PartStats* stats, int parts,
+                                             const Scale& scale) {
   // Two parts a lane at once, which is all of a vocabulary up to 131072.
   PartStats s[2];
   float max = -__builtin_huge_valf();
@@ -328,23 +368,23 @@ __device__ __forceinline__ RowStats join_row(const Exp2& exp2, const PartStats* 
 #pragma unroll
     for (int k = 0; k < 2; ++k) index = s[k].max == to ? min(index, s[k].index) : index;
     if (finite(to)) {
-      if (max != to) sum = finite(max) ? sum * exp2((static_cast<double>(max) - to) * c) : 0.0;
+      if (max != to) sum = finite(max) ? sum * exp2(max, to, scale) : 0.0;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (finite(s[k].max)) sum += s[k].sum * exp2((static_cast<double>(s[k].max) - to) * c);
+        if (finite(s[k].max)) sum += s[k].sum * exp2(s[k].max, to, scale);
       }
     }
     max = to;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) index = min(index, __shfl_xor(index, o, 64));
-  return RowStats{max, finite(max) ? wave_sum_f64(sum) : 0.0, index};
+  return RowStats{finite(max) ? wave_sum_f64(sum) : 0.0, max, index};
 }
 
 struct DrawLds {
   int stop[kVerifyWaves];
   RowStats target[kVerifyWaves], draft[kVerifyWaves];
-  double table[kExp2Entries];
+  uint2 table[kExp2Entries];
   int last;          // this block's sum was the last
   int part;          // of the drawn index; -1: no part has a weight
   double before;     // running sum before that part
@@ -482,7 +522,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
   }
   const int drafts = min(count - 1, a.max_draft);
   const bool greedy = !(t > 0.0f);
-  const double c = greedy ? 0.0 : kLog2e / static_cast<double>(t);
+  const Scale scale = scale_of(greedy ? 1.0f : t);
   const Exp2 exp2(lds.table);
   // The first row that stops: its draft is not kept, or it is the last. A wave
   // a row, so that rows do not wait for each other's reads.
@@ -501,16 +541,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
       const size_t place = static_cast<size_t>(row) * a.logits_stride + (inside ? x : 0);
       const float target_logit = sampled ? a.target[place] : 0.0f;
       const float draft_logit = sampled && a.draft != nullptr ? a.draft[place] : 0.0f;
-      const RowStats target = join_row(exp2, stats, a.parts, c);
-      RowStats draft{0.0, 0.0, x};
+      const RowStats target = join_row(exp2, stats, a.parts, scale);
+      RowStats draft{0.0, 0.0f, x};
       if (sampled && a.draft != nullptr) {
-        const RowStats d = join_row(exp2, stats + a.parts, a.parts, c);
+        const RowStats d = join_row(exp2, stats + a.parts, a.parts, scale);
         draft.max = d.max;
         draft.sum = d.sum;
       }
       if (sampled) {
-        const double p = probability(exp2, target, 1.0 / target.sum, target_logit, x, c);
-        const double q = draft.sum > 0.0 ? probability(exp2, draft, 1.0 / draft.sum, draft_logit, x, c) : 1.0;
+        const double p = probability(exp2, target, 1.0 / target.sum, target_logit, x, scale);
+        const double q = draft.sum > 0.0 ? probability(exp2, draft, 1.0 / draft.sum, draft_logit, x, scale) : 1.0;
         stop = !(inside && static_cast<double>(u) * q < p);
       } else {
         stop = i == drafts || x != target.hot;
@@ -540,7 +580,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
   if (subtract) {
     const double inv_p = 1.0 / target.sum, inv_q = 1.0 / draft.sum;
     auto weight_of = [&](float p, float q, int i) {
-      return fmax(probability(exp2, target, inv_p, p, i, c) - probability(exp2, draft, inv_q, q, i, c), 0.0);
+      return fmax(probability(exp2, target, inv_p, p, i, scale) - probability(exp2, draft, inv_q, q, i, scale), 0.0);
     };
     double* totals = a.totals + static_cast<size_t>(b) * a.parts;
     const int part = static_cast<int>(blockIdx.x) * kVerifyWaves + wave;
@@ -579,9 +619,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         [&](int i) {
           if (!(target.sum > 0.0)) return target.hot / kPart == i ? 1.0 : 0.0;
           const PartStats s = stats[i];
-          return finite(s.max) ? s.sum * exp2((static_cast<double>(s.max) - target.max) * c) : 0.0;
+          return finite(s.max) ? s.sum * exp2(s.max, target.max, scale) : 0.0;
         },
-        [&](float p, float, int i) { return probability(exp2, target, 1.0, p, i, c); });
+        [&](float p, float, int i) { return probability(exp2, target, 1.0, p, i, scale); });
   }
   for (int i = threadIdx.x; i <= a.max_draft; i += kVerifyThreads) {
     ids[i] = i < kept ? a.draft_ids[first + i] : (i == kept ? id : -1);
