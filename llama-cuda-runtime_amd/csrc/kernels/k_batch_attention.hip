@@ -31,10 +31,16 @@
 // the rows and split the keys, 32 a step, each streaming its own keys and
 // values into its own part of LDS with direct loads (no registers, no barrier):
 // the next step's keys are requested as soon as the scores are taken, its values
-// when the products are. Their results meet in LDS.
-// Many rows: bound by the exponentials and, at head_dim 128, by LDS reads and
-// the matrix cores. The waves share 64-key tiles, staged four deep, and split
-// the rows, 32 each.
+// when the products are. Their results meet in LDS. 64 sequences over 0.7 GB of
+// cache (head_dim 64, bf16) 115 us, 6.2 TB/s; a copy kernel reads 7.0.
+// Many rows: bound by the exponentials (16 cycles each on the vector units) and,
+// at head_dim 128, by LDS reads and the matrix cores. The waves share 64-key
+// tiles, staged three or four deep, and split the rows, 32 each. A tile's scores
+// are all taken before its first weights, so that products and exponentials of
+// its halves overlap in a wave: 32 keys at a time were 3 to 15 % slower. Four
+// chunks of 1000 tokens, each behind 4000 positions, 165 us, 0.89 PFLOP/s; the
+// vector units are then busy for three quarters of it. Short prompts lose to
+// the pieces' first loads and to partials: one of 2048 takes 47 us, 0.37.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>

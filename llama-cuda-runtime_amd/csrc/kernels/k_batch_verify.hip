@@ -15,8 +15,14 @@
 // again in the second. The exponentials and sums are fp64: the running sum over
 // 128256 weights has intervals of 1e-5 and less, of which fp32 weights (6e-8
 // each, and as much in p's and q's normalisers) would give some draws to a
-// neighbour. gfx950 runs fp64 fma at the fp32 rate, so that a logit's 13 fp64
-// operations take about as long as its 4 bytes.
+// neighbour. gfx950 runs fp64 fma at the fp32 rate, so that a logit's 17
+// operations (10 of them fp64) take about as long as its 4 bytes: 332 rows of
+// 128256 logits (170 MB) in 40 us, of which the vector units are busy for 25 and
+// the memory, at 7 TB/s, for 24.
+// The draw of 64 sequences takes 23 us, the rows of rejected drafts (half of
+// them, 1 MB each) and a chain of a dozen dependent reads and exchanges; alone,
+// one sequence's takes 8. Blocks of eight waves, which look at eight rows at
+// once, were slower (25 us): more waves wait for the slowest.
 // Which block arrives last decides who computes, not what: all sums have a fixed
 // order.
 #include <algorithm>
@@ -131,7 +137,8 @@ __device__ __forceinline__ float float_above(double v) {
 // a running sum over a vocabulary hands a draw of 1e-8 to a neighbour), times the
 // table's 2^((k mod 32) / 32), and k / 32 added to the exponent. 32 entries of 8
 // bytes lie on banks of their own, so that 64 lanes with an entry each read them
-// without conflicts. MEASURED
+// without conflicts. The statistics of 332 rows of 128256 take 40 us, with 64
+// entries 42, with a polynomial over [-1/2, 1/2] and no table 48.
 // The coefficients are kept in registers, scalar but for one (an instruction
 // takes one scalar): left to the compiler, each is moved before each use.
 struct Exp2 {
@@ -404,26 +411,42 @@ __device__ __forceinline__ int draw_index(DrawLds& lds, const VerifyArgs& a, flo
   const int lane = lane_id();
   const int wave = static_cast<int>(threadIdx.x) >> 6;
   if (wave == 0) {
+    // 256 parts at once, so that their reads do not wait for each other; all of
+    // a vocabulary up to 262144 is read once.
+    double v[4];
+    auto load = [&](int base) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = base + 64 * k + lane;
+        v[k] = i < a.parts ? total_of(i) : 0.0;
+      }
+    };
     double whole = 0.0;
-    for (int base = 0; base < a.parts; base += 64) {
-      const double v = base + lane < a.parts ? total_of(base + lane) : 0.0;
-      whole += read_lane_f64(wave_inclusive_scan_f64(v), 63);
+    for (int base = 0; base < a.parts; base += 256) {
+      load(base);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) whole += read_lane_f64(wave_inclusive_scan_f64(v[k]), 63);
     }
     const double goal = static_cast<double>(u) * whole;
     double before = 0.0, part_before = 0.0;
     int part = -1;
-    for (int base = 0, hit = 0; base < a.parts && hit == 0; base += 64) {
-      const double v = base + lane < a.parts ? total_of(base + lane) : 0.0;
-      const double incl = wave_inclusive_scan_f64(v);
-      const unsigned long long past = __ballot(v > 0.0 && before + incl > goal);
-      const unsigned long long weighty = __ballot(v > 0.0);
-      const int at = past != 0 ? __ffsll(past) - 1 : (weighty != 0 ? 63 - __clzll(weighty) : -1);
-      if (at >= 0) {
-        part = base + at;
-        part_before = before + read_lane_f64(incl - v, at);
-        hit = past != 0 ? 1 : 0;
+    bool hit = false;
+    for (int base = 0; base < a.parts && !hit; base += 256) {
+      if (a.parts > 256) load(base);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (hit) continue;
+        const double incl = wave_inclusive_scan_f64(v[k]);
+        const unsigned long long past = __ballot(v[k] > 0.0 && before + incl > goal);
+        const unsigned long long weighty = __ballot(v[k] > 0.0);
+        const int at = past != 0 ? __ffsll(past) - 1 : (weighty != 0 ? 63 - __clzll(weighty) : -1);
+        if (at >= 0) {
+          part = base + 64 * k + at;
+          part_before = before + read_lane_f64(incl - v[k], at);
+          hit = past != 0;
+        }
+        before += read_lane_f64(incl, 63);
       }
-      before += read_lane_f64(incl, 63);
     }
     if (lane == 0) {
       lds.part = part;
@@ -445,7 +468,7 @@ __device__ __forceinline__ int draw_index(DrawLds& lds, const VerifyArgs& a, flo
   bool weighty[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const double w = i0 + e < a.vocab ? weight_of(lp[e], lq[e], i0 + e) : 0.0;
+    const double w = e < a.vocab - i0 ? weight_of(lp[e], lq[e], i0 + e) : 0.0;
     sum += w;
     run[e] = sum;
     weighty[e] = w > 0.0;
@@ -487,8 +510,7 @@ __device__ __forceinline__ int draw_index(DrawLds& lds, const VerifyArgs& a, flo
 // past the caches of one XCD; that the exchange has returned says that its value
 // is where they all look, so that a count taken after it counts it. (Releasing
 // and acquiring with the count instead writes back and drops the whole L2, once
-// a block: 68 us against 24 for 64
-// sequences of 128256 logits.)
+// a block: 68 us against 24 for 64 sequences of 128256 logits.)
 __device__ __forceinline__ void publish(double* at, double value) {
   const unsigned long long before =
       __hip_atomic_exchange(reinterpret_cast<unsigned long long*>(at), __builtin_bit_cast(unsigned long long, value),
@@ -594,7 +616,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         if (draft_row != nullptr) load_logits(lq, draft_row, i0, a.vocab, a.vectors);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (i0 + e < a.vocab) rest += weight_of(lp[e], lq[e], i0 + e);
+          if (e < a.vocab - i0) rest += weight_of(lp[e], lq[e], i0 + e);
         }
       }
       rest = wave_sum_f64(rest);
