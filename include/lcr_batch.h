@@ -104,13 +104,17 @@ int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view, const voi
  *   out: [tokens][num_heads][head_dim]
  * view->page_table: [batch][table_stride]. max_new: no sequence has more rows
  * than that (its further rows come out as zeros). head_dim is at most 256;
- * 64 and 128 with 16-byte aligned rows run on the matrix cores.
+ * 64 and 128 with 16-byte aligned rows run on the matrix cores, and
+ * fastest with a page_size that is a multiple of 16. Tables hold up to 2^30
+ * positions.
  * A row that sees no position (lengths[b] < n) is zeros. Positions behind
  * table_stride pages do not exist. A sequence with a page outside 0 ..
  * pool_pages - 1 among those it reads may come out as NaN.
  * With a workspace of lcr_batch_attention_workspace_bytes (16-byte aligned)
- * long caches of few rows are split over the device; without one (NULL, 0, or
- * a smaller one) nothing is split. */
+ * tables of more than 1024 positions have their keys split over the device;
+ * without one (NULL, 0, or a smaller one) nothing is split. Where a sequence is
+ * split depends on the lengths of all, and the rounding of its sums with it; the
+ * same call gives the same bits. */
 int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* view, const int32_t* row_starts,
                         const int32_t* lengths, int batch, int tokens, int max_new, int num_heads,
                         int heads_per_kv, int table_stride, int pool_pages, int q_row_stride, float scale,

@@ -134,6 +134,13 @@ constexpr int kFewRows = 32;
 // waves, the output.
 constexpr int kUnitSteps = 3;
 constexpr int kStepKeys = 64;
+// Few rows beside many: a step of 64 keys takes less than one of many rows, which
+// keeps the vector units busy while the cache is read. 16 sequences of one token
+// beside two chunks of 1000, with 64, 96, 128 and 192 keys a step: heads of 64 77,
+// 74, 74 and 79 us, of 128 121, 105, 95 and 90; 64 beside two of 512: 102, 95, 99
+// and 97, and 248, 184, 156 and 147.
+template <int kHeadDim>
+constexpr int kFewStepKeys = kHeadDim == 64 ? 96 : 192;
 // A unit of at most so many steps is not cut: its partials and their join cost
 // more than the share it lengthens. Eight prompts of 256 tokens 20 us, cut 27; one
 // of 2048 50, cut 51. With 16 steps 64 sequences of 600 positions took 20 us for
@@ -167,7 +174,7 @@ __device__ __forceinline__ int steps_before_tile(const FlashPlan& plan, const Se
 }
 
 // kMany: sequences may have more rows than a tile of few.
-template <bool kMany>
+template <int kHeadDim, bool kMany>
 __device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const FlashPlan& plan, int b) {
   const int lo = a.row_starts[b], hi = a.row_starts[b + 1];
   const int length = a.lengths[b];
@@ -184,7 +191,9 @@ __device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const 
   // up to the last tile, and that
   s.steps = s.tiles;
   if (plan.split && s.tiles > 0) {
-    s.steps = kUnitSteps + max(s.visible, s.tokens) / kStepKeys;
+    const int keys = max(s.visible, s.tokens);
+    const bool few = s.tokens * a.group <= kFewRows;
+    s.steps = kUnitSteps + (kMany && few ? keys / kFewStepKeys<kHeadDim> : keys / kStepKeys);
     if (kMany && s.tiles > 1) s.steps += steps_before_tile(plan, s, s.tiles - 1);
   }
   return s;
@@ -205,7 +214,7 @@ struct ShareStart {
 
 // Where a kv head's share `index` begins: the prefix sums of the sequences'
 // steps, taken by the whole block.
-template <bool kMany, int kThreads>
+template <int kHeadDim, bool kMany, int kThreads>
 __device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const FlashPlan& plan, int index,
                                                  int* lds_sums, ShareStart* lds_found) {
   constexpr int kWaves = kThreads / 64;
@@ -216,7 +225,7 @@ __device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const F
   for (int k = 0; k < per; ++k) {
     const int b = t * per + k;
     if (b < a.batch) {
-      seq = load_sequence<kMany>(a, plan, b);
+      seq = load_sequence<kHeadDim, kMany>(a, plan, b);
       mine += seq.steps;
     }
   }
@@ -241,7 +250,7 @@ __device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const F
     for (int k = 0; k < per; ++k) {
       const int b = t * per + k;
       if (b >= a.batch) break;
-      if (per > 1) seq = load_sequence<kMany>(a, plan, b);
+      if (per > 1) seq = load_sequence<kHeadDim, kMany>(a, plan, b);
       if (at < before + seq.steps) {
         *lds_found = ShareStart{total, share, before, b, seq};
         break;
@@ -998,7 +1007,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
   const int block = static_cast<int>(blocks % 8u == 0 ? blockIdx.x % 8u * (blocks / 8u) + blockIdx.x / 8u : blockIdx.x);
   const int kv = plan.by_shares(block);
   const ShareStart found =
-      find_share<kMany, Shape::kThreads>(a, plan, block - kv * plan.shares, lds.sums, &lds.found);
+      find_share<kHeadDim, kMany, Shape::kThreads>(a, plan, block - kv * plan.shares, lds.sums, &lds.found);
   if (plan.split && threadIdx.x == 0) plan.cuts[block].rows = 0;
   if (found.sequence < 0) return;
   int b = found.sequence;
@@ -1042,7 +1051,8 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
     const bool whole = !plan.split || stop - start <= kWholeSteps;
     if (!whole && (start < at || stop > end)) {
       // steps into the unit, in keys
-      auto cut = [&](int steps) { return steps >= (p.seen_last + kStepKeys - 1) / kStepKeys ? p.seen_last : steps * kStepKeys; };
+      const int keys = kMany && single ? kFewStepKeys<kHeadDim> : kStepKeys;
+      auto cut = [&](int steps) { return steps >= (p.seen_last + keys - 1) / keys ? p.seen_last : steps * keys; };
       p.slot = 2 * block + (start < at ? 0 : 1);
       if (start < at) p.key0 = cut(at - start);
       if (stop > end) p.key1 = cut(end - start);
@@ -1075,7 +1085,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
       before += seq.steps;
       do {  // the next sequence that has rows
         if (++b == a.batch) return;
-        seq = uniform(load_sequence<kMany>(a, plan, b));
+        seq = uniform(load_sequence<kHeadDim, kMany>(a, plan, b));
       } while (seq.tiles == 0);
     }
     if constexpr (kMany) __syncthreads();  // the tiles and the flag are free again
@@ -1283,12 +1293,22 @@ void launch_flash_kernels(const BatchAttnArgs& a, const FlashPlan& plan, hipStre
 }
 
 template <int kHeadDim>
+int flash_tile_tokens(int group) {
+  return std::max(1, FlashShape<kHeadDim>::kTileRows / group);
+}
+
+// A unit a block: at most one short tile a sequence beside the full ones.
+template <int kHeadDim>
+long long most_flash_units(const BatchAttnArgs& a) {
+  return a.tokens / flash_tile_tokens<kHeadDim>(a.group) + static_cast<long long>(a.batch);
+}
+
+template <int kHeadDim>
 void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  using Shape = FlashShape<kHeadDim>;
   FlashPlan plan{};
   const int kv_heads = a.view.num_kv_heads;
   plan.group_magic = static_cast<uint32_t>((65536 + a.group - 1) / a.group);
-  plan.tile_tokens = std::max(1, Shape::kTileRows / a.group);
+  plan.tile_tokens = flash_tile_tokens<kHeadDim>(a.group);
   plan.by_page = FastDivide::by(static_cast<uint32_t>(a.view.page_size));
   plan.by_tile = FastDivide::by(static_cast<uint32_t>(plan.tile_tokens));
   plan.scale_log2e = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
@@ -1298,15 +1318,19 @@ void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   // each, cut and not: 8 of 1000 14.4 and 11.7 us, 64 of 600 18.2 and 13.1, 128 of
   // 1000 36.4 and 35.0; 8 of 2000 14.3 and 18.0.
   constexpr int kCutPositions = 1024;
-  if (a.held > kCutPositions && workspace != nullptr &&
+  const bool many = many_rows_possible(a.max_new, a.group);
+  // Steps are counted in 32 bits. Where a call's could pass them, it has units
+  // enough to fill the device uncut.
+  const long long most_units = many ? most_flash_units<kHeadDim>(a) : a.batch;
+  const long long most_steps = kUnitSteps + 1 + std::max(a.held, std::min(a.max_new, a.tokens)) / kStepKeys;
+  if (a.held > kCutPositions && most_units * most_steps <= INT32_MAX / 2 && workspace != nullptr &&
       workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
     plan.split = 1;
-    plan.shares = flash_shares<kHeadDim>(kv_heads, many_rows_possible(a.max_new, a.group));
+    plan.shares = flash_shares<kHeadDim>(kv_heads, many);
     plan.cuts = static_cast<CutUnit*>(workspace);
     plan.partials = reinterpret_cast<float*>(plan.cuts + static_cast<size_t>(plan.shares) * kv_heads);
   } else {
-    // A unit a block: at most one short tile a sequence beside the full ones.
-    plan.shares = a.tokens / plan.tile_tokens + a.batch;
+    plan.shares = static_cast<int>(most_flash_units<kHeadDim>(a));
   }
   plan.by_shares = FastDivide::by(static_cast<uint32_t>(plan.shares));
   const long long most = static_cast<long long>(a.max_new) * a.group;
@@ -1370,6 +1394,8 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
   CAPI_CHECK(table_stride > 0 && pool_pages > 0, "batch attention needs page tables and a pool of at least one page");
   CAPI_CHECK(static_cast<long long>(table_stride) * view->page_size <= INT32_MAX,
              "tables of " << table_stride << " pages of " << view->page_size << " hold positions past 32 bits");
+  CAPI_CHECK(static_cast<long long>(table_stride) * view->page_size <= (1 << 30),
+             "batch attention takes tables of up to 2^30 positions");
   CAPI_CHECK(view->page_stride >= 0 && view->head_stride >= 0, "batch attention needs non-negative cache strides");
   CAPI_CHECK(q_row_stride >= static_cast<long long>(num_heads) * view->head_dim,
              "query rows of " << num_heads << " heads cannot lie " << q_row_stride << " elements apart");
@@ -1385,7 +1411,15 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
                   lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride,
                   table_stride * view->page_size, scale};
   auto s = static_cast<hipStream_t>(stream);
-  if (flash_takes(a)) {
+  const bool flash = flash_takes(a);
+  // A launch has fewer than 2^32 threads in all.
+  const long long units = static_cast<long long>(tokens) * num_heads;
+  const long long blocks = !flash ? (units + kGenericWaves - 1) / kGenericWaves
+                           : view->num_kv_heads * (view->head_dim == 64 ? most_flash_units<64>(a) : most_flash_units<128>(a));
+  const int threads = !flash ? kGenericThreads : view->head_dim == 64 ? FlashShape<64>::kThreads : FlashShape<128>::kThreads;
+  CAPI_CHECK(blocks * threads <= UINT32_MAX, "batch attention of " << tokens << " rows of " << num_heads
+                                                                   << " heads needs more than 2^32 threads");
+  if (flash) {
     if (view->head_dim == 64) {
       launch_flash<64>(a, workspace, workspace_bytes, s);
     } else {
@@ -1394,9 +1428,7 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
     CAPI_LAUNCHED();
     return LCR_OK;
   }
-  const long long units = static_cast<long long>(tokens) * num_heads;
-  batch_attention_generic_kernel<<<static_cast<unsigned>((units + kGenericWaves - 1) / kGenericWaves), kGenericThreads,
-                                   0, s>>>(a);
+  batch_attention_generic_kernel<<<static_cast<unsigned>(blocks), kGenericThreads, 0, s>>>(a);
   CAPI_LAUNCHED();
   return LCR_OK;
 }

@@ -173,6 +173,12 @@ __global__ __launch_bounds__(kHeadsThreads) void batch_heads_generic_kernel(Head
   }
 }
 
+// Lanes that a head takes.
+int head_lanes(const HeadsArgs& a, bool aligned) {
+  const int d = a.view.head_dim;
+  return aligned && (d == 64 || d == 128 || d == 256) ? d / 16 : 64;
+}
+
 template <int kHeadDim>
 void launch_heads(const HeadsArgs& a, hipStream_t s) {
   const long long lanes = static_cast<long long>(a.tokens) * (a.num_heads + 2 * a.view.num_kv_heads) * (kHeadDim / 16);
@@ -208,7 +214,6 @@ extern "C" int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view
   CAPI_CHECK(view->page_stride >= 0 && view->head_stride >= 0, "batch_norm_rope_write_kv needs non-negative cache strides");
   const long long widest = static_cast<long long>(std::max(num_heads, view->num_kv_heads)) * view->head_dim;
   CAPI_CHECK(src_row_stride >= widest, "rows of " << widest << " elements cannot lie " << src_row_stride << " apart");
-  // 64 lanes a head at most, 256 a block, blocks counted in 31 bits
   CAPI_CHECK(tokens * heads <= (1ll << 32), "batch_norm_rope_write_kv takes up to 2^32 heads in all, got "
                                                 << tokens * heads);
   CAPI_CHECK(positions != nullptr && slots != nullptr, "batch_norm_rope_write_kv needs positions and slots");
@@ -239,6 +244,9 @@ extern "C" int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view
                        on_16_bytes(q_norm) && on_16_bytes(k_norm) && on_16_bytes(rope_table) &&
                        on_16_bytes(view->keys) && on_16_bytes(view->values) && src_row_stride % 8 == 0 &&
                        view->page_stride % 8 == 0 && view->head_stride % 8 == 0;
+  // A launch has fewer than 2^32 threads in all.
+  CAPI_CHECK(tokens * heads * head_lanes(a, aligned) <= UINT32_MAX - kHeadsThreads,
+             "batch_norm_rope_write_kv of " << tokens * heads << " heads needs more than 2^32 threads");
   if (aligned && view->head_dim == 64) {
     launch_heads<64>(a, s);
   } else if (aligned && view->head_dim == 128) {

@@ -152,3 +152,16 @@ def test_verify_of_no_sequences(lib):
     assert verify_call(lib, batch=0, temperatures=None) == 0
     assert lib.lcr_batch_verify_workspace_bytes(0, 5, 100) == 0
     assert lib.lcr_batch_verify_workspace_bytes(2, 5, 0) == 0
+
+
+def test_sizes_past_a_launch(lcr, lib):
+    """More than 2^32 threads: refused, by the layout that the call would use."""
+    refused(lib, heads_call(lcr, lib, tokens=1 << 28), "2^32 threads")
+    refused(lib, heads_call(lcr, lib, dict(head_dim=62), tokens=1 << 23), "2^32 threads")
+    refused(lib, attention_call(lcr, lib, dict(head_dim=72), tokens=1 << 23, q_row_stride=576), "2^32 threads")
+    refused(lib, attention_call(lcr, lib, dict(num_kv_heads=1), tokens=1 << 24, num_heads=80, heads_per_kv=80,
+                                q_row_stride=5120), "2^32 threads")
+
+
+def test_attention_refuses_positions_past_2_to_30(lcr, lib):
+    refused(lib, attention_call(lcr, lib, table_stride=(1 << 26) + 1), "up to 2^30 positions")
