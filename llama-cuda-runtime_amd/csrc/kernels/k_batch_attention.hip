@@ -142,10 +142,12 @@ constexpr int kStepKeys = 64;
 template <int kHeadDim>
 constexpr int kFewStepKeys = kHeadDim == 64 ? 96 : 192;
 // A unit of at most so many steps is not cut: its partials and their join cost
-// more than the share it lengthens. Eight prompts of 256 tokens 20 us, cut 27; one
-// of 2048 50, cut 51. With 16 steps 64 sequences of 600 positions took 20 us for
-// 18, and a prompt of 1024 tokens 37 for 30.
-constexpr int kWholeSteps = 8;
+// more than the share it lengthens. With 0, 4, 8 and 16: eight prompts of 256
+// tokens 28, 26, 20 and 20 us, one of 2048 49, -, 48 and 47, two of 2048 65, -, 65
+// and 67; few rows, which have less to join, 64 of 600 positions 18.2, 17.9, 19.1
+// and 20.3, 32 of 1000 16.2, 16.3, 16.8 and 19.6.
+template <bool kMany>
+constexpr int kWholeSteps = kMany ? 8 : 4;
 
 // A sequence's share of the work, in tokens and steps of one kv head.
 struct Sequence {
@@ -1048,7 +1050,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
     p.key1 = p.seen_last;
     p.slot = -1;
     // A short unit is not cut: it goes to the share that it begins in.
-    const bool whole = !plan.split || stop - start <= kWholeSteps;
+    const bool whole = !plan.split || stop - start <= kWholeSteps<kMany>;
     if (!whole && (start < at || stop > end)) {
       // steps into the unit, in keys
       const int keys = kMany && single ? kFewStepKeys<kHeadDim> : kStepKeys;
