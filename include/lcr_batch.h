@@ -111,7 +111,7 @@ int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view, const voi
  * table_stride pages do not exist. A sequence with a page outside 0 ..
  * pool_pages - 1 among those it reads may come out as NaN.
  * With a workspace of lcr_batch_attention_workspace_bytes (16-byte aligned)
- * tables of more than 1024 positions have their keys split over the device;
+ * tables of more than 768 to 1024 positions have their keys split over the device;
  * without one (NULL, 0, or a smaller one) nothing is split, which is one launch
  * less for sequences known to be short. Where a sequence is
  * split depends on the lengths of all, and the rounding of its sums with it; the

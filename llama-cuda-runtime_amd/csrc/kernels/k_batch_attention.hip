@@ -266,15 +266,15 @@ __device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const F
                     uniform(found.seq)};
 }
 
-// Waits for direct loads and for LDS reads, across which the compiler moves no
-// memory access.
+// Waits for direct loads, and for LDS reads and writes, across which the compiler
+// moves no memory access.
 template <int kCount>
 __device__ __forceinline__ void loads_landed() {
   asm volatile("" : : : "memory");
   wait_stage_landed<kCount>();
   asm volatile("" : : : "memory");
 }
-__device__ __forceinline__ void reads_returned() { loads_landed<63>(); }
+__device__ __forceinline__ void lds_settled() { loads_landed<63>(); }
 
 // One block's part of a unit.
 struct Piece {
@@ -328,6 +328,7 @@ struct FlashLds {
   int sums[FlashShape<kHeadDim>::kWaves];
   ShareStart found;
   int bad;  // a page outside the pool was read
+  int special[2];  // many rows: the last tile of even and of odd number whose values hold infinities or NaN
 };
 
 #if defined(LCR_ELEM_FP16)
@@ -761,7 +762,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
     const bool whole = key0 + 32 <= all_seen;
     TileWork<kHeadDim, kRF, 2> work;
     work.scores(rows, key_tile(t));
-    reads_returned();  // the keys have been read
+    lds_settled();  // the keys have been read
     if (more) issue(Keys{}, t + kSlots, pages);
     if (!whole) work.mask(rows, key0);
     work.raise_base(rows, plan.scale_log2e);
@@ -779,7 +780,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
       clear_special(value_tile(t), 32 * kHeadDim / 512);
     }
     work.products(rows, value_tile(t), 0);
-    reads_returned();
+    lds_settled();
     if (more) issue(Values{}, t + kSlots, pages);
   }
 
@@ -844,10 +845,11 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   __syncthreads();  // the parts may be loaded into again
 }
 
-// Many rows: the waves split them, 32 each, and share the tiles.
+// Many rows: the waves split them, 32 each, and share the tiles. `tiles_done`:
+// of the block's pieces before, so that a tile's number is its own.
 template <int kHeadDim, bool kWholePages>
 __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAttnArgs& a, const FlashPlan& plan,
-                                          const Piece& p) {
+                                          const Piece& p, int& tiles_done) {
   using Shape = FlashShape<kHeadDim>;
   constexpr int kRF = 2;
   constexpr int kRun = 64 / Shape::kWaves;          // a wave's keys of a tile
@@ -901,16 +903,26 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
     // This wave's loads of the tile have landed (the later tiles' remain);
     // behind the barrier every wave's have, and the tile before is free.
     if (t + kAhead - 1 < tiles) {
-      wait_stage_landed<(kAhead - 1) * 2 * kLoads>();
+      loads_landed<(kAhead - 1) * 2 * kLoads>();
     } else {
-      wait_stage_landed<0>();
+      loads_landed<0>();
+    }
+    // A tile that some row of the unit does not see whole: each wave looks for
+    // infinities and NaN among the values that it loaded. (In all of the tile's,
+    // heads of 128 and a prompt of 133 tokens took 18.4 us for 14.6.) The next tile
+    // of this tile's slot is looked at behind the next barrier, when every wave
+    // has read the slot.
+    const int tile0 = p.key0 + 64 * t;
+    const bool partly = tile0 + 64 > p.seen_first;
+    int* const slot = lds.special + ((tiles_done + t) & 1);
+    if (partly) {
+      const bool found = any_special(stage + (64 + kRun * wave) * kHeadDim, kRun * kHeadDim / 512);
+      if (found && lane == 0) *slot = tiles_done + t;
+      lds_settled();
     }
     plain_barrier();
     if (t + kAhead < tiles) issue(t + kAhead, next_stage, page);
-    // A tile that some row of the unit does not see whole: every wave looks for
-    // infinities and NaN among its values, and finds the same.
-    const int tile0 = p.key0 + 64 * t;
-    const bool special = tile0 + 64 > p.seen_first && any_special(stage + 64 * kHeadDim, kHeadDim / 8);
+    const bool special = partly && uniform(*slot) == tiles_done + t;
     const bool mine = tile0 < any_seen;
     const bool whole = tile0 + 64 <= all_seen;
     elem_t* values = stage + 64 * kHeadDim;
@@ -938,15 +950,16 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
         work.weights(rows, plan.scale_log2e, 0);
         work.mark_special(rows, at);
       }
-      wait_lds();
+      lds_settled();
       plain_barrier();
       static_assert(kHeadDim / 16 <= Shape::kWaves, "a wave clears one group of chunks at most");
       if (wave < kHeadDim / 16) clear_special(at + wave * 512, 1);
-      wait_lds();
+      lds_settled();
       plain_barrier();
       if (mine) work.products(rows, at, 0);
     }
   }
+  tiles_done += max(tiles, 0);
   if (__any(bad != 0) && lane == 0) lds.bad = 1;
   __syncthreads();  // every wave is done with the tiles; the flag is set
   if (!active) return;
@@ -1008,6 +1021,8 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
   const unsigned blocks = gridDim.x;
   const int block = static_cast<int>(blocks % 8u == 0 ? blockIdx.x % 8u * (blocks / 8u) + blockIdx.x / 8u : blockIdx.x);
   const int kv = plan.by_shares(block);
+  // seen by every wave behind the barriers of the search
+  if (threadIdx.x == 0) lds.special[0] = lds.special[1] = -1;
   const ShareStart found =
       find_share<kHeadDim, kMany, Shape::kThreads>(a, plan, block - kv * plan.shares, lds.sums, &lds.found);
   if (plan.split && threadIdx.x == 0) plan.cuts[block].rows = 0;
@@ -1030,6 +1045,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
       }
     }
   }
+  int tiles_done = 0;
   Piece p;
   p.kv = kv;
   p.keys = a.view.keys + static_cast<size_t>(kv) * static_cast<size_t>(a.view.head_stride);
@@ -1075,7 +1091,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
     }
     if (p.rows > 0 && !(whole && start < at)) {
       if (!single) {
-        if constexpr (kMany) many_rows<kHeadDim, kWholePages>(lds, a, plan, p);
+        if constexpr (kMany) many_rows<kHeadDim, kWholePages>(lds, a, plan, p, tiles_done);
       } else {
         few_rows<kHeadDim, kWholePages, kMaxRows == 16 ? 1 : 2, kTileRows>(lds, a, plan, p);
       }
@@ -1318,14 +1334,19 @@ void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   // Tables of at most 1024 positions: no unit is long enough for a cut and its
   // second launch to pay. By the number of sequences and positions, one token
   // each, cut and not: 8 of 1000 14.4 and 11.7 us, 64 of 600 18.2 and 13.1, 128 of
-  // 1000 36.4 and 35.0; 8 of 2000 14.3 and 18.0.
-  constexpr int kCutPositions = 1024;
+  // 1000 36.4 and 35.0; 8 of 2000 14.3 and 18.0. Where the tiles of many rows
+  // leave half of the device without work, 768: heads of 128, 8 on 4, a prompt of
+  // 837 tokens with others (76 units) 33.4 and 37.9, 16 on 8, one of 1000 (64)
+  // 39.3 and 43.9; heads of 64, 8 on 8, one of 900 (64) 19.7 and 22.9, but 8 on 2,
+  // two of 800 (78) 24.2 and 21.3, and 32 on 8, one of 500 (128) 20.1 and 16.1.
   const bool many = many_rows_possible(a.max_new, a.group);
+  const bool half_idle = many && 2 * most_flash_units<kHeadDim>(a) * kv_heads <= device_compute_units();
+  const int cut_positions = half_idle ? 768 : 1024;
   // Steps are counted in 32 bits. Where a call's could pass them, it has units
   // enough to fill the device uncut.
   const long long most_units = many ? most_flash_units<kHeadDim>(a) : a.batch;
   const long long most_steps = kUnitSteps + 1 + std::max(a.held, std::min(a.max_new, a.tokens)) / kStepKeys;
-  if (a.held > kCutPositions && most_units * most_steps <= INT32_MAX / 2 && workspace != nullptr &&
+  if (a.held > cut_positions && most_units * most_steps <= INT32_MAX / 2 && workspace != nullptr &&
       workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
     plan.split = 1;
     plan.shares = flash_shares<kHeadDim>(kv_heads, many);
