@@ -115,7 +115,7 @@ __device__ __forceinline__ T own_register(T v) {
 
 // What the matrix-core kernels need besides. Work is counted in steps of 64
 // keys.
-struct FlashPlan {
+struct TiledPlan {
   uint32_t group_magic;   // r / group = r * group_magic >> 16 for r < 256
   FastDivide by_page;     // by page_size
   FastDivide by_tile;     // by tile_tokens
@@ -168,7 +168,7 @@ __device__ __forceinline__ int keys_seen(const BatchAttnArgs& a, int before, int
 // Steps the tiles before tile i count for: tile j sees up to
 // visible - tokens + (j + 1) tile_tokens keys. An estimate besides what is seen
 // (negative positions, the table's end) only makes a share longer or shorter.
-__device__ __forceinline__ int steps_before_tile(const FlashPlan& plan, const Sequence& s, int i) {
+__device__ __forceinline__ int steps_before_tile(const TiledPlan& plan, const Sequence& s, int i) {
   if (!plan.split) return i;
   const long long tiles = i;
   const long long keys = tiles * max(s.visible - s.tokens, 0) + plan.tile_tokens * (tiles * (tiles + 1) / 2);
@@ -177,7 +177,7 @@ __device__ __forceinline__ int steps_before_tile(const FlashPlan& plan, const Se
 
 // kMany: sequences may have more rows than a tile of few.
 template <int kHeadDim, bool kMany>
-__device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const FlashPlan& plan, int b) {
+__device__ __forceinline__ Sequence load_sequence(const BatchAttnArgs& a, const TiledPlan& plan, int b) {
   const int lo = a.row_starts[b], hi = a.row_starts[b + 1];
   const int length = a.lengths[b];
   Sequence s;
@@ -217,7 +217,7 @@ struct ShareStart {
 // Where a kv head's share `index` begins: the prefix sums of the sequences'
 // steps, taken by the whole block.
 template <int kHeadDim, bool kMany, int kThreads>
-__device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const FlashPlan& plan, int index,
+__device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const TiledPlan& plan, int index,
                                                  int* lds_sums, ShareStart* lds_found) {
   constexpr int kWaves = kThreads / 64;
   const int t = threadIdx.x;
@@ -300,7 +300,7 @@ struct Piece {
 // head_dim 64, three blocks of four waves (168 registers a lane); at 128, one of
 // eight (256).
 template <int kHeadDim>
-struct FlashShape {
+struct TiledShape {
   static constexpr int kWaves = kHeadDim == 64 ? 4 : 8;
   static constexpr int kBlocks = kHeadDim == 64 ? 3 : 1;      // resident a compute unit
   // Of few rows, two: 64 sequences of 8000 positions 115 us, with three 116, and
@@ -322,10 +322,10 @@ struct FlashShape {
 };
 
 template <int kHeadDim>
-struct FlashLds {
-  elem_t ring[FlashShape<kHeadDim>::kRingElems];
-  float stats[FlashShape<kHeadDim>::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
-  int sums[FlashShape<kHeadDim>::kWaves];
+struct TiledLds {
+  elem_t ring[TiledShape<kHeadDim>::kRingElems];
+  float stats[TiledShape<kHeadDim>::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
+  int sums[TiledShape<kHeadDim>::kWaves];
   ShareStart found;
   int bad;  // a page outside the pool was read
   int special[2];  // many rows: the last tile of even and of odd number whose values hold infinities or NaN
@@ -339,9 +339,9 @@ constexpr uint32_t kInfBits = 0x7f80u, kOneBits = 0x3f80u;
 
 // A packed-row fragment's accumulators: rows 16 rf + col, per lane.
 template <int kHeadDim, int kRF>
-struct FlashRows {
-  mfma_in8 q[kRF][FlashShape<kHeadDim>::kSteps];
-  mfma_acc4 o[kRF][FlashShape<kHeadDim>::kDFrags];
+struct TiledRows {
+  mfma_in8 q[kRF][TiledShape<kHeadDim>::kSteps];
+  mfma_acc4 o[kRF][TiledShape<kHeadDim>::kDFrags];
   float base[kRF];  // +inf: no visible key yet
   mfma_acc4 sum[kRF];  // of the row's weights, four times
   int seen[kRF];    // keys the row sees, at most key1
@@ -354,7 +354,7 @@ struct FlashRows {
       sum[rf] = mfma_acc4{0.f, 0.f, 0.f, 0.f};
       up[rf] = down[rf] = 0;
 #pragma unroll
-      for (int df = 0; df < FlashShape<kHeadDim>::kDFrags; ++df) o[rf][df] = mfma_acc4{0.f, 0.f, 0.f, 0.f};
+      for (int df = 0; df < TiledShape<kHeadDim>::kDFrags; ++df) o[rf][df] = mfma_acc4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
@@ -363,7 +363,7 @@ struct FlashRows {
     for (int rf = 0; rf < kRF; ++rf) {
       if (!__any((up[rf] | down[rf]) != 0)) continue;
 #pragma unroll
-      for (int df = 0; df < FlashShape<kHeadDim>::kDFrags; ++df) {
+      for (int df = 0; df < TiledShape<kHeadDim>::kDFrags; ++df) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool plus = (up[rf] >> (4 * df + e) & 1) != 0, minus = (down[rf] >> (4 * df + e) & 1) != 0;
@@ -375,14 +375,14 @@ struct FlashRows {
   }
 };
 
-__device__ __forceinline__ int packed_token(const FlashPlan& plan, int r) {
+__device__ __forceinline__ int packed_token(const TiledPlan& plan, int r) {
   return static_cast<int>((static_cast<uint32_t>(r) * plan.group_magic) >> 16);
 }
 
 // Queries of packed rows row0 + 16 rf + col (those past the unit's rows repeat
 // its last, are never stored and see what that one sees).
 template <int kHeadDim, int kRF>
-__device__ __forceinline__ void load_rows(FlashRows<kHeadDim, kRF>& rows, const BatchAttnArgs& a, const FlashPlan& plan,
+__device__ __forceinline__ void load_rows(TiledRows<kHeadDim, kRF>& rows, const BatchAttnArgs& a, const TiledPlan& plan,
                                           const Piece& p, int row0) {
   const int col = lane_id() & 15;
   const int grp = lane_id() >> 4;
@@ -394,7 +394,7 @@ __device__ __forceinline__ void load_rows(FlashRows<kHeadDim, kRF>& rows, const 
     const elem_t* q = a.q + static_cast<size_t>(p.row0 + token) * a.q_row_stride +
                       static_cast<size_t>(head) * kHeadDim + 8 * grp;
 #pragma unroll
-    for (int ks = 0; ks < FlashShape<kHeadDim>::kSteps; ++ks) rows.q[rf][ks] = as_operand(load16(q + 32 * ks));
+    for (int ks = 0; ks < TiledShape<kHeadDim>::kSteps; ++ks) rows.q[rf][ks] = as_operand(load16(q + 32 * ks));
     rows.seen[rf] = min(keys_seen(a, p.before, token), p.key1);
   }
 }
@@ -403,11 +403,11 @@ __device__ __forceinline__ void load_rows(FlashRows<kHeadDim, kRF>& rows, const 
 // tiles, the compiler's wait for them there is one for every direct load in
 // flight, each time round.
 template <int kHeadDim, int kRF>
-__device__ __forceinline__ void hold_rows(FlashRows<kHeadDim, kRF>& rows) {
+__device__ __forceinline__ void hold_rows(TiledRows<kHeadDim, kRF>& rows) {
 #pragma unroll
   for (int rf = 0; rf < kRF; ++rf) {
 #pragma unroll
-    for (int ks = 0; ks < FlashShape<kHeadDim>::kSteps; ++ks) asm volatile("" : "+v"(rows.q[rf][ks]));
+    for (int ks = 0; ks < TiledShape<kHeadDim>::kSteps; ++ks) asm volatile("" : "+v"(rows.q[rf][ks]));
   }
 }
 
@@ -417,11 +417,11 @@ __device__ __forceinline__ void hold_rows(FlashRows<kHeadDim, kRF>& rows) {
 //   all_seen      keys that every row of the wave sees
 template <int kHeadDim, int kRF, int kKF>
 struct TileWork {
-  using Shape = FlashShape<kHeadDim>;
+  using Shape = TiledShape<kHeadDim>;
   mfma_acc4 s[kRF][kKF];
   uint32_t packed[kRF][kKF][2];
 
-  __device__ __forceinline__ void scores(const FlashRows<kHeadDim, kRF>& rows, const elem_t* keys) {
+  __device__ __forceinline__ void scores(const TiledRows<kHeadDim, kRF>& rows, const elem_t* keys) {
     const int col = lane_id() & 15;
     const int grp = lane_id() >> 4;
 #pragma unroll
@@ -438,7 +438,7 @@ struct TileWork {
     }
   }
 
-  __device__ __forceinline__ void mask(const FlashRows<kHeadDim, kRF>& rows, int key0) {
+  __device__ __forceinline__ void mask(const TiledRows<kHeadDim, kRF>& rows, int key0) {
     const int grp = lane_id() >> 4;
 #pragma unroll
     for (int rf = 0; rf < kRF; ++rf) {
@@ -454,7 +454,7 @@ struct TileWork {
   }
 
   // The running statistics: a larger base where a score needs one.
-  __device__ __forceinline__ void raise_base(FlashRows<kHeadDim, kRF>& rows, float c) {
+  __device__ __forceinline__ void raise_base(TiledRows<kHeadDim, kRF>& rows, float c) {
     float top[kRF];
     bool raise = false;
 #pragma unroll
@@ -486,7 +486,7 @@ struct TileWork {
   }
 
   // The weights of the scores of 32 keys, rounded to the element type.
-  __device__ __forceinline__ void weights(const FlashRows<kHeadDim, kRF>& rows, float c, int half) {
+  __device__ __forceinline__ void weights(const TiledRows<kHeadDim, kRF>& rows, float c, int half) {
 #pragma unroll
     for (int rf = 0; rf < kRF; ++rf) {
       // before the first visible key every score is -inf: against base 0
@@ -510,7 +510,7 @@ struct TileWork {
   // The weights' sum is a product with ones: of what the values are weighted
   // with, rounded as they are, and off the vector units, which the exponentials
   // keep busy.
-  __device__ __forceinline__ void products(FlashRows<kHeadDim, kRF>& rows, const elem_t* values, int half) {
+  __device__ __forceinline__ void products(TiledRows<kHeadDim, kRF>& rows, const elem_t* values, int half) {
     constexpr uint32_t kOnes = kOneBits << 16 | kOneBits;
     const mfma_in8 ones = as_operand(vec16{{kOnes, kOnes, kOnes, kOnes}});
 #pragma unroll
@@ -525,7 +525,7 @@ struct TileWork {
 
   // Which rows see an infinity or NaN of the tile (with a weight above 0), by a
   // product with 1 in its place; a NaN counts as both infinities.
-  __device__ __forceinline__ void mark_special(FlashRows<kHeadDim, kRF>& rows, const elem_t* values) {
+  __device__ __forceinline__ void mark_special(TiledRows<kHeadDim, kRF>& rows, const elem_t* values) {
 #pragma unroll
     for (int half = 0; half < kKF / 2; ++half) {
 #pragma unroll 1
@@ -611,7 +611,7 @@ __device__ __forceinline__ int run_start(int key, int last) {
 }
 
 template <bool kWholePages, int kRun>
-__device__ __forceinline__ RunPage find_run(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
+__device__ __forceinline__ RunPage find_run(const BatchAttnArgs& a, const TiledPlan& plan, const Piece& p, int last,
                                             int key) {
   if constexpr (kWholePages) {
     typedef const __attribute__((address_space(4))) int32_t* constant_ptr;
@@ -635,9 +635,9 @@ __device__ __forceinline__ int pool_page(const BatchAttnArgs& a, int page, int& 
 // r of LDS starts r rows behind the tile, in memory as in LDS, so the loads of a
 // run differ by one offset that counts in both.
 template <int kHeadDim, bool kWholePages, int kRun, bool kKeys, bool kStream>
-__device__ __forceinline__ void load_run(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int last,
+__device__ __forceinline__ void load_run(const BatchAttnArgs& a, const TiledPlan& plan, const Piece& p, int last,
                                          const RunPage& run, int& bad, elem_t* tile, int key, int row0) {
-  using Shape = FlashShape<kHeadDim>;
+  using Shape = TiledShape<kHeadDim>;
   constexpr int kLoads = kRun / Shape::kLoadRows;
   constexpr int kLoadBytes = Shape::kLoadRows * kHeadDim * 2;
   static_assert(kLoadBytes == 1024 && kLoads <= 4, "offsets of 12 bits");
@@ -682,22 +682,22 @@ __device__ __forceinline__ void load_run(const BatchAttnArgs& a, const FlashPlan
 
 // One element's place in the output, from a packed row.
 template <int kHeadDim>
-__device__ __forceinline__ size_t out_at(const BatchAttnArgs& a, const FlashPlan& plan, const Piece& p, int r) {
+__device__ __forceinline__ size_t out_at(const BatchAttnArgs& a, const TiledPlan& plan, const Piece& p, int r) {
   const int token = packed_token(plan, r);
   return (static_cast<size_t>(p.row0 + token) * a.num_heads + p.kv * a.group + (r - token * a.group)) *
          kHeadDim;
 }
 
 template <int kHeadDim>
-__device__ __forceinline__ float* partial_stats(const FlashPlan& plan, int kv_heads, int tile_rows) {
+__device__ __forceinline__ float* partial_stats(const TiledPlan& plan, int kv_heads, int tile_rows) {
   return plan.partials + static_cast<size_t>(2 * plan.shares) * kv_heads * tile_rows * kHeadDim;
 }
 
 // At most 32 rows: the waves split the keys.
 template <int kHeadDim, bool kWholePages, int kRF, int kTileRows>
-__device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAttnArgs& a, const FlashPlan& plan,
+__device__ __forceinline__ void few_rows(TiledLds<kHeadDim>& lds, const BatchAttnArgs& a, const TiledPlan& plan,
                                          const Piece& p) {
-  using Shape = FlashShape<kHeadDim>;
+  using Shape = TiledShape<kHeadDim>;
   constexpr int kLoads = 32 / Shape::kLoadRows;
   constexpr int kSlots = Shape::kSlots;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -730,7 +730,7 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
   using Keys = std::integral_constant<bool, true>;
   using Values = std::integral_constant<bool, false>;
 
-  FlashRows<kHeadDim, kRF> rows;
+  TiledRows<kHeadDim, kRF> rows;
   rows.clear();
   if (count > 0) {
     load_rows<kHeadDim, kRF>(rows, a, plan, p, 0);
@@ -848,9 +848,9 @@ __device__ __forceinline__ void few_rows(FlashLds<kHeadDim>& lds, const BatchAtt
 // Many rows: the waves split them, 32 each, and share the tiles. `tiles_done`:
 // of the block's pieces before, so that a tile's number is its own.
 template <int kHeadDim, bool kWholePages>
-__device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAttnArgs& a, const FlashPlan& plan,
+__device__ __forceinline__ void many_rows(TiledLds<kHeadDim>& lds, const BatchAttnArgs& a, const TiledPlan& plan,
                                           const Piece& p, int& tiles_done) {
-  using Shape = FlashShape<kHeadDim>;
+  using Shape = TiledShape<kHeadDim>;
   constexpr int kRF = 2;
   constexpr int kRun = 64 / Shape::kWaves;          // a wave's keys of a tile
   constexpr int kLoads = kRun / Shape::kLoadRows;
@@ -875,7 +875,7 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
 
   const int row0 = 32 * wave;
   const bool active = row0 < p.rows;
-  FlashRows<kHeadDim, kRF> rows;
+  TiledRows<kHeadDim, kRF> rows;
   rows.clear();
   int all_seen = 0, any_seen = 0;
   if (active) {
@@ -999,19 +999,19 @@ __device__ __forceinline__ void many_rows(FlashLds<kHeadDim>& lds, const BatchAt
 
 // kMaxRows: packed rows a sequence may have, 16, 32 or any number (0).
 template <int kHeadDim, int kMaxRows, bool kWholePages>
-__global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim>::kSimdWaves) void batch_attention_kernel(
-    BatchAttnArgs args, FlashPlan flash_plan) {
-  using Shape = FlashShape<kHeadDim>;
+__global__ __launch_bounds__(TiledShape<kHeadDim>::kThreads, TiledShape<kHeadDim>::kSimdWaves) void batch_attention_kernel(
+    BatchAttnArgs args, TiledPlan tiled_plan) {
+  using Shape = TiledShape<kHeadDim>;
   constexpr bool kMany = kMaxRows == 0;
   constexpr int kTileRows = kMany ? Shape::kTileRows : kFewRows;
-  __shared__ __attribute__((aligned(1024))) FlashLds<kHeadDim> lds;
+  __shared__ __attribute__((aligned(1024))) TiledLds<kHeadDim> lds;
   BatchAttnArgs a = args;
   a.view.page_size = own_register(a.view.page_size);
   a.view.page_stride = own_register(a.view.page_stride);
   a.pool_pages = own_register(a.pool_pages);
   a.held = own_register(a.held);
   a.group = own_register(a.group);
-  FlashPlan plan = flash_plan;
+  TiledPlan plan = tiled_plan;
   plan.by_page.magic = own_register(plan.by_page.magic);
   plan.by_page.shift = own_register(plan.by_page.shift);
   plan.group_magic = own_register(plan.group_magic);
@@ -1118,7 +1118,7 @@ __global__ __launch_bounds__(FlashShape<kHeadDim>::kThreads, FlashShape<kHeadDim
 constexpr int kJoinThreads = 256;
 
 template <int kHeadDim, bool kRowEach>
-__global__ __launch_bounds__(kJoinThreads) void batch_attention_join_kernel(BatchAttnArgs a, FlashPlan plan,
+__global__ __launch_bounds__(kJoinThreads) void batch_attention_join_kernel(BatchAttnArgs a, TiledPlan plan,
                                                                            int tile_rows) {
   constexpr int kRowLanes = kHeadDim / 4;
   constexpr int kGroups = 64 / kRowLanes;
@@ -1281,24 +1281,24 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
 
 // A kv head's shares: all heads' together are the blocks resident at once.
 template <int kHeadDim>
-int flash_shares(int kv_heads, bool many) {
-  const int blocks = many ? FlashShape<kHeadDim>::kBlocks : FlashShape<kHeadDim>::kFewBlocks;
+int tiled_shares(int kv_heads, bool many) {
+  const int blocks = many ? TiledShape<kHeadDim>::kBlocks : TiledShape<kHeadDim>::kFewBlocks;
   return std::max(1, device_compute_units() * blocks / kv_heads);
 }
 
 bool many_rows_possible(int max_new, int group) { return static_cast<long long>(max_new) * group > kFewRows; }
 
 template <int kHeadDim>
-size_t flash_workspace(int max_new, int kv_heads, int group) {
+size_t tiled_workspace(int max_new, int kv_heads, int group) {
   const bool many = many_rows_possible(max_new, group);
-  const size_t rows = many ? FlashShape<kHeadDim>::kTileRows : kFewRows;
-  const size_t shares = static_cast<size_t>(flash_shares<kHeadDim>(kv_heads, many)) * static_cast<size_t>(kv_heads);
+  const size_t rows = many ? TiledShape<kHeadDim>::kTileRows : kFewRows;
+  const size_t shares = static_cast<size_t>(tiled_shares<kHeadDim>(kv_heads, many)) * static_cast<size_t>(kv_heads);
   return shares * (sizeof(CutUnit) + 2 * rows * (kHeadDim + 2) * sizeof(float));
 }
 
 template <int kHeadDim, int kMaxRows, bool kWholePages>
-void launch_flash_kernels(const BatchAttnArgs& a, const FlashPlan& plan, hipStream_t s) {
-  using Shape = FlashShape<kHeadDim>;
+void launch_tiled_kernels(const BatchAttnArgs& a, const TiledPlan& plan, hipStream_t s) {
+  using Shape = TiledShape<kHeadDim>;
   constexpr int kTileRows = kMaxRows == 0 ? Shape::kTileRows : kFewRows;
   const unsigned blocks = static_cast<unsigned>(plan.shares) * static_cast<unsigned>(a.view.num_kv_heads);
   batch_attention_kernel<kHeadDim, kMaxRows, kWholePages><<<blocks, Shape::kThreads, 0, s>>>(a, plan);
@@ -1311,22 +1311,22 @@ void launch_flash_kernels(const BatchAttnArgs& a, const FlashPlan& plan, hipStre
 }
 
 template <int kHeadDim>
-int flash_tile_tokens(int group) {
-  return std::max(1, FlashShape<kHeadDim>::kTileRows / group);
+int tiled_tile_tokens(int group) {
+  return std::max(1, TiledShape<kHeadDim>::kTileRows / group);
 }
 
 // A unit a block: at most one short tile a sequence beside the full ones.
 template <int kHeadDim>
-long long most_flash_units(const BatchAttnArgs& a) {
-  return a.tokens / flash_tile_tokens<kHeadDim>(a.group) + static_cast<long long>(a.batch);
+long long most_tiled_units(const BatchAttnArgs& a) {
+  return a.tokens / tiled_tile_tokens<kHeadDim>(a.group) + static_cast<long long>(a.batch);
 }
 
 template <int kHeadDim>
-void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  FlashPlan plan{};
+void launch_tiled(const BatchAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  TiledPlan plan{};
   const int kv_heads = a.view.num_kv_heads;
   plan.group_magic = static_cast<uint32_t>((65536 + a.group - 1) / a.group);
-  plan.tile_tokens = flash_tile_tokens<kHeadDim>(a.group);
+  plan.tile_tokens = tiled_tile_tokens<kHeadDim>(a.group);
   plan.by_page = FastDivide::by(static_cast<uint32_t>(a.view.page_size));
   plan.by_tile = FastDivide::by(static_cast<uint32_t>(plan.tile_tokens));
   plan.scale_log2e = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
@@ -1340,35 +1340,35 @@ void launch_flash(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   // 39.3 and 43.9; heads of 64, 8 on 8, one of 900 (64) 19.7 and 22.9, but 8 on 2,
   // two of 800 (78) 24.2 and 21.3, and 32 on 8, one of 500 (128) 20.1 and 16.1.
   const bool many = many_rows_possible(a.max_new, a.group);
-  const bool half_idle = many && 2 * most_flash_units<kHeadDim>(a) * kv_heads <= device_compute_units();
+  const bool half_idle = many && 2 * most_tiled_units<kHeadDim>(a) * kv_heads <= device_compute_units();
   const int cut_positions = half_idle ? 768 : 1024;
   // Steps are counted in 32 bits. Where a call's could pass them, it has units
   // enough to fill the device uncut.
-  const long long most_units = many ? most_flash_units<kHeadDim>(a) : a.batch;
+  const long long most_units = many ? most_tiled_units<kHeadDim>(a) : a.batch;
   const long long most_steps = kUnitSteps + 1 + std::max(a.held, std::min(a.max_new, a.tokens)) / kStepKeys;
   if (a.held > cut_positions && most_units * most_steps <= INT32_MAX / 2 && workspace != nullptr &&
-      workspace_bytes >= flash_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
+      workspace_bytes >= tiled_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
     plan.split = 1;
-    plan.shares = flash_shares<kHeadDim>(kv_heads, many);
+    plan.shares = tiled_shares<kHeadDim>(kv_heads, many);
     plan.cuts = static_cast<CutUnit*>(workspace);
     plan.partials = reinterpret_cast<float*>(plan.cuts + static_cast<size_t>(plan.shares) * kv_heads);
   } else {
-    plan.shares = static_cast<int>(most_flash_units<kHeadDim>(a));
+    plan.shares = static_cast<int>(most_tiled_units<kHeadDim>(a));
   }
   plan.by_shares = FastDivide::by(static_cast<uint32_t>(plan.shares));
   const long long most = static_cast<long long>(a.max_new) * a.group;
   if (a.view.page_size % 16 == 0) {
     if (most <= 16) {
-      launch_flash_kernels<kHeadDim, 16, true>(a, plan, s);
+      launch_tiled_kernels<kHeadDim, 16, true>(a, plan, s);
     } else if (most <= kFewRows) {
-      launch_flash_kernels<kHeadDim, 32, true>(a, plan, s);
+      launch_tiled_kernels<kHeadDim, 32, true>(a, plan, s);
     } else {
-      launch_flash_kernels<kHeadDim, 0, true>(a, plan, s);
+      launch_tiled_kernels<kHeadDim, 0, true>(a, plan, s);
     }
   } else if (most <= kFewRows) {
-    launch_flash_kernels<kHeadDim, 32, false>(a, plan, s);
+    launch_tiled_kernels<kHeadDim, 32, false>(a, plan, s);
   } else {
-    launch_flash_kernels<kHeadDim, 0, false>(a, plan, s);
+    launch_tiled_kernels<kHeadDim, 0, false>(a, plan, s);
   }
 }
 
@@ -1376,9 +1376,9 @@ bool on_bytes(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p
 
 // The matrix-core kernels take a positive scale (the running maximum is the
 // scores') and a group that fits a tile.
-bool flash_takes(const BatchAttnArgs& a) {
+bool tiled_takes(const BatchAttnArgs& a) {
   return (a.view.head_dim == 64 || a.view.head_dim == 128) &&
-         a.group <= (a.view.head_dim == 64 ? FlashShape<64>::kTileRows : FlashShape<128>::kTileRows) &&
+         a.group <= (a.view.head_dim == 64 ? TiledShape<64>::kTileRows : TiledShape<128>::kTileRows) &&
          a.scale > 0.0f && a.scale < 1e30f && a.q_row_stride % 8 == 0 && a.view.page_stride % 8 == 0 &&
          a.view.head_stride % 8 == 0 && on_bytes(a.q, 16) && on_bytes(a.out, 8) && on_bytes(a.view.keys, 16) &&
          on_bytes(a.view.values, 16);
@@ -1393,8 +1393,8 @@ extern "C" size_t lcr_batch_attention_workspace_bytes(int batch, int tokens, int
                                                       int heads_per_kv, int head_dim) {
   if (batch <= 0 || tokens <= 0 || max_new <= 0 || num_heads <= 0 || heads_per_kv <= 0) return 0;
   const int kv_heads = std::max(1, num_heads / heads_per_kv);
-  if (head_dim == 64) return flash_workspace<64>(max_new, kv_heads, heads_per_kv);
-  if (head_dim == 128) return flash_workspace<128>(max_new, kv_heads, heads_per_kv);
+  if (head_dim == 64) return tiled_workspace<64>(max_new, kv_heads, heads_per_kv);
+  if (head_dim == 128) return tiled_workspace<128>(max_new, kv_heads, heads_per_kv);
   return 0;
 }
 
@@ -1434,19 +1434,19 @@ extern "C" int lcr_batch_attention(void* out, const void* q, const lcr_kv_view* 
                   lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride,
                   table_stride * view->page_size, scale};
   auto s = static_cast<hipStream_t>(stream);
-  const bool flash = flash_takes(a);
+  const bool tiled = tiled_takes(a);
   // A launch has fewer than 2^32 threads in all.
   const long long units = static_cast<long long>(tokens) * num_heads;
-  const long long blocks = !flash ? (units + kGenericWaves - 1) / kGenericWaves
-                           : view->num_kv_heads * (view->head_dim == 64 ? most_flash_units<64>(a) : most_flash_units<128>(a));
-  const int threads = !flash ? kGenericThreads : view->head_dim == 64 ? FlashShape<64>::kThreads : FlashShape<128>::kThreads;
+  const long long blocks = !tiled ? (units + kGenericWaves - 1) / kGenericWaves
+                           : view->num_kv_heads * (view->head_dim == 64 ? most_tiled_units<64>(a) : most_tiled_units<128>(a));
+  const int threads = !tiled ? kGenericThreads : view->head_dim == 64 ? TiledShape<64>::kThreads : TiledShape<128>::kThreads;
   CAPI_CHECK(blocks * threads <= UINT32_MAX, "batch attention of " << tokens << " rows of " << num_heads
                                                                    << " heads needs more than 2^32 threads");
-  if (flash) {
+  if (tiled) {
     if (view->head_dim == 64) {
-      launch_flash<64>(a, workspace, workspace_bytes, s);
+      launch_tiled<64>(a, workspace, workspace_bytes, s);
     } else {
-      launch_flash<128>(a, workspace, workspace_bytes, s);
+      launch_tiled<128>(a, workspace, workspace_bytes, s);
     }
     CAPI_LAUNCHED();
     return LCR_OK;

@@ -258,3 +258,26 @@ def test_scales(lcr, gpu, scale):
         c = Case("bf16", [1300, 5], [2, 7], heads=4, kv=2, d=d, seed=38)
         c.scale = scale
         c.check(lcr)
+
+
+@pytest.mark.parametrize("positions", [None, 1100])
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinities_in_many_tiles_of_a_unit(lcr, gpu, d, positions):
+    """Values that only a unit's later rows see, in neighbouring tiles and in
+    every second one: each reaches its element of the rows from its position
+    on, and nothing else changes."""
+    for past, new in (([0], [600]), ([330, 0], [290, 410])):
+        c = Case("bf16", past, new, heads=1, kv=1, d=d, seed=39)
+        if positions:
+            wide(c, positions)
+        clean = c.run(lcr)
+        expected = to_f32(clean, c.kind).copy()
+        r = rng(40)
+        for b, (first, n) in enumerate(zip(c.starts, new)):
+            at = sorted(r.choice(n - 2, 9, replace=False).tolist()) + [n - 2]
+            for dim, (i, value) in enumerate(zip(at, [np.inf, -np.inf, np.nan] * 4)):
+                c.values[c.position_index(b, 0, past[b] + i) + dim] = elems(np.array([value], np.float32), c.kind)[0]
+                expected[first + i:first + n, 0, dim] = value
+        got = to_f32(c.run(lcr), c.kind)
+        assert (np.isnan(got) == np.isnan(expected)).all()
+        assert ((got == expected) | np.isnan(expected)).all()
