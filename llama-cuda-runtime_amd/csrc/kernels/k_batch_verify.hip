@@ -456,7 +456,10 @@ __device__ __forceinline__ int draw_index(DrawLds& lds, const VerifyArgs& a, flo
   }
   __syncthreads();
   const int part = lds.part;
-  if (part < 0) return -1;
+  if (part < 0) {
+    __syncthreads();  // every wave has read it: `lds` may be drawn with again
+    return -1;
+  }
   // Four neighbouring weights a thread.
   static_assert(kPart == 4 * kVerifyThreads, "one 16-byte load a thread");
   const int i0 = part * kPart + 4 * static_cast<int>(threadIdx.x);
