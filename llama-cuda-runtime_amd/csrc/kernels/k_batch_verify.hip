@@ -335,17 +335,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     const double m = max;
     const double lowest = lowest_of(max, scale);
     const Exp2 exp2(lds_table);
-    if (lowest >= -static_cast<double>(FLT_MAX)) {
-      // Beside the 1 of the largest, 2^-1020 for a logit below the lowest is
-      // nothing: one operation, where a choice of 0 takes three.
-      const float low = float_above(lowest);
+    const float low = float_above(lowest);
+    if (lowest >= -static_cast<double>(FLT_MAX) && low < max) {
+      // Clamped to the next float above the lowest, a logit weighs nothing beside
+      // the 1 of the largest: it is below that by at least the spacing of floats
+      // above `low`, and short of `span` by less than the spacing below it (twice
+      // the other at most), so below by more than span / 3: 2^-340 at most. One
+      // operation, where a choice of 0 takes three.
 #pragma unroll
       for (int j = 0; j < kPerLane; ++j) {
         sum += exp2.inside(__builtin_amdgcn_fmed3f(l[j], low, max), m, scale);  // NaN is the lowest
       }
     } else {
-      // A temperature so high that every finite logit weighs something, and
-      // -inf nothing.
+      // A temperature so high that every finite logit weighs something, and -inf
+      // nothing; or so low that no float lies between the lowest and the largest.
 #pragma unroll
       for (int j = 0; j < kPerLane; ++j) sum += exp2(l[j], max, scale);
     }
