@@ -62,6 +62,10 @@ extern "C" {
  * or a negative entry in lengths, new_tokens or mapped. That sequence and all
  * behind it get no rows and no pages, for the caller to try again.
  *
+ * A batch of 0 is a step without rows: row_starts[0], positions, slots and counts
+ * are written as for any other, the sequences' arrays are not looked at and may
+ * be NULL. (Nothing is done where one of those outputs or free_count is NULL.)
+ *
  * Out: row_starts[batch + 1]; positions[max_rows] and slots[max_rows], with
  * slot = page * page_size + position % page_size, both -1 behind the last row
  * (slots also where the page is outside 0 .. pool_pages - 1); lengths_out and

@@ -86,6 +86,7 @@ __global__ __launch_bounds__(kMapThreads) void batch_map_kernel(MapArgs a) {
   const int first = t * per;
   const int free = min(max(a.free_count[0], 0), a.free_capacity);
   const long long capacity = static_cast<long long>(a.table_stride) * a.page_size;
+  if (t == 0 && a.batch == 0) row_start[0] = page_start[0] = 0;  // read behind the barriers
 
   // Sums over this thread's sequences. They are kept in 64 bits: before the
   // first sequence that fails they fit 32, behind it they only have to stay
@@ -184,6 +185,36 @@ __global__ __launch_bounds__(kMapThreads) void batch_map_kernel(MapArgs a) {
   }
 }
 
+int launch_map(const MapArgs& a, void* stream) {
+  // One row or sequence a thread up to 512 blocks.
+  const int items = std::max(a.max_rows, a.batch + 1);
+  const int blocks = std::min(512, (items - 1) / kMapThreads + 1);
+  batch_map_kernel<<<blocks, kMapThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+  CAPI_LAUNCHED();
+  return LCR_OK;
+}
+
+// Whether this process's HIP runtime knows the address.
+bool known_address(const void* p) {
+  hipPointerAttribute_t attributes{};
+  const bool known = hipPointerGetAttributes(&attributes, p) == hipSuccess &&
+                     attributes.type != hipMemoryTypeUnregistered;
+  (void)hipGetLastError();  // an address that is not known leaves an error
+  return known;
+}
+
+// A step of no sequences is a step: no rows, and the free count handed on. Its
+// sequences' arrays are not read and may be NULL. Where only some of them are,
+// the call may have been made of stand-ins for arrays, which are not followed.
+int map_nothing(MapArgs a, void* stream) {
+  const bool rows = a.max_rows == 0 || (a.positions != nullptr && a.slots != nullptr);
+  if (a.row_starts == nullptr || a.counts == nullptr || a.free_count == nullptr || !rows) return LCR_OK;
+  const int given = (a.lengths != nullptr) + (a.new_tokens != nullptr) + (a.mapped != nullptr);
+  if (given != 0 && given != 3 && !known_address(a.counts)) return LCR_OK;
+  a.free_capacity = std::max(a.free_capacity, 0);
+  return launch_map(a, stream);
+}
+
 }  // namespace
 }  // namespace lcr
 
@@ -197,7 +228,9 @@ extern "C" int lcr_batch_map(int32_t* row_starts, int32_t* positions, int32_t* s
   CAPI_CHECK(batch >= 0 && max_rows >= 0, "batch_map needs non-negative sizes");
   CAPI_CHECK(batch <= LCR_BATCH_MAX_SEQUENCES,
              "batch_map takes up to " << LCR_BATCH_MAX_SEQUENCES << " sequences, got " << batch);
-  if (batch == 0) return LCR_OK;
+  MapArgs a{row_starts, positions, slots,     lengths_out, mapped_out, counts,   page_tables, lengths,    new_tokens,
+            mapped,     free_pages, free_count, batch,      max_rows,   table_stride, page_size, pool_pages, free_capacity};
+  if (batch == 0) return map_nothing(a, stream);
   CAPI_CHECK(page_size > 0, "batch_map needs a positive page size, got " << page_size);
   CAPI_CHECK(table_stride > 0, "batch_map needs page tables of at least one page, got " << table_stride);
   CAPI_CHECK(pool_pages >= 0 && free_capacity >= 0, "batch_map needs non-negative page counts");
@@ -215,12 +248,5 @@ extern "C" int lcr_batch_map(int32_t* row_starts, int32_t* positions, int32_t* s
   CAPI_CHECK(lengths_out != lengths && lengths_out != new_tokens && mapped_out != mapped && counts != free_count &&
                  counts + 1 != free_count,
              "batch_map writes its outputs beside its inputs, not over them");
-  MapArgs a{row_starts, positions, slots,     lengths_out, mapped_out, counts,   page_tables, lengths,    new_tokens,
-            mapped,     free_pages, free_count, batch,      max_rows,   table_stride, page_size, pool_pages, free_capacity};
-  // One row or sequence a thread up to 512 blocks.
-  const int items = std::max(max_rows, batch + 1);
-  const int blocks = std::min(512, (items - 1) / kMapThreads + 1);
-  batch_map_kernel<<<blocks, kMapThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
-  CAPI_LAUNCHED();
-  return LCR_OK;
+  return launch_map(a, stream);
 }
