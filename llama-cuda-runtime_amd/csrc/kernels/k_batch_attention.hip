@@ -653,7 +653,7 @@ __device__ __forceinline__ void load_run(const BatchAttnArgs& a, const TiledPlan
     const int first = run_start<kRun>(key, last);
     const int page = pool_page(a, run.page, bad);
     const elem_t* from = pool + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                         static_cast<size_t>(run.slot * kHeadDim);
+                         static_cast<size_t>(static_cast<uint32_t>(run.slot)) * kHeadDim;
     if (last - first >= kRun - 1) {
       const uint32_t row_at = static_cast<uint32_t>(load_row * kHeadDim * 2);
       load_to_lds16<0, kStream>(from, row_at + chunk(0), to);
