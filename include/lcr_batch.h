@@ -31,7 +31,9 @@
  *
  * What the device finds wrong in its arrays (a page outside the pool, a token
  * outside the vocabulary) cannot fail the call; each entry says what then
- * comes out. No such value makes a kernel read or write out of bounds.
+ * comes out. No such value makes a kernel read or write out of bounds. Of row
+ * starts that do not ascend, as lcr_batch_map's do, nothing is said but that:
+ * the outputs may hold anything, or what they held.
  */
 #ifndef LCR_BATCH_H_
 #define LCR_BATCH_H_

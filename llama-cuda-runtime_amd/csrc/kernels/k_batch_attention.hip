@@ -214,41 +214,51 @@ struct ShareStart {
   Sequence seq;
 };
 
+// Steps that a kv head may count for: what the host allows of a call whose
+// sequences have rows of their own. Row starts that overlap can count for more,
+// past what the steps' arithmetic holds; such a call has no work.
+constexpr int kMostSteps = INT32_MAX / 2;
+
+// Sums of steps, which stay at the largest number instead of wrapping.
+__device__ __forceinline__ uint32_t add_steps(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
 // Where a kv head's share `index` begins: the prefix sums of the sequences'
 // steps, taken by the whole block.
 template <int kHeadDim, bool kMany, int kThreads>
 __device__ __forceinline__ ShareStart find_share(const BatchAttnArgs& a, const TiledPlan& plan, int index,
-                                                 int* lds_sums, ShareStart* lds_found) {
+                                                 uint32_t* lds_sums, ShareStart* lds_found) {
   constexpr int kWaves = kThreads / 64;
   const int t = threadIdx.x;
   const int per = (a.batch + kThreads - 1) / kThreads;
-  int mine = 0;
+  uint32_t mine = 0;
   Sequence seq{};
   for (int k = 0; k < per; ++k) {
     const int b = t * per + k;
     if (b < a.batch) {
       seq = load_sequence<kHeadDim, kMany>(a, plan, b);
-      mine += seq.steps;
+      mine = add_steps(mine, static_cast<uint32_t>(seq.steps));
     }
   }
-  int to = mine;
+  uint32_t to = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int other = __shfl_up(to, o, 64);
-    if (lane_id() >= o) to += other;
+    const uint32_t other = __shfl_up(to, o, 64);
+    if (lane_id() >= o) to = add_steps(to, other);
   }
   if (lane_id() == 63) lds_sums[t >> 6] = to;
   if (t == 0) lds_found->sequence = -1;
   __syncthreads();
-  int total = 0, before = to - mine;
+  uint32_t all = 0, ahead = to - mine;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w < (t >> 6)) before += lds_sums[w];
-    total += lds_sums[w];
+    if (w < (t >> 6)) ahead = add_steps(ahead, lds_sums[w]);
+    all = add_steps(all, lds_sums[w]);
   }
+  const int total = all <= kMostSteps ? static_cast<int>(all) : 0;
+  int before = static_cast<int>(ahead);
   const int share = plan.split ? max(plan.by_shares(total + plan.shares - 1), plan.min_share) : 1;
   const int at = index * share;
-  if (at >= before && at < before + mine) {
+  if (total > 0 && at >= before && at < before + static_cast<int>(mine)) {
     for (int k = 0; k < per; ++k) {
       const int b = t * per + k;
       if (b >= a.batch) break;
@@ -325,7 +335,7 @@ template <int kHeadDim>
 struct TiledLds {
   elem_t ring[TiledShape<kHeadDim>::kRingElems];
   float stats[TiledShape<kHeadDim>::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
-  int sums[TiledShape<kHeadDim>::kWaves];
+  uint32_t sums[TiledShape<kHeadDim>::kWaves];
   ShareStart found;
   int bad;  // a page outside the pool was read
   int special[2];  // many rows: the last tile of even and of odd number whose values hold infinities or NaN
@@ -1350,7 +1360,7 @@ void launch_tiled(const BatchAttnArgs& a, void* workspace, size_t workspace_byte
   // enough to fill the device uncut.
   const long long most_units = many ? most_tiled_units<kHeadDim>(a) : a.batch;
   const long long most_steps = kUnitSteps + 1 + std::max(a.held, std::min(a.max_new, a.tokens)) / kStepKeys;
-  if (a.held > cut_positions && most_units * most_steps <= INT32_MAX / 2 && workspace != nullptr &&
+  if (a.held > cut_positions && most_units * most_steps <= kMostSteps && workspace != nullptr &&
       workspace_bytes >= tiled_workspace<kHeadDim>(a.max_new, kv_heads, a.group)) {
     plan.split = 1;
     plan.shares = tiled_shares<kHeadDim>(kv_heads, many);
