@@ -113,6 +113,9 @@ int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view, const voi
  * 64 and 128 with 16-byte aligned rows run on the matrix cores, and
  * fastest with a page_size that is a multiple of 16. Tables hold up to 2^30
  * positions.
+ * Infinities and NaN in places that a row does not see leave it as it is; of a
+ * value that it sees, its element becomes infinite or NaN, also where the weight
+ * rounds to 0.
  * A row that sees no position (lengths[b] < n) is zeros. Positions behind
  * table_stride pages do not exist. A sequence with a page outside 0 ..
  * pool_pages - 1 among those it reads may come out as NaN.

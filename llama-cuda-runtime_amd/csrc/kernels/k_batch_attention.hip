@@ -533,9 +533,24 @@ struct TileWork {
     }
   }
 
-  // Which rows see an infinity or NaN of the tile (with a weight above 0), by a
-  // product with 1 in its place; a NaN counts as both infinities.
-  __device__ __forceinline__ void mark_special(TiledRows<kHeadDim, kRF>& rows, const elem_t* values) {
+  // 1 for each of 32 keys that a lane's row sees, in the order of weight_operand.
+  __device__ __forceinline__ mfma_in8 seen_operand(const TiledRows<kHeadDim, kRF>& rows, int rf, int half, int key0) const {
+    int left = rows.seen[rf] - key0 - 32 * half - 4 * (lane_id() >> 4);
+    asm volatile("" : "+v"(left));  // made again each time: kept, they cost registers in every tile
+    vec16 seen;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 16 * (i >> 1) + 2 * (i & 1);
+      seen.w[i] = (key < left ? kOneBits : 0u) | (key + 1 < left ? kOneBits << 16 : 0u);
+    }
+    return as_operand(seen);
+  }
+
+  // Which rows see an infinity or NaN of the tile, by a product of ones in place
+  // of it and of what they see; a NaN counts as both infinities. (With the weights
+  // instead, one that rounds to 0 would lose it: in fp16, of any key 17 below the
+  // largest score.)
+  __device__ __forceinline__ void mark_special(TiledRows<kHeadDim, kRF>& rows, const elem_t* values, int key0) {
 #pragma unroll
     for (int half = 0; half < kKF / 2; ++half) {
 #pragma unroll 1
@@ -558,8 +573,8 @@ struct TileWork {
 #pragma unroll
         for (int rf = 0; rf < kRF; ++rf) {
           const mfma_acc4 zero{0.f, 0.f, 0.f, 0.f};
-          const mfma_acc4 a = mfma16x16x32(as_operand(up), weight_operand(rf, half), zero);
-          const mfma_acc4 b = mfma16x16x32(as_operand(down), weight_operand(rf, half), zero);
+          const mfma_acc4 a = mfma16x16x32(as_operand(up), seen_operand(rows, rf, half, key0), zero);
+          const mfma_acc4 b = mfma16x16x32(as_operand(down), seen_operand(rows, rf, half, key0), zero);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             rows.up[rf] |= (a[e] > 0.0f ? 1u : 0u) << (4 * df + e);
@@ -786,7 +801,7 @@ __device__ __forceinline__ void few_rows(TiledLds<kHeadDim>& lds, const BatchAtt
       loads_landed<0>();
     }
     if (!whole && any_special(value_tile(t), 32 * kHeadDim / 512)) {
-      work.mark_special(rows, value_tile(t));
+      work.mark_special(rows, value_tile(t), key0);
       clear_special(value_tile(t), 32 * kHeadDim / 512);
     }
     work.products(rows, value_tile(t), 0);
@@ -958,7 +973,7 @@ __device__ __forceinline__ void many_rows(TiledLds<kHeadDim>& lds, const BatchAt
         work.scores(rows, stage + half * 32 * kHeadDim);
         if (!whole) work.mask(rows, tile0 + 32 * half);
         work.weights(rows, plan.scale_log2e, 0);
-        work.mark_special(rows, at);
+        work.mark_special(rows, at, tile0 + 32 * half);
       }
       lds_settled();
       plain_barrier();
