@@ -20,7 +20,10 @@
  * The rows of a step are the sequences' new tokens one after another: sequence
  * b has rows row_starts[b] .. row_starts[b + 1] - 1. The buffers may hold more
  * rows behind the last sequence's; those have slot and position -1 and are
- * neither read nor written. A sequence may have no rows.
+ * neither read nor written (lcr_batch_verify may read their target_logits, to no
+ * effect). A sequence may have no rows. A call of some of a step's sequences takes
+ * its row starts from the first of them on; rows before that stay as they were,
+ * as those behind the last.
  *
  * Conventions (element pointers, streams, status, error text) are those of
  * lcr_kernels.h. Nothing here allocates or waits; arrays named on the device

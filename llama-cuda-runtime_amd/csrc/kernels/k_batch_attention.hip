@@ -1241,6 +1241,8 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
   if (lo == a.batch) return;  // behind the last sequence
   const int b = lo;
   const int in_sequence = row - a.row_starts[b];
+  // before the first sequence, or of one whose rows the buffer does not hold
+  if (in_sequence < 0 || a.row_starts[b + 1] > a.tokens) return;
   const int head_dim = a.view.head_dim;
   const int kv = head / a.group;
   const long long position = static_cast<long long>(a.lengths[b]) - (a.row_starts[b + 1] - row);
