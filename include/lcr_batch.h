@@ -108,7 +108,9 @@ int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view, const voi
  * Row i of sequence b's n rows is at position lengths[b] - n + i (lengths
  * counts the new tokens, whose keys and values are in the cache) and sees
  * positions 0 .. its own:  out = softmax(scale q . k) v, statistics and sums in
- * fp32, the probabilities rounded to the element type before the value product.
+ * fp32. On the matrix cores the weights exp(s - max) are rounded to the element
+ * type, for the value product and for their sum alike: by half a step each, and
+ * in fp16 by 2^-32 of the row's largest where that is more.
  *   q:   [tokens] rows q_row_stride elements apart, [num_heads][head_dim] each
  *   out: [tokens][num_heads][head_dim]
  * view->page_table: [batch][table_stride]. max_new: no sequence has more rows

@@ -18,14 +18,15 @@
 //
 // Arithmetic. S^T = K . Q^T on 16x16x32 matrix instructions: a lane holds one
 // packed row and four keys of each sixteen. One pass over the keys:
-//   p = exp2(c s + b), c = scale log2 e, b = -(c m) for a running maximum m
+//   p = exp2(c s + b), c = scale log2 e, b = e - c m for a running maximum m (e is
+//   0, and 7 in fp16)
 //   l += 1 . P^T;  O^T += V^T . P^T
-// A new m is taken when some p would pass 2^8, and l and O then move to the new
-// base by exp2(b_new - b); a row's l and O always share one base, so its
-// rounding cancels in O / l. p is rounded to the element type for the value
-// product (the matrix cores take no wider operand beside 16-bit values: half a
-// step of each weight, against two more products for a second half of p);
-// everything else is fp32.
+// A new m is taken when some p would pass 2^(e + 8), and l and O then move to the
+// new base by exp2(b_new - b); a row's l and O always share one base, so its
+// rounding cancels in O / l. p is rounded to the element type for the products
+// (the matrix cores take no wider operand beside 16-bit values: half a step of
+// each weight, against two more products for a second half of p); everything else
+// is fp32.
 //
 // Few rows (at most 32): bound by the cache's bytes. The waves of a block share
 // the rows and split the keys, 32 a step, each streaming its own keys and
@@ -341,10 +342,16 @@ struct TiledLds {
   int special[2];  // many rows: the last tile of even and of odd number whose values hold infinities or NaN
 };
 
+// kTop: the exponent of a row's largest weight when its base is taken. The base is
+// kept until a weight would pass 8 more. In fp16 weights are held as high as that
+// leaves them (2^15), as they round coarsely below 2^-14 and to 0 below 2^-25:
+// with kTop 0, 9000 keys of e^-18 of the largest each counted for nothing.
 #if defined(LCR_ELEM_FP16)
 constexpr uint32_t kInfBits = 0x7c00u, kOneBits = 0x3c00u;
+constexpr float kTop = 7.0f;
 #else
 constexpr uint32_t kInfBits = 0x7f80u, kOneBits = 0x3f80u;
+constexpr float kTop = 0.0f;
 #endif
 
 // A packed-row fragment's accumulators: rows 16 rf + col, per lane.
@@ -477,15 +484,15 @@ struct TileWork {
       }
       // c top + base: the largest weight's exponent (inf for a first visible
       // key, NaN, which compares false, while there is none)
-      raise |= __builtin_fmaf(top[rf], c, rows.base[rf]) > 8.0f;
+      raise |= __builtin_fmaf(top[rf], c, rows.base[rf]) > kTop + 8.0f;
     }
     if (!__any(raise)) return;
 #pragma unroll
     for (int rf = 0; rf < kRF; ++rf) {
       float most = fmaxf(top[rf], xor_lane<16>(top[rf]));
       most = fmaxf(most, xor_lane<32>(most));
-      if (__builtin_fmaf(most, c, rows.base[rf]) > 0.0f) {
-        const float base = -(most * c);
+      if (__builtin_fmaf(most, c, rows.base[rf]) > kTop) {
+        const float base = kTop - most * c;
         const float move = __builtin_amdgcn_exp2f(base - rows.base[rf]);
         rows.base[rf] = base;
         rows.sum[rf] *= move;
@@ -1284,7 +1291,7 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_generic_kerne
     const float p = lane < n ? lcr_expf(s - m_new) : 0.0f;
     m = m_new;
     l = l * keep + p;
-    weights[wave][lane] = elem_to_float(float_to_elem(p));
+    weights[wave][lane] = p;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
