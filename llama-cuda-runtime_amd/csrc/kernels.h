@@ -9,7 +9,6 @@
 
 #include <cstdint>
 
-#include "../../include/lcr_batch.h"
 #include "../../include/lcr_kernels.h"
 #include "dtype.h"
 #include "kv_cache.h"
@@ -153,58 +152,6 @@ inline void launch_prefill_attention(elem_t* out, const elem_t* q_heads, const K
   const lcr_kv_view v = view.to_c();
   check_kernel_status(lcr_prefill_attention(out, q_heads, &v, num_heads, heads_per_kv, tokens,
                                             start_position, scale, paged ? 1 : 0, stream));
-}
-
-// A step of several sequences over one paged cache (lcr_batch.h).
-inline void launch_batch_map(int32_t* row_starts, int32_t* positions, int32_t* slots, int32_t* lengths_out,
-                             int32_t* mapped_out, int32_t* counts, int32_t* page_tables, const int32_t* lengths,
-                             const int32_t* new_tokens, const int32_t* mapped, const int32_t* free_pages,
-                             const int32_t* free_count, int batch, int max_rows, int table_stride, int page_size,
-                             int pool_pages, int free_capacity, hipStream_t stream) {
-  check_kernel_status(lcr_batch_map(row_starts, positions, slots, lengths_out, mapped_out, counts, page_tables, lengths,
-                                    new_tokens, mapped, free_pages, free_count, batch, max_rows, table_stride,
-                                    page_size, pool_pages, free_capacity, stream));
-}
-
-inline void launch_batch_norm_rope_write_kv(elem_t* q_out, const KvCacheView& view, const elem_t* q, const elem_t* k,
-                                            const elem_t* v, const elem_t* q_norm, const elem_t* k_norm, float eps,
-                                            const float2* rope_table, int table_positions, const int32_t* positions,
-                                            const int32_t* slots, int tokens, int num_heads, int pool_pages,
-                                            int src_row_stride, hipStream_t stream) {
-  const lcr_kv_view c = view.to_c();
-  check_kernel_status(lcr_batch_norm_rope_write_kv(q_out, &c, q, k, v, q_norm, k_norm, eps,
-                                                   reinterpret_cast<const float*>(rope_table), table_positions,
-                                                   positions, slots, tokens, num_heads, pool_pages, src_row_stride,
-                                                   stream));
-}
-
-inline void launch_batch_attention(elem_t* out, const elem_t* q, const KvCacheView& view, const int32_t* row_starts,
-                                   const int32_t* lengths, int batch, int tokens, int max_new, int num_heads,
-                                   int heads_per_kv, int table_stride, int pool_pages, int q_row_stride, float scale,
-                                   void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  const lcr_kv_view c = view.to_c();
-  check_kernel_status(lcr_batch_attention(out, q, &c, row_starts, lengths, batch, tokens, max_new, num_heads,
-                                          heads_per_kv, table_stride, pool_pages, q_row_stride, scale, workspace,
-                                          workspace_bytes, stream));
-}
-
-inline size_t batch_attention_workspace_bytes(int batch, int tokens, int max_new, int num_heads, int heads_per_kv,
-                                              int head_dim) {
-  return lcr_batch_attention_workspace_bytes(batch, tokens, max_new, num_heads, heads_per_kv, head_dim);
-}
-
-inline void launch_batch_verify(int32_t* out_ids, int32_t* out_counts, const float* target_logits,
-                                const float* draft_logits, const int32_t* draft_ids, const int32_t* row_starts,
-                                const float* temperatures, const float* accept_uniforms, const float* sample_uniforms,
-                                int batch, int rows, int max_draft, int vocab, int logits_stride, void* workspace,
-                                size_t workspace_bytes, hipStream_t stream) {
-  check_kernel_status(lcr_batch_verify(out_ids, out_counts, target_logits, draft_logits, draft_ids, row_starts,
-                                       temperatures, accept_uniforms, sample_uniforms, batch, rows, max_draft, vocab,
-                                       logits_stride, workspace, workspace_bytes, stream));
-}
-
-inline size_t batch_verify_workspace_bytes(int batch, int rows, int vocab) {
-  return lcr_batch_verify_workspace_bytes(batch, rows, vocab);
 }
 
 }  // namespace lcr

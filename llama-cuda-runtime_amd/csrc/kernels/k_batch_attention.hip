@@ -320,14 +320,13 @@ struct TiledShape {
   static constexpr int kSimdWaves = kWaves * kBlocks / 4;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kTileRows = 32 * kWaves;               // packed rows of a tile of many rows
-  static constexpr int kSlots = 1;                            // few rows: steps in flight a wave
   static constexpr int kStages = kHeadDim == 64 ? 3 : 4;      // many rows: tiles staged
   static constexpr int kRowChunks = kHeadDim / 8;             // 16-byte chunks of a key
   static constexpr int kLoadRows = 64 / kRowChunks;           // keys of one 1 KiB direct load
   static constexpr int kSteps = kHeadDim / 32;                // k-steps of a score
   static constexpr int kDFrags = kHeadDim / 16;               // output fragments
-  // elements of LDS: a wave's slots (few) or a block's stages (many)
-  static constexpr int kWaveElems = kSlots * 2 * 32 * kHeadDim;
+  // elements of LDS: a wave's step (few) or a block's stages (many)
+  static constexpr int kWaveElems = 2 * 32 * kHeadDim;
   static constexpr int kRingElems = kStages * 2 * 64 * kHeadDim;
   static_assert(kRingElems >= kWaves * kWaveElems, "both use the same LDS");
 };
@@ -731,14 +730,13 @@ __device__ __forceinline__ void few_rows(TiledLds<kHeadDim>& lds, const BatchAtt
                                          const Piece& p) {
   using Shape = TiledShape<kHeadDim>;
   constexpr int kLoads = 32 / Shape::kLoadRows;
-  constexpr int kSlots = Shape::kSlots;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int lane = lane_id();
   const int col = lane & 15;
   const int grp = lane >> 4;
   elem_t* mine = lds.ring + wave * Shape::kWaveElems;
-  auto key_tile = [&](int t) { return mine + (t % kSlots) * (2 * 32 * kHeadDim); };
-  auto value_tile = [&](int t) { return key_tile(t) + 32 * kHeadDim; };
+  elem_t* const key_tile = mine;
+  elem_t* const value_tile = mine + 32 * kHeadDim;
   const int tiles = (p.key1 - p.key0 + 31) / 32;
   const int count = tiles > wave ? (tiles - wave - 1) / Shape::kWaves + 1 : 0;
   const int last = p.key1 - 1;
@@ -755,8 +753,8 @@ __device__ __forceinline__ void few_rows(TiledLds<kHeadDim>& lds, const BatchAtt
     constexpr bool kKeys = decltype(is_keys)::value;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      load_run<kHeadDim, kWholePages, 16, kKeys, true>(a, plan, p, last, pages.run[n], bad, kKeys ? key_tile(t) : value_tile(t),
-                                                 first_key(t) + 16 * n, 16 * n);
+      load_run<kHeadDim, kWholePages, 16, kKeys, true>(a, plan, p, last, pages.run[n], bad,
+                                                       kKeys ? key_tile : value_tile, first_key(t) + 16 * n, 16 * n);
     }
   };
   using Keys = std::integral_constant<bool, true>;
@@ -766,54 +764,38 @@ __device__ __forceinline__ void few_rows(TiledLds<kHeadDim>& lds, const BatchAtt
   rows.clear();
   if (count > 0) {
     load_rows<kHeadDim, kRF>(rows, a, plan, p, 0);
-    StepPages pages[kSlots];
-#pragma unroll
-    for (int t = 0; t < kSlots; ++t) pages[t] = pages_of(t);
-#pragma unroll
-    for (int t = 0; t < kSlots; ++t) {
-      if (t < count) {
-        issue(Keys{}, t, pages[t]);
-        issue(Values{}, t, pages[t]);
-      }
-    }
+    const StepPages pages = pages_of(0);
+    issue(Keys{}, 0, pages);
+    issue(Values{}, 0, pages);
   }
   hold_rows(rows);
   const int all_seen = min(p.seen_first, p.key1);
   for (int t = 0; t < count; ++t) {
-    const int left = count - 1 - t;
-    const bool more = left >= kSlots;
+    const bool more = t + 1 < count;
     StepPages pages{};
-    if (more) pages = pages_of(t + kSlots);
-    // In flight behind step t's keys: its values, and the later steps' both.
-    if (kSlots > 1 && left > 0) {
-      loads_landed<3 * kLoads>();
-    } else {
-      loads_landed<kLoads>();
-    }
+    if (more) pages = pages_of(t + 1);
+    loads_landed<kLoads>();  // step t's keys; behind them its values are in flight
     const int key0 = first_key(t);
     const bool whole = key0 + 32 <= all_seen;
     TileWork<kHeadDim, kRF, 2> work;
-    work.scores(rows, key_tile(t));
+    work.scores(rows, key_tile);
     lds_settled();  // the keys have been read
-    if (more) issue(Keys{}, t + kSlots, pages);
+    if (more) issue(Keys{}, t + 1, pages);
     if (!whole) work.mask(rows, key0);
     work.raise_base(rows, plan.scale_log2e);
     work.weights(rows, plan.scale_log2e, 0);
-    // Behind step t's values: the later steps' keys and values.
     if (more) {
-      loads_landed<(2 * (kSlots - 1) + 1) * kLoads>();
-    } else if (kSlots > 1 && left > 0) {
-      loads_landed<2 * kLoads>();
+      loads_landed<kLoads>();  // step t's values; behind them the next keys
     } else {
       loads_landed<0>();
     }
-    if (!whole && any_special(value_tile(t), 32 * kHeadDim / 512)) {
-      work.mark_special(rows, value_tile(t), key0);
-      clear_special(value_tile(t), 32 * kHeadDim / 512);
+    if (!whole && any_special(value_tile, 32 * kHeadDim / 512)) {
+      work.mark_special(rows, value_tile, key0);
+      clear_special(value_tile, 32 * kHeadDim / 512);
     }
-    work.products(rows, value_tile(t), 0);
+    work.products(rows, value_tile, 0);
     lds_settled();
-    if (more) issue(Values{}, t + kSlots, pages);
+    if (more) issue(Values{}, t + 1, pages);
   }
 
   rows.add_special();
