@@ -161,7 +161,8 @@ __global__ __launch_bounds__(kMapThreads) void batch_map_kernel(MapArgs a) {
     }
   }
   // New page j is free_pages[free - 1 - j].
-  for (int j = me; j < all_pages; j += step) {
+  for (long long i = me; i < all_pages; i += step) {
+    const int j = static_cast<int>(i);
     const int b = bisect(page_start, placed, j);
     const int column = a.mapped[b] + j - page_start[b];
     a.page_tables[static_cast<size_t>(b) * a.table_stride + column] = a.free_pages[free - 1 - j];
