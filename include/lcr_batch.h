@@ -143,8 +143,8 @@ size_t lcr_batch_attention_workspace_bytes(int batch, int tokens, int max_new, i
  * of n - 1 drafted tokens; draft_ids[row] is the token drafted behind that row,
  * draft_logits[row] what it was drawn from (NULL: drafted without a
  * distribution, so q below is 1 at the drafted token). Of a sequence's last
- * row neither is read. Rows are logits_stride floats apart. At most max_draft
- * drafts are taken.
+ * row neither is read. Rows are logits_stride floats apart, at most 65535. At most
+ * max_draft drafts are taken (itself at most 2^30).
  *   temperature T = temperatures[b] > 0: p = softmax(target / T), q =
  *     softmax(draft / T); the draft x of row i is kept iff
  *     accept_uniforms[row] * q(x) < p(x). Behind the first one not kept comes a

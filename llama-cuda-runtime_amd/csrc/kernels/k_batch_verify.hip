@@ -692,7 +692,8 @@ extern "C" int lcr_batch_verify(int32_t* out_ids, int32_t* out_counts, const flo
              "batch_verify takes up to " << LCR_BATCH_MAX_SEQUENCES << " sequences, got " << batch);
   if (batch == 0) return LCR_OK;
   CAPI_CHECK(vocab > 0, "cannot sample from an empty vocabulary");
-  CAPI_CHECK(max_draft < INT32_MAX, "batch_verify takes fewer than 2^31 - 1 drafts");
+  // counted in 32 bits, a block's threads at a time
+  CAPI_CHECK(max_draft <= (1 << 30), "batch_verify takes up to 2^30 drafts, got " << max_draft);
   CAPI_CHECK(logits_stride >= vocab, "rows of " << vocab << " logits cannot lie " << logits_stride << " apart");
   CAPI_CHECK(rows <= 65535, "batch_verify takes up to 65535 rows, got " << rows);
   CAPI_CHECK(out_ids != nullptr && out_counts != nullptr && row_starts != nullptr && temperatures != nullptr &&

@@ -5,6 +5,13 @@ import ctypes
 import numpy as np
 import pytest
 
+from test_batch_refusals import lib, refused, verify_call  # noqa: F401  (a fixture)
+
+
+def test_verify_refuses_drafts_past_2_to_30(lib):  # noqa: F811
+    refused(lib, verify_call(lib, max_draft=(1 << 30) + 1), "up to 2^30 drafts")
+    refused(lib, verify_call(lib, max_draft=2 ** 31 - 2), "up to 2^30 drafts, got 2147483646")
+
 
 @pytest.mark.gpu
 def test_map_of_nearly_2_to_31_pages(lcr, gpu):
