@@ -120,7 +120,8 @@ int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view, const voi
  * positions.
  * Infinities and NaN in places that a row does not see leave it as it is; of a
  * value that it sees, its element becomes infinite or NaN, also where the weight
- * rounds to 0.
+ * rounds to 0. Scores, scale q . k, may be up to 2^26 in size (beyond that a row
+ * may come out as NaN).
  * A row that sees no position (lengths[b] < n) is zeros. Positions behind
  * table_stride pages do not exist. A sequence with a page outside 0 ..
  * pool_pages - 1 among those it reads may come out as NaN.
@@ -151,8 +152,9 @@ size_t lcr_batch_attention_workspace_bytes(int batch, int tokens, int max_new, i
  *     token drawn from max(p - q, 0), behind n - 1 kept ones a token drawn from
  *     the last row's p: the first index whose running sum exceeds
  *     sample_uniforms[b] times the whole sum. (From p where max(p - q, 0) is 0
- *     everywhere.) Exponentials and sums are in fp64: whole draws hang on
- *     intervals of the running sum narrower than fp32 resolves.
+ *     everywhere.) Sums are in fp64, exponentials to 2e-13 of their value: whole
+ *     draws hang on intervals of the running sum narrower than fp32 resolves.
+ *     Logits that top-k, top-p or a grammar leave out are -inf in the rows given.
  *   T <= 0 or NaN: p is 1 at the largest logit (ties to the lowest index), a
  *     draft is kept iff it is that index.
  * A NaN logit counts as -inf. Where a row's largest logit is not finite, its p

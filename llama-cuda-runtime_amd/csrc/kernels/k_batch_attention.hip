@@ -13,8 +13,12 @@
 // two a block, which a second kernel joins. Each block finds its share from the
 // sequences' lengths by itself (a prefix sum over the batch), so nothing is
 // planned on the host and a captured call replays for other lengths. Blocks of
-// one XCD (block id mod 8) take neighbouring shares: with eight kv heads an
-// XCD's L2 holds one head's keys.
+// one XCD (block id mod 8) take neighbouring shares: with eight kv heads an XCD
+// reads one head's keys, which short caches keep in its L2.
+//
+// Sizes in the measurements below are the largest of a ragged batch: the first
+// chunk has all of the tokens named, others half to all, and caches have a third
+// to all of the positions named.
 //
 // Arithmetic. S^T = K . Q^T on 16x16x32 matrix instructions: a lane holds one
 // packed row and four keys of each sixteen. One pass over the keys:
@@ -33,13 +37,13 @@
 // values into its own part of LDS with direct loads (no registers, no barrier):
 // the next step's keys are requested as soon as the scores are taken, its values
 // when the products are. Their results meet in LDS. 64 sequences over 0.7 GB of
-// cache (head_dim 64, bf16) 115 us, 6.2 TB/s; a copy kernel reads 7.0.
+// cache (head_dim 64, bf16) 115 us, 6.2 TB/s; a streaming read reaches 7.0.
 // Many rows: bound by the exponentials (16 cycles each on the vector units) and,
 // at head_dim 128, by LDS reads and the matrix cores. The waves share 64-key
 // tiles, staged three or four deep, and split the rows, 32 each. A tile's scores
 // are all taken before its first weights, so that products and exponentials of
 // its halves overlap in a wave: 32 keys at a time were 3 to 15 % slower. Four
-// chunks of 1000 tokens, each behind 4000 positions, 165 us, 0.89 PFLOP/s; the
+// chunks of 1000 tokens behind 4000 positions (110 GFLOP) 163 us, 0.68 PFLOP/s; the
 // vector units are then busy for three quarters of it. Short prompts lose to
 // the pieces' first loads and to partials: one of 2048 takes 47 us, 0.37.
 #include <algorithm>

@@ -8,8 +8,8 @@
 // rather than waiting for another block or kernel to have done so; then the
 // blocks share the rows, the new pages and the sequences, each finding its
 // sequence by bisection. The work is a chain of dependent reads (lengths, scan,
-// bisection, table entry), so it is bound by their latency and not by bytes: 3.7
-// us for 8 sequences of one token, 5.1 for 256 with 4021 rows, 7.8 for 1024 with
+// bisection, table entry), so it is bound by their latency and not by bytes: 3.6
+// us for 8 sequences of one token, 5.2 for 256 with 4021 rows, 7.9 for 1024 with
 // 46309 (0.4 MB, which a copy moves in 0.1).
 #include <algorithm>
 #include <cstdint>

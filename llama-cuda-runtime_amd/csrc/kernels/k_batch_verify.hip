@@ -18,11 +18,13 @@
 // neighbour. gfx950 runs fp64 fma at the fp32 rate, so that a logit's 17
 // operations (10 of them fp64) take about as long as its 4 bytes: 332 rows of
 // 128256 logits (170 MB) in 40 us, of which the vector units are busy for 25 and
-// the memory, at 7 TB/s, for 24.
+// the memory, at 7 TB/s, for 24. A wave loads its part, waits, and computes, so
+// that the two overlap only where other waves of its compute unit are at the other.
 // The draw of 64 sequences takes 23 us, the rows of rejected drafts (half of
 // them, 1 MB each) and a chain of a dozen dependent reads and exchanges; alone,
-// one sequence's takes 8. Blocks of eight waves, which look at eight rows at
-// once, were slower (25 us): more waves wait for the slowest.
+// one sequence's takes 8 where all drafts are kept and 13 where one is not. Blocks
+// of eight waves, which look at eight rows at once, were slower (25 us for 64
+// sequences): more waves wait for the slowest.
 // Which block arrives last decides who computes, not what: all sums have a fixed
 // order.
 #include <algorithm>
