@@ -153,7 +153,8 @@ size_t lcr_batch_attention_workspace_bytes(int batch, int tokens, int max_new, i
  *     the last row's p: the first index whose running sum exceeds
  *     sample_uniforms[b] times the whole sum. (From p where max(p - q, 0) is 0
  *     everywhere.) Sums are in fp64, exponentials to 2e-13 of their value: whole
- *     draws hang on intervals of the running sum narrower than fp32 resolves.
+ *     draws hang on intervals of the running sum narrower than fp32 resolves. A
+ *     probability of less than 2^-1020 of its row's largest is 0.
  *     Logits that top-k, top-p or a grammar leave out are -inf in the rows given.
  *   T <= 0 or NaN: p is 1 at the largest logit (ties to the lowest index), a
  *     draft is kept iff it is that index.
