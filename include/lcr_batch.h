@@ -14,6 +14,14 @@
  *                                  keys and values into their slots
  *   lcr_batch_attention            each sequence's rows over its pages
  *   lcr_batch_verify               drafted tokens against the target's logits
+ *   lcr_batch_logprobs             what an answer says beside its tokens: their log
+ *                                  probabilities, entropies, likeliest ids
+ *
+ * and, over a cache of 8-bit numbers with a scale for every 16 positions of a
+ * head (lcr_kv8_view), in place of the second and third:
+ *
+ *   lcr_batch_norm_rope_write_kv8
+ *   lcr_batch_attention_kv8
  *
  * No counterpart in the reference, which serves one sequence.
  *
@@ -171,6 +179,110 @@ int lcr_batch_verify(int32_t* out_ids, int32_t* out_counts, const float* target_
                      size_t workspace_bytes, void* stream);
 
 size_t lcr_batch_verify_workspace_bytes(int batch, int rows, int vocab);
+
+/* Alternatives of a row, at most. */
+#define LCR_BATCH_MAX_ALTERNATIVES 32
+
+/* Log probabilities of given tokens, with their rows' entropies and likeliest ids.
+ * Of row t of the logits (rows are logits_stride floats apart), p = softmax(logits):
+ *   logprobs[t]      log p of token_ids[t]; -inf for an id past the vocabulary
+ *   ranks[t]         how many ids have a larger logit than it (0: the likeliest;
+ *                    vocab for an id past the vocabulary)
+ *   entropies[t]     -sum p log p, in nats
+ *   top_ids[t][top], top_logprobs[t][top]
+ *                    the ids of the largest logits in descending order, equal ones
+ *                    by ascending id, and their log p; top is at most
+ *                    LCR_BATCH_MAX_ALTERNATIVES. Behind a vocabulary smaller than
+ *                    top, -1 and -inf.
+ * A row whose token id is negative is left out: nothing of it is read or written.
+ * token_ids NULL: no tokens are given, logprobs and ranks are not written, and no
+ * row is left out. logprobs, ranks and entropies may each be NULL for what is not
+ * wanted, and with top 0 the last two.
+ * Sums and logarithms are fp32 over parts of 4096 logits and fp64 over those.
+ * A NaN logit counts as -inf, whose p is 0. Where a row's largest logit is not
+ * finite, p is 1 at the lowest index of that value, as for lcr_batch_verify.
+ * With a workspace of lcr_batch_logprobs_workspace_bytes (16-byte aligned) few rows
+ * are split over the device, in two launches; without one (NULL, 0, or a smaller
+ * one) a row is read by one compute unit. The same call gives the same bits. */
+int lcr_batch_logprobs(float* logprobs, int32_t* ranks, float* entropies, int32_t* top_ids, float* top_logprobs,
+                       const float* logits, const int32_t* token_ids, int rows, int top, int vocab,
+                       int logits_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t lcr_batch_logprobs_workspace_bytes(int rows, int top, int vocab);
+
+/* ---- a cache of 8-bit numbers -------------------------------------------- */
+
+/* Positions of a block: those of a head that share a scale. */
+#define LCR_KV8_BLOCK 16
+
+/* One layer of a paged cache of e4m3 numbers (four bits of exponent, three of
+ * mantissa, no infinities). Positions lie in blocks of 16, a block in a page
+ * (page_size is a multiple of 16), and block n of a page's head is
+ *   16 head_dim bytes from page * page_stride + head * head_stride + n * 16 head_dim on,
+ *   a scale at     page * scale_page_stride + head * scale_head_stride + n
+ * in keys and key_scales, values and value_scales. In a block, dim i of position t
+ * (of 16) is byte
+ *   t head_dim + i                          of its keys,
+ *   (t / 4) 4 head_dim + 4 i + t % 4        of its values: four positions side by
+ *                                           side, as matrix instructions take them.
+ * It stands for its number times the block's scale, a power of two. That is a value
+ * of the library's element type itself, so that the cache is a 16-bit one whose
+ * values were rounded. head_dim is a multiple of 16, at most 256. Strides are in
+ * bytes and in floats, and multiples of 16 bytes for the numbers, which begin on 16
+ * bytes. page_table as in lcr_kv_view. */
+typedef struct lcr_kv8_view {
+  void* keys;
+  void* values;
+  float* key_scales;
+  float* value_scales;
+  const int32_t* page_table;
+  int page_size;
+  int page_stride;
+  int head_stride;
+  int scale_page_stride;
+  int scale_head_stride;
+  int num_kv_heads;
+  int head_dim;
+} lcr_kv8_view;
+
+/* lcr_batch_norm_rope_write_kv with keys and values appended to an 8-bit cache.
+ * A row's slot, as lcr_batch_map gives it, is its position's place in the pool.
+ * A block's scale is the least power of two with which its largest number is at
+ * most 448, and at least 2^-117 (fp16: 2^-15). Writing to a block's position 0
+ * begins the block: its scale is that of the positions written in this call, and what
+ * it held counts for nothing. Writing to others keeps the block's scale if it
+ * suffices; otherwise the numbers that it holds are rounded to the larger one, in
+ * place. However often that happens, a number is off by less than one step of the
+ * last scale's grid at its size. Scales do not fall before a block is begun again
+ * (also not when drafts that raised them are rejected).
+ * Keys are normed and rotated in fp64 and rounded to fp32, where scales are
+ * decided, so that one at the edge of a power of two does not hang on the order
+ * of sums; queries as for the 16-bit cache. An infinity or a NaN is held as NaN and
+ * does not count for the scale; finite values past the largest product that the
+ * element type holds (61440 in fp16, 1.875 * 2^127 in bf16) are held as that.
+ * All rows of a call whose slots lie in one block have to be among 16 rows that
+ * follow each other, as those of a sequence are; slots differ from row to row. Of
+ * blocks for which that is not so, nothing is said but that nothing out of bounds
+ * is touched. */
+int lcr_batch_norm_rope_write_kv8(void* q_out, const lcr_kv8_view* view, const void* q, const void* k,
+                                  const void* v, const void* q_norm, const void* k_norm, float eps,
+                                  const float* rope_table, int table_positions, const int32_t* positions,
+                                  const int32_t* slots, int tokens, int num_heads, int pool_pages,
+                                  int src_row_stride, void* stream);
+
+/* lcr_batch_attention over an 8-bit cache: of the values that the cache stands for,
+ * the same results, to the rounding of sums, with the same arguments, limits and
+ * workspace rules (head_dim a multiple of 16 up to 256; 64 and 128 run on the matrix
+ * cores). Positions that no row of a sequence sees may hold anything, scales
+ * included, and numbers that a row does not see leave it as it is; a NaN that it sees
+ * makes its element NaN, also where the weight rounds to 0. */
+int lcr_batch_attention_kv8(void* out, const void* q, const lcr_kv8_view* view, const int32_t* row_starts,
+                            const int32_t* lengths, int batch, int tokens, int max_new, int num_heads,
+                            int heads_per_kv, int table_stride, int pool_pages, int q_row_stride, float scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+size_t lcr_batch_attention_kv8_workspace_bytes(int batch, int tokens, int max_new, int num_heads,
+                                               int heads_per_kv, int head_dim);
 
 #ifdef __cplusplus
 }

@@ -85,6 +85,23 @@ class KvView(ctypes.Structure):
     ]
 
 
+class Kv8View(ctypes.Structure):
+    _fields_ = [
+        ("keys", ctypes.c_void_p),
+        ("values", ctypes.c_void_p),
+        ("key_scales", ctypes.c_void_p),
+        ("value_scales", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("page_size", ctypes.c_int),
+        ("page_stride", ctypes.c_int),
+        ("head_stride", ctypes.c_int),
+        ("scale_page_stride", ctypes.c_int),
+        ("scale_head_stride", ctypes.c_int),
+        ("num_kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+    ]
+
+
 class ModelOptions(ctypes.Structure):
     _fields_ = [
         ("device", ctypes.c_int),
@@ -172,6 +189,13 @@ SIGNATURES = {
     "lcr_batch_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "lcr_batch_verify": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P]),
     "lcr_batch_verify_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "lcr_batch_logprobs": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _SZ, _P]),
+    "lcr_batch_logprobs_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "lcr_batch_norm_rope_write_kv8": (_I, [_P, ctypes.POINTER(Kv8View), _P, _P, _P, _P, _P, _F, _P, _I, _P, _P, _I, _I,
+                                           _I, _I, _P]),
+    "lcr_batch_attention_kv8": (_I, [_P, _P, ctypes.POINTER(Kv8View), _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P,
+                                     _SZ, _P]),
+    "lcr_batch_attention_kv8_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     # lcr_model.h
     "lcr_model_default_options": (None, [ctypes.POINTER(ModelOptions)]),
     "lcr_model_create": (_I, [ctypes.c_char_p, ctypes.POINTER(ModelOptions), ctypes.POINTER(_P)]),
