@@ -1,31 +1,495 @@
 // lcr_batch_attention_kv8: causal GQA attention of many sequences' rows over one
-// paged cache of 8-bit numbers.
+// paged cache of 8-bit numbers. Work division and arithmetic are
+// batch_attention.h's; this is how the cache's numbers become operands.
+//
+// A number times its block's scale is a value of the element type (kv8.h), and one
+// instruction makes two of them, so nothing is rounded on the way and the products
+// are those of a 16-bit cache. The layout gives a lane what its operands need in
+// 16 contiguous bytes: of keys 16 dims of one position, two k-steps' worth (queries
+// are loaded in the same order of dims); of values four positions of four dims.
+//
+// Few rows (at most 32): bound by the cache's bytes. The waves of a block share the
+// rows and split the keys, 32 a step. Keys and values go from memory to registers,
+// where they are widened: no LDS and no barrier until the waves' results meet.
+// Many rows: the waves share 64-key tiles and split the rows, 32 each. A wave loads
+// its part of a tile, widens it and leaves it in LDS as the operands that all waves
+// read, two tiles in turn.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "../capi_util.h"
+#include "batch_attention.h"
 #include "kv8.h"
 
 namespace lcr {
 namespace {
 
-struct BatchAttn8Args {
-  elem_t* out;
-  const elem_t* q;
-  Kv8View view;
-  const int32_t* row_starts;
-  const int32_t* lengths;
-  int batch;
-  int tokens;
-  int max_new;
-  int num_heads;
-  int group;
-  int table_stride;
-  int pool_pages;
-  int q_row_stride;
-  int held;  // positions that a table has pages for
-  float scale;
+using Args = BatchAttnArgs<Kv8View>;
+using KvPiece = Piece<uint8_t>;
+
+// ---------------------------------------------------------------------------
+// Matrix-core kernels
+// ---------------------------------------------------------------------------
+
+// kMaxRows: packed rows a sequence may have, 16, 32 or any number (0).
+template <int kDim, int kMaxRows>
+struct Shape8 {
+  static constexpr bool kMany = kMaxRows == 0;
+  static constexpr int kHeadDim = kDim;
+  static constexpr int kWaves = kMany && kHeadDim == 128 ? 8 : 4;
+  static constexpr int kThreads = 64 * kWaves;
+  // resident a compute unit
+  static constexpr int kBlocks = kHeadDim == 64 ? 3 : 1;
+  static constexpr int kFewBlocks = kHeadDim == 64 ? (kMaxRows == 16 ? 4 : 3) : 2;
+  static constexpr int kSimdWaves = kWaves * (kMany ? kBlocks : kFewBlocks) / 4;
+  static constexpr int kTileRows = 32 * kWaves;     // packed rows of a tile of many rows
+  static constexpr int kSteps = kHeadDim / 32;      // k-steps of a score
+  static constexpr int kDFrags = kHeadDim / 16;     // output fragments
+  static constexpr int kChunks = kHeadDim / 64;     // 16-byte chunks of a lane's in a block
+  static constexpr int kBlockBytes = kKv8Block * kHeadDim;
+  static constexpr int kTileElems = 2 * 64 * kHeadDim;  // many rows: a tile's keys, then its values
+  static constexpr int kFewStepKeys = kHeadDim == 64 ? 96 : 192;
+  static constexpr int kDepth = kMaxRows == 16 ? 2 : 1;  // few rows: steps in flight
+  static constexpr int kFewFrags = kMaxRows == 16 ? 1 : 2;
+  static constexpr int kWaveOutputs = 16 * kFewFrags * kHeadDim;
+
+  // Chunk h of keys has dims 64 h + 16 grp .. + 15, k-steps 2 h and 2 h + 1.
+  static __device__ __forceinline__ int q_dim(int ks, int grp) { return 64 * (ks >> 1) + 16 * grp + 8 * (ks & 1); }
+  // Row m of output fragment 4 h + j is dim 64 h + 4 m + j, so that a lane's
+  // 4 grp + e of four fragments are neighbours.
+  static __device__ __forceinline__ int out_dim(int n, int grp) { return 64 * (n >> 2) + 16 * grp + 4 * (n & 3); }
+  static __device__ __forceinline__ mfma_acc4 out_piece(const mfma_acc4* o, int n) {
+    const mfma_acc4* f = o + (n & ~3);
+    const int e = n & 3;
+    return mfma_acc4{f[0][e], f[1][e], f[2][e], f[3][e]};
+  }
 };
+
+template <typename Shape>
+struct Lds8 {
+  union {
+    float outputs[Shape::kWaves * Shape::kWaveOutputs];  // few rows: the waves' results
+    elem_t tiles[Shape::kMany ? 2 : 1][Shape::kMany ? Shape::kTileElems : 8];
+  };
+  float stats[Shape::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
+  uint32_t sums[Shape::kWaves];
+  ShareStart found;
+  int bad;         // a page outside the pool was read
+  int special[2];  // many rows: the last tile of even and of odd number whose values hold NaN
+};
+
+// Two neighbouring numbers of a word as elements.
+template <bool kHigh>
+__device__ __forceinline__ uint32_t widen_pair(uint32_t numbers, float scale) {
+#if defined(LCR_ELEM_FP16)
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(numbers, scale, kHigh));
+#else
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(numbers, scale, kHigh));
+#endif
+}
+
+__device__ __forceinline__ mfma_in8 widen(uint32_t a, float scale_a, uint32_t b, float scale_b) {
+  return as_operand(vec16{{widen_pair<false>(a, scale_a), widen_pair<true>(a, scale_a), widen_pair<false>(b, scale_b),
+                           widen_pair<true>(b, scale_b)}});
+}
+
+// A tile without the infinities and NaN of its values.
+template <typename Tile>
+struct Cleared {
+  const Tile& tile;
+
+  __device__ __forceinline__ mfma_in8 value(int half, int df) const {
+    vec16 v = __builtin_bit_cast(vec16, tile.value(half, df));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((v.w[i] & kInfBits) == kInfBits) v.w[i] &= 0xffff0000u;
+      if (((v.w[i] >> 16) & kInfBits) == kInfBits) v.w[i] &= 0xffffu;
+    }
+    return as_operand(v);
+  }
+};
+
+// Whether a word of numbers holds a NaN (0x7f, 0xff).
+__device__ __forceinline__ bool number_nan(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+
+// A word of four positions' numbers without those from `count` on.
+__device__ __forceinline__ uint32_t first_numbers(int count) {
+  return count >= 4 ? ~0u : (1u << (8 * max(count, 0))) - 1u;
+}
+
+typedef const __attribute__((address_space(4))) int32_t* constant_ints;
+typedef const __attribute__((address_space(4))) float* constant_floats;
+
+// Where 16 positions of a sequence lie: the same for the whole wave.
+struct BlockPlace {
+  int page;   // as the table has it
+  int block;  // within the page
+};
+
+// Of the piece's keys 16 n .. 16 n + 15; blocks past the last repeat it.
+__device__ __forceinline__ BlockPlace find_block(const Args& a, const TiledPlan& plan, const KvPiece& p, int n) {
+  const constant_ints table = (constant_ints)(reinterpret_cast<uintptr_t>(p.table));
+  const int at = uniform(min(n, (p.key1 - 1) / kKv8Block));
+  const int index = plan.by_page(at * kKv8Block);
+  return BlockPlace{table[index], at - index * (a.view.page_size / kKv8Block)};
+}
+
+// One chunk of a block's keys and values, as a lane loads them, and their scales.
+struct BlockScales {
+  float key;
+  float value;
+};
+
+template <bool kStream>
+__device__ __forceinline__ vec16 load_numbers(const uint8_t* base, uint32_t at) {
+  if constexpr (kStream) {
+    return load16_stream(base + at);
+  } else {
+    return load16(base + at);
+  }
+}
+
+__device__ __forceinline__ BlockScales load_scales(const Args& a, const KvPiece& p, int page, int block) {
+  const size_t at = a.view.scale_at(page, p.kv, block);
+  return BlockScales{((constant_floats)(reinterpret_cast<uintptr_t>(a.view.key_scales)))[at],
+                     ((constant_floats)(reinterpret_cast<uintptr_t>(a.view.value_scales)))[at]};
+}
+
+template <typename Shape>
+__device__ __forceinline__ uint32_t key_chunk_at(int h) {
+  return static_cast<uint32_t>((lane_id() & 15) * Shape::kHeadDim + 64 * h + 16 * (lane_id() >> 4));
+}
+template <typename Shape>
+__device__ __forceinline__ uint32_t value_chunk_at(int h) {
+  return static_cast<uint32_t>((lane_id() >> 4) * 4 * Shape::kHeadDim + 256 * h + 16 * (lane_id() & 15));
+}
+
+// 32 keys and their values in registers.
+template <typename Shape>
+struct RawTile {
+  vec16 keys[2][Shape::kChunks];
+  vec16 values[2][Shape::kChunks];
+  BlockScales scales[2];
+
+  __device__ __forceinline__ mfma_in8 key(int kf, int ks) const {
+    const vec16& c = keys[kf][ks >> 1];
+    const int w = 2 * (ks & 1);
+    return widen(c.w[w], scales[kf].key, c.w[w + 1], scales[kf].key);
+  }
+  __device__ __forceinline__ mfma_in8 value(int, int df) const {
+    return widen(values[0][df >> 2].w[df & 3], scales[0].value, values[1][df >> 2].w[df & 3], scales[1].value);
+  }
+};
+
+// The values of a RawTile in LDS, a word of four positions at a time, for loops that
+// are not unrolled.
+template <typename Shape>
+struct StashedValues {
+  uint32_t* words;
+  BlockScales scales[2];
+
+  __device__ __forceinline__ StashedValues(const RawTile<Shape>& tile, float* lds)
+      : words(reinterpret_cast<uint32_t*>(lds)), scales{tile.scales[0], tile.scales[1]} {
+    static_assert(Shape::kWaveOutputs >= 64 * 2 * Shape::kDFrags, "a wave's values fit");
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int df = 0; df < Shape::kDFrags; ++df) words[at(n, df)] = tile.values[n][df >> 2].w[df & 3];
+    }
+    lds_settled();
+  }
+  static __device__ __forceinline__ int at(int n, int df) { return (n * Shape::kDFrags + df) * 64 + lane_id(); }
+  __device__ __forceinline__ mfma_in8 value(int, int df) const {
+    return widen(words[at(0, df)], scales[0].value, words[at(1, df)], scales[1].value);
+  }
+};
+
+// At most 32 rows: the waves split the keys.
+template <typename Shape, int kTileRows>
+__device__ __forceinline__ void few_rows(Lds8<Shape>& lds, const Args& a, const TiledPlan& plan, const KvPiece& p) {
+  constexpr int kDepth = Shape::kDepth;
+  constexpr int kRF = Shape::kFewFrags;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int tiles = (p.key1 - p.key0 + 31) / 32;
+  const int count = tiles > wave ? (tiles - wave - 1) / Shape::kWaves + 1 : 0;
+  int bad = 0;
+  auto first_key = [&](int t) { return p.key0 + 32 * (wave + Shape::kWaves * t); };
+  struct Places {
+    BlockPlace of[2];
+  };
+  auto places_of = [&](int t) {
+    const int n = first_key(t) / kKv8Block;
+    return Places{{find_block(a, plan, p, n), find_block(a, plan, p, n + 1)}};
+  };
+  auto load_keys = [&](RawTile<Shape>& tile, const Places& places) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int page = pool_page(a, places.of[n].page, bad);
+      const uint8_t* from = p.keys + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                            static_cast<size_t>(places.of[n].block * Shape::kBlockBytes);
+#pragma unroll
+      for (int h = 0; h < Shape::kChunks; ++h) tile.keys[n][h] = load_numbers<true>(from, key_chunk_at<Shape>(h));
+      tile.scales[n].key = load_scales(a, p, page, places.of[n].block).key;
+    }
+  };
+  auto load_values = [&](RawTile<Shape>& tile, const Places& places) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int page = pool_page(a, places.of[n].page, bad);
+      const uint8_t* from = p.values + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                            static_cast<size_t>(places.of[n].block * Shape::kBlockBytes);
+#pragma unroll
+      for (int h = 0; h < Shape::kChunks; ++h) tile.values[n][h] = load_numbers<true>(from, value_chunk_at<Shape>(h));
+      tile.scales[n].value = load_scales(a, p, page, places.of[n].block).value;
+    }
+  };
+
+  TiledRows<Shape, kRF> rows;
+  rows.clear();
+  RawTile<Shape> raw[kDepth];
+  Places next{};
+  if (count > 0) {
+    load_rows(rows, a, plan, p, 0);
+#pragma unroll
+    for (int t = 0; t < kDepth; ++t) {
+      if (t < count) {
+        const Places places = places_of(t);
+        load_keys(raw[t], places);
+        load_values(raw[t], places);
+      }
+    }
+    next = places_of(min(kDepth, count - 1));
+  }
+  const int all_seen = min(p.seen_first, p.key1);
+  for (int t0 = 0; t0 < count; t0 += kDepth) {
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int t = t0 + u;
+      if (t >= count) break;
+      RawTile<Shape>& tile = raw[u];
+      const bool more = t + kDepth < count;
+      const Places places = next;
+      const int key0 = first_key(t);
+      const bool whole = key0 + 32 <= all_seen;
+      TileWork<Shape, kRF, 2> work;
+      work.scores(rows, tile);
+      if (more) {
+        load_keys(tile, places);
+        next = places_of(min(t + kDepth + 1, count - 1));
+      }
+      if (!whole) work.mask(rows, key0);
+      work.raise_base(rows, plan.scale_log2e);
+      work.weights(rows, plan.scale_log2e, 0);
+      bool special = false;
+      if (!whole) {
+        // numbers behind the last key that counts may be any
+        bool found = false;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const uint32_t keep = first_numbers(p.key1 - key0 - 16 * n - 4 * (lane_id() >> 4));
+#pragma unroll
+          for (int h = 0; h < Shape::kChunks; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              tile.values[n][h].w[i] &= keep;
+              found |= number_nan(tile.values[n][h].w[i]);
+            }
+          }
+        }
+        special = __any(found);
+      }
+      if (special) {
+        const StashedValues<Shape> values(tile, lds.outputs + wave * Shape::kWaveOutputs);
+        work.mark_special(rows, values, key0);
+        work.products(rows, Cleared<StashedValues<Shape>>{values}, 0);
+      } else {
+        work.products(rows, tile, 0);
+      }
+      if (more) load_values(tile, places);
+    }
+  }
+  join_waves<Shape, kTileRows, Shape::kWaveOutputs>(rows, bad, lds.outputs, lds.stats, a, plan, p);
+}
+
+// 64 keys and their values as operands in LDS: lane by lane, 16 bytes each.
+template <typename Shape>
+struct OperandTile {
+  const elem_t* tile;
+
+  static __device__ __forceinline__ int key_at(int kf, int ks) { return ((kf * Shape::kSteps + ks) * 64 + lane_id()) * 8; }
+  static __device__ __forceinline__ int value_at(int half, int df) {
+    return 64 * Shape::kHeadDim + ((half * Shape::kDFrags + df) * 64 + lane_id()) * 8;
+  }
+  __device__ __forceinline__ mfma_in8 key(int kf, int ks) const { return lds_operand(tile + key_at(kf, ks)); }
+  __device__ __forceinline__ mfma_in8 value(int half, int df) const { return lds_operand(tile + value_at(half, df)); }
+};
+
+// The lower or upper half of a tile, as a tile.
+template <typename Shape>
+struct OperandHalf {
+  const OperandTile<Shape>& tile;
+  int half;
+
+  __device__ __forceinline__ mfma_in8 key(int kf, int ks) const { return tile.key(2 * half + kf, ks); }
+  __device__ __forceinline__ mfma_in8 value(int, int df) const { return tile.value(half, df); }
+};
+
+// Many rows: the waves split them, 32 each, and share the tiles. `tiles_done`:
+// of the block's pieces before, so that a tile's number is its own.
+template <typename Shape>
+__device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const TiledPlan& plan, const KvPiece& p,
+                                          int& tiles_done) {
+  constexpr int kRF = 2;
+  static_assert(Shape::kWaves == 4 * Shape::kChunks, "a wave stages one chunk of one block of a tile");
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int my_block = wave / Shape::kChunks;
+  const int my_chunk = wave % Shape::kChunks;
+  const int tiles = (p.key1 - p.key0 + 63) / 64;
+  int bad = 0;
+  if (threadIdx.x == 0) lds.bad = 0;
+
+  struct Raw {
+    vec16 keys;
+    vec16 values;
+    BlockScales scales;
+  };
+  auto place_of = [&](int t) { return find_block(a, plan, p, (p.key0 + 64 * t) / kKv8Block + my_block); };
+  auto load = [&](const BlockPlace& place) {
+    const int page = pool_page(a, place.page, bad);
+    const size_t at = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                      static_cast<size_t>(place.block * Shape::kBlockBytes);
+    Raw raw;
+    raw.keys = load_numbers<false>(p.keys + at, key_chunk_at<Shape>(my_chunk));
+    raw.values = load_numbers<false>(p.values + at, value_chunk_at<Shape>(my_chunk));
+    raw.scales = load_scales(a, p, page, place.block);
+    return raw;
+  };
+  // Widens a wave's part of tile t and leaves it in LDS.
+  auto stage = [&](int t, Raw& raw) {
+    elem_t* tile = lds.tiles[t & 1];
+    const int key0 = p.key0 + 64 * t + 16 * my_block;
+    if (p.key0 + 64 * t + 64 > p.seen_first) {
+      // A tile that some row of the unit does not see whole. Numbers behind the
+      // last key that counts may be any.
+      const uint32_t keep = first_numbers(p.key1 - key0 - 4 * (lane_id() >> 4));
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        raw.values.w[i] &= keep;
+        found |= number_nan(raw.values.w[i]);
+      }
+      if (__any(found) && lane_id() == 0) lds.special[(tiles_done + t) & 1] = tiles_done + t;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<mfma_in8*>(tile + OperandTile<Shape>::key_at(my_block, 2 * my_chunk + i)) =
+          widen(raw.keys.w[2 * i], raw.scales.key, raw.keys.w[2 * i + 1], raw.scales.key);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint2 four = make_uint2(widen_pair<false>(raw.values.w[i], raw.scales.value),
+                                    widen_pair<true>(raw.values.w[i], raw.scales.value));
+      *reinterpret_cast<uint2*>(tile + OperandTile<Shape>::value_at(my_block >> 1, 4 * my_chunk + i) +
+                                4 * (my_block & 1)) = four;
+    }
+  };
+
+  const int row0 = 32 * wave;
+  const bool active = row0 < p.rows;
+  TiledRows<Shape, kRF> rows;
+  rows.clear();
+  int all_seen = 0, any_seen = 0;
+  if (active) {
+    load_rows(rows, a, plan, p, row0);
+    all_seen = min(keys_seen(a, p.before, packed_token(plan, row0)), p.key1);
+    any_seen = min(keys_seen(a, p.before, packed_token(plan, min(row0 + 31, p.rows - 1))), p.key1);
+  }
+  Raw raw{};
+  BlockPlace next{};
+  if (tiles > 0) {
+    raw = load(place_of(0));
+    const BlockPlace second = place_of(min(1, tiles - 1));
+    next = place_of(min(2, tiles - 1));
+    stage(0, raw);
+    if (tiles > 1) raw = load(second);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    // Behind the barrier tile t is staged, and the tile before has been read.
+    lds_settled();
+    plain_barrier();
+    if (t + 1 < tiles) {
+      stage(t + 1, raw);
+      if (t + 2 < tiles) {
+        raw = load(next);
+        next = place_of(min(t + 3, tiles - 1));
+      }
+    }
+    const int tile0 = p.key0 + 64 * t;
+    if (tile0 >= any_seen) continue;
+    const bool whole = tile0 + 64 <= all_seen;
+    const bool special = tile0 + 64 > p.seen_first && uniform(lds.special[(tiles_done + t) & 1]) == tiles_done + t;
+    const OperandTile<Shape> tile{lds.tiles[t & 1]};
+    TileWork<Shape, kRF, 4> work;
+    work.scores(rows, tile);
+    if (!whole) work.mask(rows, tile0);
+    work.raise_base(rows, plan.scale_log2e);
+    if (!special) {
+      work.weights(rows, plan.scale_log2e, 0);
+      work.products(rows, tile, 0);
+      work.weights(rows, plan.scale_log2e, 1);
+      work.products(rows, tile, 1);
+      continue;
+    }
+    // Half a tile at a time, its scores once more: registers for the marks.
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const OperandHalf<Shape> part{tile, half};
+      TileWork<Shape, kRF, 2> again;
+      again.scores(rows, part);
+      if (!whole) again.mask(rows, tile0 + 32 * half);
+      again.weights(rows, plan.scale_log2e, 0);
+      again.mark_special(rows, part, tile0 + 32 * half);
+      again.products(rows, Cleared<OperandHalf<Shape>>{part}, 0);
+    }
+  }
+  tiles_done += max(tiles, 0);
+  if (__any(bad != 0) && lane_id() == 0) lds.bad = 1;
+  __syncthreads();  // every wave is done with the tiles; the flag is set
+  if (!active) return;
+  rows.add_special();
+  store_rows(rows, lds.bad != 0, row0, a, plan, p);
+}
+
+template <typename Shape>
+__global__ __launch_bounds__(Shape::kThreads, Shape::kSimdWaves) void batch_attention_kv8_kernel(Args args,
+                                                                                               TiledPlan tiled_plan) {
+  constexpr bool kMany = Shape::kMany;
+  constexpr int kTileRows = kMany ? Shape::kTileRows : kFewRows;
+  __shared__ __attribute__((aligned(1024))) Lds8<Shape> lds;
+  Args a = args;
+  a.view.page_size = own_register(a.view.page_size);
+  a.view.page_stride = own_register(a.view.page_stride);
+  a.pool_pages = own_register(a.pool_pages);
+  a.held = own_register(a.held);
+  a.group = own_register(a.group);
+  TiledPlan plan = tiled_plan;
+  plan.by_page.magic = own_register(plan.by_page.magic);
+  plan.by_page.shift = own_register(plan.by_page.shift);
+  plan.group_magic = own_register(plan.group_magic);
+  plan.scale_log2e = own_register(plan.scale_log2e);
+  // seen by every wave behind the barriers of the search for the share
+  if (threadIdx.x == 0) lds.special[0] = lds.special[1] = -1;
+  int tiles_done = 0;
+  walk_share<Shape, kMany, uint8_t>(
+      a, plan, lds.sums, &lds.found,
+      [&](const KvPiece& p) { few_rows<Shape, kTileRows>(lds, a, plan, p); },
+      [&](const KvPiece& p) {
+        if constexpr (kMany) many_rows<Shape>(lds, a, plan, p, tiles_done);
+      });
+}
 
 // ---------------------------------------------------------------------------
 // Any head_dim that is a multiple of 16 up to 256: a wave per (row, query head).
@@ -45,7 +509,7 @@ __device__ __forceinline__ void wave_settled() {
 // their scales, go through LDS, and lane L then holds elements L, L + 64, ... of
 // the output. Nothing is shared between heads or rows and nothing split: the way
 // for what the tiles above do not take, not for speed.
-__global__ __launch_bounds__(kGenericThreads) void batch_attention_kv8_generic_kernel(BatchAttn8Args a) {
+__global__ __launch_bounds__(kGenericThreads) void batch_attention_kv8_generic_kernel(Args a) {
   constexpr int kDims = kGenericMaxDim / 64;
   __shared__ float q_lds[kGenericWaves][kGenericMaxDim];
   __shared__ float weights[kGenericWaves][64];
@@ -134,6 +598,51 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_kv8_generic_k
   }
 }
 
+template <int kHeadDim, int kMaxRows>
+void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  using Shape = Shape8<kHeadDim, kMaxRows>;
+  constexpr int kTileRows = kMaxRows == 0 ? Shape::kTileRows : kFewRows;
+  const TiledPlan plan = plan_tiled<Shape>(a, workspace, workspace_bytes);
+  const unsigned blocks = static_cast<unsigned>(plan.shares) * static_cast<unsigned>(a.view.num_kv_heads);
+  batch_attention_kv8_kernel<Shape><<<blocks, Shape::kThreads, 0, s>>>(a, plan);
+  if (!plan.split) return;
+  // A row is a chain of loads, so few follow each other: one time round for
+  // many rows, two for few.
+  constexpr bool kRowEach = kMaxRows == 0;
+  const dim3 join(blocks, kRowEach ? kTileRows / (4 * 256 / kHeadDim) : kTileRows / 8);
+  batch_attention_join_kernel<kHeadDim, kRowEach, Args><<<join, kJoinThreads, 0, s>>>(a, plan, kTileRows);
+}
+
+template <int kHeadDim>
+void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const long long most = static_cast<long long>(a.max_new) * a.group;
+  if (most <= 16) {
+    launch_tiled<kHeadDim, 16>(a, workspace, workspace_bytes, s);
+  } else if (most <= kFewRows) {
+    launch_tiled<kHeadDim, 32>(a, workspace, workspace_bytes, s);
+  } else {
+    launch_tiled<kHeadDim, 0>(a, workspace, workspace_bytes, s);
+  }
+}
+
+bool on_bytes(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The matrix-core kernels take a positive scale (the running maximum is the
+// scores') and a group that fits a tile.
+bool tiled_takes(const Args& a) {
+  return (a.view.head_dim == 64 || a.view.head_dim == 128) &&
+         a.group <= (a.view.head_dim == 64 ? Shape8<64, 0>::kTileRows : Shape8<128, 0>::kTileRows) && a.scale > 0.0f &&
+         a.scale < 1e30f && a.q_row_stride % 8 == 0 && on_bytes(a.q, 16) && on_bytes(a.out, 8);
+}
+
+template <int kHeadDim>
+size_t workspace_for(int max_new, int kv_heads, int group) {
+  const long long most = static_cast<long long>(max_new) * group;
+  if (most <= 16) return tiled_workspace<Shape8<kHeadDim, 16>>(max_new, kv_heads, group);
+  if (most <= kFewRows) return tiled_workspace<Shape8<kHeadDim, 32>>(max_new, kv_heads, group);
+  return tiled_workspace<Shape8<kHeadDim, 0>>(max_new, kv_heads, group);
+}
+
 }  // namespace
 }  // namespace lcr
 
@@ -141,6 +650,10 @@ using namespace lcr;
 
 extern "C" size_t lcr_batch_attention_kv8_workspace_bytes(int batch, int tokens, int max_new, int num_heads,
                                                           int heads_per_kv, int head_dim) {
+  if (batch <= 0 || tokens <= 0 || max_new <= 0 || num_heads <= 0 || heads_per_kv <= 0) return 0;
+  const int kv_heads = std::max(1, num_heads / heads_per_kv);
+  if (head_dim == 64) return workspace_for<64>(max_new, kv_heads, heads_per_kv);
+  if (head_dim == 128) return workspace_for<128>(max_new, kv_heads, heads_per_kv);
   return 0;
 }
 
@@ -181,15 +694,29 @@ extern "C" int lcr_batch_attention_kv8(void* out, const void* q, const lcr_kv8_v
   CAPI_CHECK(workspace != nullptr || workspace_bytes == 0,
              "batch attention workspace of " << workspace_bytes << " bytes has no pointer");
   CAPI_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "batch attention workspace must be 16-byte aligned");
-  BatchAttn8Args a{static_cast<elem_t*>(out), static_cast<const elem_t*>(q), Kv8View::from_c(*view), row_starts,
+  Args a{static_cast<elem_t*>(out), static_cast<const elem_t*>(q), Kv8View::from_c(*view), row_starts,
                    lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride,
                    table_stride * view->page_size, scale};
   auto s = static_cast<hipStream_t>(stream);
+  const bool tiled = tiled_takes(a);
   // A launch has fewer than 2^32 threads in all.
   const long long units = static_cast<long long>(tokens) * num_heads;
-  const long long blocks = (units + kGenericWaves - 1) / kGenericWaves;
-  CAPI_CHECK(blocks * kGenericThreads <= UINT32_MAX, "batch attention of " << tokens << " rows of " << num_heads
-                                                                           << " heads needs more than 2^32 threads");
+  const long long blocks =
+      !tiled ? (units + kGenericWaves - 1) / kGenericWaves
+             : view->num_kv_heads * (view->head_dim == 64 ? most_tiled_units<Shape8<64, 32>>(a)
+                                                          : most_tiled_units<Shape8<128, 32>>(a));
+  const int threads = !tiled ? kGenericThreads : view->head_dim == 64 ? Shape8<64, 0>::kThreads : Shape8<128, 0>::kThreads;
+  CAPI_CHECK(blocks * threads <= UINT32_MAX, "batch attention of " << tokens << " rows of " << num_heads
+                                                                   << " heads needs more than 2^32 threads");
+  if (tiled) {
+    if (view->head_dim == 64) {
+      launch_tiled<64>(a, workspace, workspace_bytes, s);
+    } else {
+      launch_tiled<128>(a, workspace, workspace_bytes, s);
+    }
+    CAPI_LAUNCHED();
+    return LCR_OK;
+  }
   batch_attention_kv8_generic_kernel<<<static_cast<unsigned>(blocks), kGenericThreads, 0, s>>>(a);
   CAPI_LAUNCHED();
   return LCR_OK;
