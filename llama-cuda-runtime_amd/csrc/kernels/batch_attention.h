@@ -13,8 +13,8 @@
 // two a block, which a second kernel joins. Each block finds its share from the
 // sequences' lengths by itself (a prefix sum over the batch), so nothing is
 // planned on the host and a captured call replays for other lengths. Blocks of
-// one XCD (block id mod 8) take neighbouring shares: with eight kv heads an XCD
-// reads one head's keys, which short caches keep in its L2.
+// one XCD (block id mod 8) take neighbouring shares (kNeighbours): with eight kv
+// heads an XCD reads one head's keys, which short caches keep in its L2.
 //
 // Arithmetic. S^T = K . Q^T on 16x16x32 matrix instructions: a lane holds one
 // packed row and four keys of each sixteen. One pass over the keys:
@@ -29,8 +29,9 @@
 // is fp32.
 //
 // A kernel's Shape says how many waves a block has (kWaves, kThreads) and rows a
-// tile of many (kTileRows), how its lanes hold dims (q_dim, out_dim, out_piece), and
-// what a step of few rows weighs beside one of many (kFewStepKeys).
+// tile of many (kTileRows), how its lanes hold dims (q_dim, out_dim, out_piece),
+// what a step of few rows weighs beside one of many (kFewStepKeys), and which
+// blocks take neighbouring shares (kNeighbours).
 #pragma once
 
 #include <algorithm>
@@ -286,6 +287,7 @@ struct Piece {
   int key0;        // keys [key0, key1)
   int key1;
   int slot;        // partial slot, or -1: the unit is whole
+  int done;        // steps of the share before it
 };
 
 // kTop: the exponent of a row's largest weight when its base is taken. The base is
@@ -708,13 +710,16 @@ __device__ __forceinline__ void store_rows(const TiledRows<Shape, kRF>& rows, bo
 
 // A block's share, piece by piece: few(piece) for pieces of at most 32 rows,
 // many(piece) for others (kMany).
-template <typename Shape, bool kMany, typename Number, typename Args, typename Few, typename Many>
+// begin(steps) is told the share's length.
+template <typename Shape, bool kMany, typename Number, typename Args, typename Begin, typename Few, typename Many>
 __device__ __forceinline__ void walk_share(const Args& a, const TiledPlan& plan, uint32_t* sums, ShareStart* found_at,
-                                           const Few& few, const Many& many) {
+                                           const Begin& begin, const Few& few, const Many& many) {
   constexpr int kHeadDim = Shape::kHeadDim;
   // Share: neighbours on one XCD where the grid is a multiple of 8.
   const unsigned blocks = gridDim.x;
-  const int block = static_cast<int>(blocks % 8u == 0 ? blockIdx.x % 8u * (blocks / 8u) + blockIdx.x / 8u : blockIdx.x);
+  const int block = static_cast<int>(Shape::kNeighbours && blocks % 8u == 0
+                                         ? blockIdx.x % 8u * (blocks / 8u) + blockIdx.x / 8u
+                                         : blockIdx.x);
   const int kv = plan.by_shares(block);
   const ShareStart found =
       find_share<Shape, kMany>(a, plan, block - kv * plan.shares, sums, found_at);
@@ -723,7 +728,9 @@ __device__ __forceinline__ void walk_share(const Args& a, const TiledPlan& plan,
   int b = found.sequence;
   Sequence seq = found.seq;
   int at = (block - kv * plan.shares) * found.share;
+  const int first = at;
   const int end = min(at + found.share, found.total);
+  begin(end - first);
   int before = found.before;  // steps before the sequence
   // The tile that the share begins in: the last that starts at or before it.
   int tile = 0;
@@ -757,6 +764,7 @@ __device__ __forceinline__ void walk_share(const Args& a, const TiledPlan& plan,
     p.key0 = 0;
     p.key1 = p.seen_last;
     p.slot = -1;
+    p.done = max(start, at) - first;
     // A short unit is not cut: it goes to the share that it begins in.
     const bool whole = !plan.split || stop - start <= kWholeSteps<kMany>;
     if (!whole && (start < at || stop > end)) {

@@ -67,6 +67,7 @@ struct TiledShape {
   // 74, 74 and 79 us, of 128 121, 105, 95 and 90; 64 beside two of 512: 102, 95, 99
   // and 97, and 248, 184, 156 and 147.
   static constexpr int kFewStepKeys = kHeadDim == 64 ? 96 : 192;
+  static constexpr bool kNeighbours = true;
 
   // A lane's first dim of k-step ks of a query, and of four neighbouring dims of its
   // outputs.
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(TiledShape<kHeadDim>::kThreads, TiledShape<kHeadDim
   if (threadIdx.x == 0) lds.special[0] = lds.special[1] = -1;
   int tiles_done = 0;
   walk_share<Shape, kMany, elem_t>(
-      a, plan, lds.sums, &lds.found,
+      a, plan, lds.sums, &lds.found, [](int) {},
       [&](const KvPiece& p) {
         few_rows<kHeadDim, kWholePages, kMaxRows == 16 ? 1 : 2, kTileRows>(lds, a, plan, p);
       },

@@ -37,11 +37,11 @@ template <int kDim, int kMaxRows>
 struct Shape8 {
   static constexpr bool kMany = kMaxRows == 0;
   static constexpr int kHeadDim = kDim;
-  static constexpr int kWaves = kMany && kHeadDim == 128 ? 8 : 4;
+  static constexpr int kWaves = kMaxRows == 16 || (kMany && kHeadDim == 128) ? 8 : 4;
   static constexpr int kThreads = 64 * kWaves;
   // resident a compute unit
   static constexpr int kBlocks = kHeadDim == 64 ? 3 : 1;
-  static constexpr int kFewBlocks = kHeadDim == 64 ? (kMaxRows == 16 ? 4 : 3) : 2;
+  static constexpr int kFewBlocks = kMaxRows == 16 && kHeadDim == 128 ? 1 : 2;
   static constexpr int kSimdWaves = kWaves * (kMany ? kBlocks : kFewBlocks) / 4;
   static constexpr int kTileRows = 32 * kWaves;     // packed rows of a tile of many rows
   static constexpr int kSteps = kHeadDim / 32;      // k-steps of a score
@@ -50,7 +50,12 @@ struct Shape8 {
   static constexpr int kBlockBytes = kKv8Block * kHeadDim;
   static constexpr int kTileElems = 2 * 64 * kHeadDim;  // many rows: a tile's keys, then its values
   static constexpr int kFewStepKeys = kHeadDim == 64 ? 96 : 192;
-  static constexpr int kDepth = kMaxRows == 16 ? 2 : 1;  // few rows: steps in flight
+  // Few rows read each key once, and an XCD that reads one head alone loads some
+  // memory channels more than others: 64 sequences of 8000 positions 65.5 us with
+  // neighbouring shares on an XCD, 63.8 without.
+  static constexpr bool kNeighbours = kMany;
+  static constexpr bool kPaced = kMany && kBlocks > 1;  // blocks of a compute unit take turns (Pace)
+  static constexpr int kFewStepBlocks = 2;          // few rows: blocks of a wave's step
   static constexpr int kFewFrags = kMaxRows == 16 ? 1 : 2;
   static constexpr int kWaveOutputs = 16 * kFewFrags * kHeadDim;
 
@@ -72,11 +77,47 @@ struct Lds8 {
     float outputs[Shape::kWaves * Shape::kWaveOutputs];  // few rows: the waves' results
     elem_t tiles[Shape::kMany ? 2 : 1][Shape::kMany ? Shape::kTileElems : 8];
   };
+  // many rows: the NaN of a tile's values, a lane's words as it loaded them
+  vec16 marks[Shape::kMany ? 2 : 1][Shape::kMany ? Shape::kThreads : 1];
   float stats[Shape::kWaves][kFewRows][2];  // few rows: a wave's bases and sums
   uint32_t sums[Shape::kWaves];
   ShareStart found;
   int bad;         // a page outside the pool was read
   int special[2];  // many rows: the last tile of even and of odd number whose values hold NaN
+};
+
+// The blocks of a compute unit take turns by how far they are. Waves that were there
+// first are served first, so that of three blocks with equal shares the oldest was
+// done after 107 us, the second after 137 and the third, at last alone, after 170
+// (four chunks of 1000 tokens behind 4000 positions). A wave's priority falls when
+// half of its share is done, and half of the rest, and half of that: the same
+// chunks take 147 us for 158, and two of them beside 16 single tokens 66 for 72;
+// falling by quarters 150 and 68.
+struct Pace {
+  int left;       // steps of the share
+  int next;       // steps done at which the priority falls
+  int level = 0;  // the priority; at 0 it stays
+
+  __device__ __forceinline__ void begin(int steps) {
+    left = steps;
+    next = steps - (left >>= 1);
+    level = 3;
+    __builtin_amdgcn_s_setprio(3);
+  }
+  __device__ __forceinline__ void reached(int steps) {
+    while (steps >= next && level > 0) {
+      next += left - (left >> 1);
+      left >>= 1;
+      --level;
+      if (level == 2) {
+        __builtin_amdgcn_s_setprio(2);
+      } else if (level == 1) {
+        __builtin_amdgcn_s_setprio(1);
+      } else {
+        __builtin_amdgcn_s_setprio(0);
+      }
+    }
+  }
 };
 
 // Two neighbouring numbers of a word as elements.
@@ -94,25 +135,10 @@ __device__ __forceinline__ mfma_in8 widen(uint32_t a, float scale_a, uint32_t b,
                            widen_pair<true>(b, scale_b)}});
 }
 
-// A tile without the infinities and NaN of its values.
-template <typename Tile>
-struct Cleared {
-  const Tile& tile;
-
-  __device__ __forceinline__ mfma_in8 value(int half, int df) const {
-    vec16 v = __builtin_bit_cast(vec16, tile.value(half, df));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if ((v.w[i] & kInfBits) == kInfBits) v.w[i] &= 0xffff0000u;
-      if (((v.w[i] >> 16) & kInfBits) == kInfBits) v.w[i] &= 0xffffu;
-    }
-    return as_operand(v);
-  }
-};
-
-// Whether a word of numbers holds a NaN (0x7f, 0xff).
-__device__ __forceinline__ bool number_nan(uint32_t w) {
-  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+// All bits of the bytes of a word of numbers that are NaN (0x7f, 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  const uint32_t marks = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (marks >> 7) * 0xffu;
 }
 
 // A word of four positions' numbers without those from `count` on.
@@ -167,20 +193,23 @@ __device__ __forceinline__ uint32_t value_chunk_at(int h) {
   return static_cast<uint32_t>((lane_id() >> 4) * 4 * Shape::kHeadDim + 256 * h + 16 * (lane_id() & 15));
 }
 
-// 32 keys and their values in registers.
+// A step's keys and their values in registers, a block of 16 beside the other.
 template <typename Shape>
 struct RawTile {
-  vec16 keys[2][Shape::kChunks];
-  vec16 values[2][Shape::kChunks];
-  BlockScales scales[2];
+  static constexpr int kBlocks = Shape::kFewStepBlocks;
+  vec16 keys[kBlocks][Shape::kChunks];
+  vec16 values[kBlocks][Shape::kChunks];
+  float key_scales[kBlocks];
+  float value_scales[kBlocks];
 
   __device__ __forceinline__ mfma_in8 key(int kf, int ks) const {
     const vec16& c = keys[kf][ks >> 1];
     const int w = 2 * (ks & 1);
-    return widen(c.w[w], scales[kf].key, c.w[w + 1], scales[kf].key);
+    return widen(c.w[w], key_scales[kf], c.w[w + 1], key_scales[kf]);
   }
-  __device__ __forceinline__ mfma_in8 value(int, int df) const {
-    return widen(values[0][df >> 2].w[df & 3], scales[0].value, values[1][df >> 2].w[df & 3], scales[1].value);
+  __device__ __forceinline__ mfma_in8 value(int half, int df) const {
+    const int n = 2 * half;
+    return widen(values[n][df >> 2].w[df & 3], value_scales[n], values[n + 1][df >> 2].w[df & 3], value_scales[n + 1]);
   }
 };
 
@@ -188,128 +217,147 @@ struct RawTile {
 // are not unrolled.
 template <typename Shape>
 struct StashedValues {
+  static constexpr int kBlocks = Shape::kFewStepBlocks;
   uint32_t* words;
-  BlockScales scales[2];
+  float scales[kBlocks];
 
   __device__ __forceinline__ StashedValues(const RawTile<Shape>& tile, float* lds)
-      : words(reinterpret_cast<uint32_t*>(lds)), scales{tile.scales[0], tile.scales[1]} {
-    static_assert(Shape::kWaveOutputs >= 64 * 2 * Shape::kDFrags, "a wave's values fit");
+      : words(reinterpret_cast<uint32_t*>(lds)) {
+    static_assert(Shape::kWaveOutputs >= 64 * kBlocks * Shape::kDFrags, "a wave's values fit");
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < kBlocks; ++n) {
+      scales[n] = tile.value_scales[n];
 #pragma unroll
       for (int df = 0; df < Shape::kDFrags; ++df) words[at(n, df)] = tile.values[n][df >> 2].w[df & 3];
     }
     lds_settled();
   }
   static __device__ __forceinline__ int at(int n, int df) { return (n * Shape::kDFrags + df) * 64 + lane_id(); }
-  __device__ __forceinline__ mfma_in8 value(int, int df) const {
-    return widen(words[at(0, df)], scales[0].value, words[at(1, df)], scales[1].value);
+  __device__ __forceinline__ mfma_in8 value(int half, int df) const {
+    return widen(words[at(2 * half, df)], scales[2 * half], words[at(2 * half + 1, df)], scales[2 * half + 1]);
   }
 };
 
 // At most 32 rows: the waves split the keys.
 template <typename Shape, int kTileRows>
-__device__ __forceinline__ void few_rows(Lds8<Shape>& lds, const Args& a, const TiledPlan& plan, const KvPiece& p) {
-  constexpr int kDepth = Shape::kDepth;
+__device__ __forceinline__ void few_rows(Lds8<Shape>& lds, const Args& a, const TiledPlan& plan, const KvPiece& p,
+                                         Pace& pace) {
   constexpr int kRF = Shape::kFewFrags;
+  constexpr int kBlocks = Shape::kFewStepBlocks;
+  constexpr int kKeys = kKv8Block * kBlocks;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int tiles = (p.key1 - p.key0 + 31) / 32;
+  const int tiles = (p.key1 - p.key0 + kKeys - 1) / kKeys;
   const int count = tiles > wave ? (tiles - wave - 1) / Shape::kWaves + 1 : 0;
   int bad = 0;
-  auto first_key = [&](int t) { return p.key0 + 32 * (wave + Shape::kWaves * t); };
+  auto first_key = [&](int t) { return p.key0 + kKeys * (wave + Shape::kWaves * t); };
+  const size_t scales_at = static_cast<size_t>(p.kv) * static_cast<size_t>(a.view.scale_head_stride);
+  const constant_floats key_scales = (constant_floats)(reinterpret_cast<uintptr_t>(a.view.key_scales + scales_at));
+  const constant_floats value_scales = (constant_floats)(reinterpret_cast<uintptr_t>(a.view.value_scales + scales_at));
   struct Places {
-    BlockPlace of[2];
+    BlockPlace of[kBlocks];
   };
   auto places_of = [&](int t) {
-    const int n = first_key(t) / kKv8Block;
-    return Places{{find_block(a, plan, p, n), find_block(a, plan, p, n + 1)}};
+    const int n0 = first_key(t) / kKv8Block;
+    Places places;
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) places.of[n] = find_block(a, plan, p, n0 + n);
+    return places;
+  };
+  // Bytes from the kv head's first to each block, and its values' scale.
+  struct ValuesAt {
+    size_t of[kBlocks];
+    float scales[kBlocks];
   };
   auto load_keys = [&](RawTile<Shape>& tile, const Places& places) {
+    ValuesAt at;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < kBlocks; ++n) {
       const int page = pool_page(a, places.of[n].page, bad);
-      const uint8_t* from = p.keys + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                            static_cast<size_t>(places.of[n].block * Shape::kBlockBytes);
+      const int block = places.of[n].block;
+      at.of[n] = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
+                 static_cast<size_t>(static_cast<uint32_t>(block * Shape::kBlockBytes));
 #pragma unroll
-      for (int h = 0; h < Shape::kChunks; ++h) tile.keys[n][h] = load_numbers<true>(from, key_chunk_at<Shape>(h));
-      tile.scales[n].key = load_scales(a, p, page, places.of[n].block).key;
+      for (int h = 0; h < Shape::kChunks; ++h) {
+        tile.keys[n][h] = load_numbers<true>(p.keys + at.of[n], key_chunk_at<Shape>(h));
+      }
+      const size_t scale = static_cast<size_t>(page) * static_cast<size_t>(a.view.scale_page_stride) +
+                           static_cast<size_t>(static_cast<uint32_t>(block));
+      tile.key_scales[n] = key_scales[scale];
+      at.scales[n] = value_scales[scale];
     }
+    return at;
   };
-  auto load_values = [&](RawTile<Shape>& tile, const Places& places) {
+  auto load_values = [&](RawTile<Shape>& tile, const ValuesAt& at) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int page = pool_page(a, places.of[n].page, bad);
-      const uint8_t* from = p.values + static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                            static_cast<size_t>(places.of[n].block * Shape::kBlockBytes);
+    for (int n = 0; n < kBlocks; ++n) {
+      tile.value_scales[n] = at.scales[n];
 #pragma unroll
-      for (int h = 0; h < Shape::kChunks; ++h) tile.values[n][h] = load_numbers<true>(from, value_chunk_at<Shape>(h));
-      tile.scales[n].value = load_scales(a, p, page, places.of[n].block).value;
+      for (int h = 0; h < Shape::kChunks; ++h) {
+        tile.values[n][h] = load_numbers<true>(p.values + at.of[n], value_chunk_at<Shape>(h));
+      }
     }
   };
 
   TiledRows<Shape, kRF> rows;
   rows.clear();
-  RawTile<Shape> raw[kDepth];
+  RawTile<Shape> tile;
   Places next{};
   if (count > 0) {
+    const Places places = places_of(0);
     load_rows(rows, a, plan, p, 0);
-#pragma unroll
-    for (int t = 0; t < kDepth; ++t) {
-      if (t < count) {
-        const Places places = places_of(t);
-        load_keys(raw[t], places);
-        load_values(raw[t], places);
-      }
-    }
-    next = places_of(min(kDepth, count - 1));
+    const ValuesAt at = load_keys(tile, places);
+    load_values(tile, at);
+    next = places_of(min(1, count - 1));
   }
+  hold_rows(rows);
   const int all_seen = min(p.seen_first, p.key1);
-  for (int t0 = 0; t0 < count; t0 += kDepth) {
+  for (int t = 0; t < count; ++t) {
+    const bool more = t + 1 < count;
+    const int key0 = first_key(t);
+    const bool whole = key0 + kKeys <= all_seen;
+    if constexpr (Shape::kPaced) pace.reached(p.done + (key0 - p.key0) / Shape::kFewStepKeys);
+    TileWork<Shape, kRF, kBlocks> work;
+    work.scores(rows, tile);
+    ValuesAt at{};
+    if (more) {
+      at = load_keys(tile, next);
+      next = places_of(min(t + 2, count - 1));
+    }
+    if (!whole) work.mask(rows, key0);
+    work.raise_base(rows, plan.scale_log2e);
 #pragma unroll
-    for (int u = 0; u < kDepth; ++u) {
-      const int t = t0 + u;
-      if (t >= count) break;
-      RawTile<Shape>& tile = raw[u];
-      const bool more = t + kDepth < count;
-      const Places places = next;
-      const int key0 = first_key(t);
-      const bool whole = key0 + 32 <= all_seen;
-      TileWork<Shape, kRF, 2> work;
-      work.scores(rows, tile);
-      if (more) {
-        load_keys(tile, places);
-        next = places_of(min(t + kDepth + 1, count - 1));
+    for (int half = 0; half < kBlocks / 2; ++half) work.weights(rows, plan.scale_log2e, half);
+    if (!whole) {
+      // numbers behind the last key that counts may be any
+      bool found = false;
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) {
+        const uint32_t keep = first_numbers(p.key1 - key0 - 16 * n - 4 * (lane_id() >> 4));
+#pragma unroll
+        for (int h = 0; h < Shape::kChunks; ++h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            tile.values[n][h].w[i] &= keep;
+            found |= nan_bytes(tile.values[n][h].w[i]) != 0;
+          }
+        }
       }
-      if (!whole) work.mask(rows, key0);
-      work.raise_base(rows, plan.scale_log2e);
-      work.weights(rows, plan.scale_log2e, 0);
-      bool special = false;
-      if (!whole) {
-        // numbers behind the last key that counts may be any
-        bool found = false;
+      if (__any(found)) {
+        const StashedValues<Shape> values(tile, lds.outputs + wave * Shape::kWaveOutputs);
+        work.mark_special(rows, values, key0);  // rows that see them get them at the end
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint32_t keep = first_numbers(p.key1 - key0 - 16 * n - 4 * (lane_id() >> 4));
+        for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
           for (int h = 0; h < Shape::kChunks; ++h) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              tile.values[n][h].w[i] &= keep;
-              found |= number_nan(tile.values[n][h].w[i]);
-            }
+            for (int i = 0; i < 4; ++i) tile.values[n][h].w[i] &= ~nan_bytes(tile.values[n][h].w[i]);
           }
         }
-        special = __any(found);
       }
-      if (special) {
-        const StashedValues<Shape> values(tile, lds.outputs + wave * Shape::kWaveOutputs);
-        work.mark_special(rows, values, key0);
-        work.products(rows, Cleared<StashedValues<Shape>>{values}, 0);
-      } else {
-        work.products(rows, tile, 0);
-      }
-      if (more) load_values(tile, places);
     }
+#pragma unroll
+    for (int half = 0; half < kBlocks / 2; ++half) work.products(rows, tile, half);
+    if (more) load_values(tile, at);
   }
   join_waves<Shape, kTileRows, Shape::kWaveOutputs>(rows, bad, lds.outputs, lds.stats, a, plan, p);
 }
@@ -327,21 +375,24 @@ struct OperandTile {
   __device__ __forceinline__ mfma_in8 value(int half, int df) const { return lds_operand(tile + value_at(half, df)); }
 };
 
-// The lower or upper half of a tile, as a tile.
+// A tile's NaN as values, 0 elsewhere, from the waves' marks.
 template <typename Shape>
-struct OperandHalf {
-  const OperandTile<Shape>& tile;
-  int half;
+struct MarkedValues {
+  const vec16* marks;
 
-  __device__ __forceinline__ mfma_in8 key(int kf, int ks) const { return tile.key(2 * half + kf, ks); }
-  __device__ __forceinline__ mfma_in8 value(int, int df) const { return tile.value(half, df); }
+  __device__ __forceinline__ mfma_in8 value(int half, int df) const {
+    auto words = [&](int block) {
+      return reinterpret_cast<const uint32_t*>(marks + (block * Shape::kChunks + (df >> 2)) * 64 + lane_id())[df & 3];
+    };
+    return widen(words(2 * half), 1.0f, words(2 * half + 1), 1.0f);
+  }
 };
 
 // Many rows: the waves split them, 32 each, and share the tiles. `tiles_done`:
 // of the block's pieces before, so that a tile's number is its own.
 template <typename Shape>
 __device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const TiledPlan& plan, const KvPiece& p,
-                                          int& tiles_done) {
+                                          Pace& pace, int& tiles_done) {
   constexpr int kRF = 2;
   static_assert(Shape::kWaves == 4 * Shape::kChunks, "a wave stages one chunk of one block of a tile");
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -373,14 +424,18 @@ __device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const
     const int key0 = p.key0 + 64 * t + 16 * my_block;
     if (p.key0 + 64 * t + 64 > p.seen_first) {
       // A tile that some row of the unit does not see whole. Numbers behind the
-      // last key that counts may be any.
+      // last key that counts may be any; NaN would reach, as 0 * NaN, rows that do
+      // not see them, and are left beside the tile for those that do.
       const uint32_t keep = first_numbers(p.key1 - key0 - 4 * (lane_id() >> 4));
+      vec16 marks;
       bool found = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        raw.values.w[i] &= keep;
-        found |= number_nan(raw.values.w[i]);
+        marks.w[i] = nan_bytes(raw.values.w[i] & keep);
+        raw.values.w[i] &= keep & ~marks.w[i];
+        found |= marks.w[i] != 0;
       }
+      lds.marks[t & 1][threadIdx.x] = marks;
       if (__any(found) && lane_id() == 0) lds.special[(tiles_done + t) & 1] = tiles_done + t;
     }
 #pragma unroll
@@ -416,10 +471,12 @@ __device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const
     stage(0, raw);
     if (tiles > 1) raw = load(second);
   }
+  hold_rows(rows);
   for (int t = 0; t < tiles; ++t) {
     // Behind the barrier tile t is staged, and the tile before has been read.
     lds_settled();
     plain_barrier();
+    if constexpr (Shape::kPaced) pace.reached(p.done + t);
     if (t + 1 < tiles) {
       stage(t + 1, raw);
       if (t + 2 < tiles) {
@@ -436,24 +493,11 @@ __device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const
     work.scores(rows, tile);
     if (!whole) work.mask(rows, tile0);
     work.raise_base(rows, plan.scale_log2e);
-    if (!special) {
-      work.weights(rows, plan.scale_log2e, 0);
-      work.products(rows, tile, 0);
-      work.weights(rows, plan.scale_log2e, 1);
-      work.products(rows, tile, 1);
-      continue;
-    }
-    // Half a tile at a time, its scores once more: registers for the marks.
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      const OperandHalf<Shape> part{tile, half};
-      TileWork<Shape, kRF, 2> again;
-      again.scores(rows, part);
-      if (!whole) again.mask(rows, tile0 + 32 * half);
-      again.weights(rows, plan.scale_log2e, 0);
-      again.mark_special(rows, part, tile0 + 32 * half);
-      again.products(rows, Cleared<OperandHalf<Shape>>{part}, 0);
-    }
+    if (special) work.mark_special(rows, MarkedValues<Shape>{lds.marks[t & 1]}, tile0);
+    work.weights(rows, plan.scale_log2e, 0);
+    work.products(rows, tile, 0);
+    work.weights(rows, plan.scale_log2e, 1);
+    work.products(rows, tile, 1);
   }
   tiles_done += max(tiles, 0);
   if (__any(bad != 0) && lane_id() == 0) lds.bad = 1;
@@ -483,11 +527,12 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kSimdWaves) void batch_atte
   // seen by every wave behind the barriers of the search for the share
   if (threadIdx.x == 0) lds.special[0] = lds.special[1] = -1;
   int tiles_done = 0;
+  Pace pace;
   walk_share<Shape, kMany, uint8_t>(
-      a, plan, lds.sums, &lds.found,
-      [&](const KvPiece& p) { few_rows<Shape, kTileRows>(lds, a, plan, p); },
+      a, plan, lds.sums, &lds.found, [&](int steps) { if (Shape::kPaced && plan.split) pace.begin(steps); },
+      [&](const KvPiece& p) { few_rows<Shape, kTileRows>(lds, a, plan, p, pace); },
       [&](const KvPiece& p) {
-        if constexpr (kMany) many_rows<Shape>(lds, a, plan, p, tiles_done);
+        if constexpr (kMany) many_rows<Shape>(lds, a, plan, p, pace, tiles_done);
       });
 }
 
@@ -606,10 +651,10 @@ void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStr
   const unsigned blocks = static_cast<unsigned>(plan.shares) * static_cast<unsigned>(a.view.num_kv_heads);
   batch_attention_kv8_kernel<Shape><<<blocks, Shape::kThreads, 0, s>>>(a, plan);
   if (!plan.split) return;
-  // A row is a chain of loads, so few follow each other: one time round for
-  // many rows, two for few.
+  // A row is a chain of loads, so none follows another.
   constexpr bool kRowEach = kMaxRows == 0;
-  const dim3 join(blocks, kRowEach ? kTileRows / (4 * 256 / kHeadDim) : kTileRows / 8);
+  const int few_rows = static_cast<int>(std::min<long long>(static_cast<long long>(a.max_new) * a.group, kFewRows));
+  const dim3 join(blocks, kRowEach ? kTileRows / (4 * 256 / kHeadDim) : (few_rows + 3) / 4);
   batch_attention_join_kernel<kHeadDim, kRowEach, Args><<<join, kJoinThreads, 0, s>>>(a, plan, kTileRows);
 }
 
