@@ -192,13 +192,14 @@ size_t lcr_batch_verify_workspace_bytes(int batch, int rows, int vocab);
  *   top_ids[t][top], top_logprobs[t][top]
  *                    the ids of the largest logits in descending order, equal ones
  *                    by ascending id, and their log p; top is at most
- *                    LCR_BATCH_MAX_ALTERNATIVES. Behind a vocabulary smaller than
- *                    top, -1 and -inf.
+ *                    LCR_BATCH_MAX_ALTERNATIVES. Logits of -inf are no alternatives:
+ *                    where fewer than top others are left, -1 and -inf behind them.
  * A row whose token id is negative is left out: nothing of it is read or written.
  * token_ids NULL: no tokens are given, logprobs and ranks are not written, and no
  * row is left out. logprobs, ranks and entropies may each be NULL for what is not
  * wanted, and with top 0 the last two.
- * Sums and logarithms are fp32 over parts of 4096 logits and fp64 over those.
+ * Weights are fp32, summed in fp32 sixteen at a time and in fp64 beyond that; the
+ * logarithm is fp64.
  * A NaN logit counts as -inf, whose p is 0. Where a row's largest logit is not
  * finite, p is 1 at the lowest index of that value, as for lcr_batch_verify.
  * With a workspace of lcr_batch_logprobs_workspace_bytes (16-byte aligned) few rows

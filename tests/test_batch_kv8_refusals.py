@@ -125,7 +125,8 @@ def logprobs_call(lib, **changed):
 @pytest.mark.parametrize("changed,text", [
     (dict(rows=-1), "non-negative sizes"), (dict(top=-1), "non-negative sizes"),
     (dict(top=33), "up to 32 alternatives, got 33"), (dict(vocab=0), "a vocabulary, got 0"),
-    (dict(vocab=-5), "a vocabulary"), (dict(logits_stride=999), "cannot lie 999 apart"),
+    (dict(vocab=-5), "a vocabulary"), (dict(vocab=(1 << 30) + 1, logits_stride=2 ** 31 - 1), "up to 2^30 ids"),
+    (dict(logits=6 * A + 2), "4-byte boundaries"), (dict(logits_stride=999), "cannot lie 999 apart"),
     (dict(logits=None), "needs logits"), (dict(top_ids=None), "room for its alternatives"),
     (dict(top_logprobs=None), "room for its alternatives"), (dict(token_ids=None), "needs the tokens"),
     (dict(token_ids=None, logprobs=None), "needs the tokens"), (dict(workspace_bytes=16), "has no pointer"),

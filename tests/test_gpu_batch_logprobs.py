@@ -2,7 +2,8 @@
 
 Allowed, with e = 2^-24 and d = l - max: a weight exp(d) takes its argument from two
 fp32 roundings and a rounded constant, and the exponential's own two: 4 e |d| + 4 e
-of its size. Up to 64 of them are added in fp32 before wider sums: 64 e. So the sum
+of its size. Up to 64 factors and terms of such an error lead to a sum (16 are added
+in fp32, and a lane's largest rises a few times): 64 e. So the sum
 S is off by S_rel = e (4 E|d| + 68) of its size, and log S by as much; a log
 probability by that, d's rounding and its own. The entropy log S - E d: by S_rel,
 by the weights' errors in the weighted sum, sum p |d| (4 e |d| + 5 e) + 64 e E|d|, and
@@ -42,7 +43,7 @@ def definition(row, token, top):
         entropy, allow_lp, allow_entropy = 0.0, np.zeros(vocab), 0.0
     ids = np.full(top, -1, np.int64)
     tops = np.full(top, -np.inf)
-    n = min(top, vocab)
+    n = min(top, int((x > -np.inf).sum()))
     ids[:n], tops[:n] = order[:n], lp[order[:n]]
     inside = 0 <= token < vocab
     return dict(logprob=lp[token] if inside else -np.inf, rank=int((x > x[token]).sum()) if inside else vocab,
@@ -206,6 +207,7 @@ def test_masked_and_special(lcr, gpu, vocab):
     x[11] = np.where(np.arange(vocab) % 2, low, -low)
     x[12, 0], x[12, vocab - 1] = np.inf, np.nan
     x[13, 1:] = -np.inf
+    x[5].view(np.uint32)[np.isnan(x[5])] = 0x7F800001  # signalling
     for top in (0, 1, 8, 32):
         both(lcr, x, r.integers(0, vocab, 14), top)
         both(lcr, x, [0] * 14, top)
