@@ -7,9 +7,9 @@
 //   log p = l - m - log s,  entropy = log s - t / s.
 // Sixteen logits at a time are summed in fp32, and those sums in fp64.
 //
-// The likeliest ids need no second order of all logits: the k-th largest of the
-// lanes' largest logits is one that at least k logits reach, and few others do. The
-// lanes that hold one read theirs again, and those at least as large (about k) are
+// The likeliest ids need no order of all logits: the k-th largest of the lanes'
+// largest logits is one that at least k logits reach, and few others do. What the
+// lanes that hold one had is read again, and logits at least as large (about k) are
 // ranked by counting. The streaming pass does nothing for it but keep the largest.
 //
 // Bound by memory: 11 operations a logit, the exponential four times as long as the
@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../../include/lcr_batch.h"
 #include "../capi_util.h"
@@ -25,8 +26,12 @@
 namespace lcr {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
+// Threads of a block. A row of few tiles has little for many waves, and its choice of
+// likeliest ids, a chain of short steps, wants more blocks beside it: 4000 rows of
+// 8000 logits 46 us by blocks of 512 threads, 33 by 256; 256 rows of 128256 28 and 33.
+constexpr int kManyThreads = 512;
+constexpr int kFewThreads = 256;
+constexpr int kFewThreadTiles = 16;
 constexpr int kTile = 1024;            // logits of a wave's step: four times four a lane
 constexpr int kMostCandidates = 1024;
 constexpr int kMostTop = LCR_BATCH_MAX_ALTERNATIVES;
@@ -39,7 +44,6 @@ struct alignas(16) PartSums {
   float max;
   int above;   // logits larger than the given token's
   int hot;     // the lowest index of the largest logit, where it is not finite
-  int count;   // of its likeliest ids
 };
 
 struct LogprobArgs {
@@ -54,8 +58,8 @@ struct LogprobArgs {
   int vocab;
   int logits_stride;
   int parts;
-  PartSums* sums;            // [rows][parts]
-  unsigned long long* keys;  // [rows][parts][top]
+  PartSums* sums;   // [rows][parts]
+  float* largest;   // [rows][parts][kManyThreads]: of each thread's logits
 };
 
 __device__ __forceinline__ float infinity() { return __builtin_huge_valf(); }
@@ -106,14 +110,24 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   return v + xor_lane_f64<1>(v);
 }
 
-// A part of a row. Loads are 16-byte aligned, so that index i of the row is place
-// i + shift of them; places outside the row hold -inf.
-struct RowPart {
+// A row in tiles of kTile places, cut into parts. Loads are 16-byte aligned, so that
+// index i of the row is place i + shift of them; places outside the row hold -inf.
+struct RowTiles {
   const float* row;
   int shift;   // 0 .. 3
   int places;  // shift + vocab
-  int tile0;   // [tile0, tile1) of kTile places
-  int tile1;
+  int tiles;
+  int parts;
+
+  __device__ __forceinline__ RowTiles(const LogprobArgs& a, int r)
+      : row(a.logits + static_cast<size_t>(r) * static_cast<size_t>(a.logits_stride)),
+        shift(static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 2 & 3u)),
+        places(shift + a.vocab),
+        tiles((places + kTile - 1) / kTile),
+        parts(a.parts) {}
+
+  // The first tile of a part (tiles are at most 2^20 + 1, parts 32).
+  __device__ __forceinline__ int first_tile(int part) const { return tiles * part / parts; }
 
   // Places 4 g .. 4 g + 3.
   __device__ __forceinline__ float4 load(int g) const {
@@ -130,7 +144,7 @@ struct RowPart {
 struct Tile {
   float l[16];
 
-  __device__ __forceinline__ void load(const RowPart& p, int tile) {
+  __device__ __forceinline__ void load(const RowTiles& p, int tile) {
     const int g = tile * (kTile / 4) + lane_id();
     // whole tiles without a test of each load
     const bool whole = 1024 * tile >= p.shift && 1024 * tile + 1023 < p.places;
@@ -158,16 +172,40 @@ struct Tile {
   }
 };
 
-struct Lds {
+constexpr int kMostParts = 32;
+
+constexpr int kMostSlots = 16;
+constexpr int kMostReads = 1024;
+
+// What the choice of likeliest ids needs.
+template <int kThreads>
+struct ChoiceLds {
+  static constexpr int kWaves = kThreads / 64;
   float lists[kWaves][64];
   unsigned long long candidates[kMostCandidates];
+  uint16_t reads[kMostReads];   // what is read again, as the Source names it
+  int found[kWaves];
+  int read_count;
+  int count;   // of candidates
+  float reach;
+};
+
+template <int kWaves>
+struct SumsLds {
   double sums[kWaves][2];
   float max[kWaves];
   int above[kWaves];
   int hot[kWaves];
-  int count;
-  float reach;
 };
+
+// A place in a list for each lane that `wants` one: one count a wave, not a lane.
+__device__ __forceinline__ int take_place(int* count, bool wants) {
+  const unsigned long long mask = __ballot(wants);
+  if (mask == 0) return 0;
+  int base = 0;
+  if (lane_id() == 0) base = atomicAdd(count, __popcll(mask));
+  return __builtin_amdgcn_readfirstlane(base) + __popcll(mask & ((1ull << lane_id()) - 1));
+}
 
 // A compare and exchange over lanes kMask apart: the larger to the lower lane where
 // `down`.
@@ -210,7 +248,9 @@ __device__ __forceinline__ float sort_wave(float v) {
 }
 
 // The top-th largest of the block's 64 kWaves values, for all of it.
-__device__ __forceinline__ float largest_reached(Lds& lds, float v, int top) {
+template <int kThreads>
+__device__ __forceinline__ float largest_reached(ChoiceLds<kThreads>& lds, float v, int top) {
+  constexpr int kWaves = kThreads / 64;
   const int wave = static_cast<int>(threadIdx.x) >> 6;
   v = sort_wave(v);
 #pragma unroll
@@ -225,33 +265,105 @@ __device__ __forceinline__ float largest_reached(Lds& lds, float v, int top) {
   return lds.reach;
 }
 
-// The part's logits at or above (kAbove: above) `reach` as candidates, by the lanes
-// whose largest reaches it; -inf is none.
-template <bool kAbove>
-__device__ __forceinline__ int gather(Lds& lds, const RowPart& p, float reach, float lane_max) {
-  if (threadIdx.x == 0) lds.count = 0;
-  __syncthreads();
+// Upper bits of a value's place in the order of values.
+__device__ __forceinline__ uint32_t order16(float l) { return static_cast<uint32_t>(key_of(l, 0) >> 48); }
+
+// Where a thread's logits of a whole row were: its tiles in up to kMostSlots groups,
+// with the upper bits of each group's largest.
+template <int kThreads>
+struct RowSource {
+  static constexpr int kWaves = kThreads / 64;
+  uint16_t (*most)[kThreads];
+  float largest;
+  int steps;   // a wave's tiles, at most
+  int group;   // steps of a slot
+
+  // Names to `take` what may hold logits that `counts` (at or above reach) takes.
+  template <typename Counts, typename Take>
+  __device__ __forceinline__ void find(float reach, const Counts& counts, const Take& take) const {
+    const bool mine = counts(largest);
+    if (!__any(mine)) return;
+    const uint32_t least = max(order16(reach), order16(-infinity()) + 1);
+    for (int slot = 0; slot * group < steps; ++slot) {
+      take(mine && most[slot][threadIdx.x] >= least, static_cast<int>(threadIdx.x) * kMostSlots + slot);
+    }
+  }
+  // Fours of logits behind a name, and the place of one, or -1.
+  __device__ __forceinline__ int fours() const { return 4 * group; }
+  __device__ __forceinline__ int four_at(const RowTiles& p, int name, int four) const {
+    const int thread = name / kMostSlots;
+    const int tile = (thread >> 6) + kWaves * (name % kMostSlots * group + (four >> 2));
+    return tile < p.tiles ? tile * (kTile / 4) + 64 * (four & 3) + (thread & 63) : -1;
+  }
+};
+
+// Of a row in parts: a thread's largest of each.
+template <int kThreads>
+struct PartsSource {
+  static constexpr int kWaves = kThreads / 64;
+  const float (&largest)[kMostParts];
+  int parts;
+  int steps;
+
+  template <typename Counts, typename Take>
+  __device__ __forceinline__ void find(float, const Counts& counts, const Take& take) const {
+#pragma unroll
+    for (int part = 0; part < kMostParts; ++part) {
+      if (part < parts) take(counts(largest[part]), part * kThreads + static_cast<int>(threadIdx.x));
+    }
+  }
+  __device__ __forceinline__ int fours() const { return 4 * steps; }
+  __device__ __forceinline__ int four_at(const RowTiles& p, int name, int four) const {
+    const int part = name / kThreads, thread = name % kThreads;
+    const int tile = p.first_tile(part) + (thread >> 6) + kWaves * (four >> 2);
+    return tile < p.first_tile(part + 1) ? tile * (kTile / 4) + 64 * (four & 3) + (thread & 63) : -1;
+  }
+};
+
+// The row's logits at or above (kAbove: above) `reach` as candidates; -inf is none.
+// What the lanes that reach it had is read again, four logits at a time, by the whole
+// block. 256 rows of 128256, 20 ids: with those lanes reading theirs, one step behind
+// the other, 60 us; all that they had by the block 30; the tiles that reach it 26; no
+// ids at all 22.
+template <bool kAbove, int kThreads, typename Source>
+__device__ __forceinline__ int gather(ChoiceLds<kThreads>& lds, const RowTiles& p, float reach, const Source& source) {
   auto counts = [&](float l) { return (kAbove ? l > reach : l >= reach) && l > -infinity(); };
-  const bool mine = counts(lane_max);
-  if (__any(mine)) {
-    const int wave = static_cast<int>(threadIdx.x) >> 6;
-    for (int tile = p.tile0 + wave; tile < p.tile1; tile += kWaves) {
-      if (!mine) continue;
-      const int g = tile * (kTile / 4) + lane_id();
-      float4 v[4];
+  if (threadIdx.x == 0) lds.count = lds.read_count = 0;
+  __syncthreads();
+  source.find(reach, counts, [&](bool wanted, int name) {
+    const int at = take_place(&lds.read_count, wanted);
+    if (wanted && at < kMostReads) lds.reads[at] = static_cast<uint16_t>(name);
+  });
+  __syncthreads();
+  if (lds.read_count > kMostReads) {
+    __syncthreads();  // it may be counted in again
+    return kMostCandidates + 1;
+  }
+  const uint32_t fours = static_cast<uint32_t>(source.fours());
+  const uint32_t items = static_cast<uint32_t>(lds.read_count) * fours;  // under 2^30
+  constexpr int kAtOnce = 2;
+  for (uint32_t first = 0; first < items; first += kAtOnce * kThreads) {
+    float4 v[kAtOnce];
+    int g[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = p.load(g + 64 * j);
+    for (int n = 0; n < kAtOnce; ++n) {
+      const uint32_t item = first + n * kThreads + threadIdx.x;
+      const uint32_t read = item < items ? item / fours : 0;
+      g[n] = item < items ? source.four_at(p, lds.reads[read], static_cast<int>(item - read * fours)) : -1;
+      v[n] = g[n] >= 0 ? p.load(g[n]) : make_float4(-infinity(), -infinity(), -infinity(), -infinity());
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float l[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+    for (int n = 0; n < kAtOnce; ++n) {
+      const float l[4] = {v[n].x, v[n].y, v[n].z, v[n].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!counts(l[i])) continue;
-          const int at = atomicAdd(&lds.count, 1);
-          if (at < kMostCandidates) lds.candidates[at] = key_of(l[i], 4 * (g + 64 * j) + i - p.shift);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const bool wanted = counts(l[i]);
+        const int at = take_place(&lds.count, wanted);
+        if (wanted && at < kMostCandidates) lds.candidates[at] = key_of(l[i], 4 * g[n] + i - p.shift);
       }
     }
+    // more than there is room for: counted no further
+    if (lds.count > kMostCandidates) break;
   }
   __syncthreads();
   const int n = lds.count;
@@ -259,21 +371,24 @@ __device__ __forceinline__ int gather(Lds& lds, const RowPart& p, float reach, f
   return n;
 }
 
-// Adds the first `want` of the part's logits that equal `reach`, in the order of
+// Adds the first `want` of the row's logits that equal `reach`, in the order of
 // their ids, behind `have` candidates.
-__device__ __forceinline__ void gather_equal(Lds& lds, const RowPart& p, float reach, int have, int want) {
+template <int kThreads>
+__device__ __forceinline__ void gather_equal(ChoiceLds<kThreads>& lds, const RowTiles& p, float reach, int have,
+                                             int want) {
+  constexpr int kWaves = kThreads / 64;
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int end = min(p.tile1 * kTile, p.places);
-  for (int base = p.tile0 * kTile; base < end && want > 0; base += kThreads) {
-    const int i = base + static_cast<int>(threadIdx.x) - p.shift;
-    const bool equal = i >= 0 && i + p.shift < end && p.row[i] == reach;
+  const int vocab = p.places - p.shift;
+  for (int base = 0; base < vocab && want > 0; base += kThreads) {
+    const int i = base + static_cast<int>(threadIdx.x);
+    const bool equal = i < vocab && p.row[i] == reach;
     const unsigned long long mask = __ballot(equal);
-    if (lane_id() == 0) lds.above[wave] = __popcll(mask);
+    if (lane_id() == 0) lds.found[wave] = __popcll(mask);
     __syncthreads();
     int before = 0, all = 0;
     for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) before += lds.above[w];
-      all += lds.above[w];
+      if (w < wave) before += lds.found[w];
+      all += lds.found[w];
     }
     before += __popcll(mask & ((1ull << lane_id()) - 1));
     if (equal && before < want) lds.candidates[have + before] = key_of(reach, i);
@@ -283,19 +398,20 @@ __device__ __forceinline__ void gather_equal(Lds& lds, const RowPart& p, float r
   }
 }
 
-// The part's `top` largest, one pass over it for each: for parts with too many
+// The row's `top` largest, one pass over it for each: for rows with too many
 // candidates, whose large logits all lie with few lanes.
-__device__ __forceinline__ int gather_slowly(Lds& lds, const RowPart& p, int top) {
+template <int kThreads>
+__device__ __forceinline__ int gather_slowly(ChoiceLds<kThreads>& lds, const RowTiles& p, int top) {
+  constexpr int kWaves = kThreads / 64;
   const int wave = static_cast<int>(threadIdx.x) >> 6;
-  const int end = min(p.tile1 * kTile, p.places);
+  const int vocab = p.places - p.shift;
   unsigned long long last = ~0ull;
   for (int k = 0; k < top; ++k) {
     unsigned long long best = 0;
-    for (int at = p.tile0 * kTile + static_cast<int>(threadIdx.x); at < end; at += kThreads) {
-      if (at < p.shift) continue;
-      const float l = p.row[at - p.shift];
+    for (int i = threadIdx.x; i < vocab; i += kThreads) {
+      const float l = p.row[i];
       if (!(l > -infinity())) continue;
-      const unsigned long long key = key_of(l, at - p.shift);
+      const unsigned long long key = key_of(l, i);
       if (key < last && key > best) best = key;
     }
 #pragma unroll
@@ -322,7 +438,7 @@ __device__ __forceinline__ int gather_slowly(Lds& lds, const RowPart& p, int top
 }
 
 // Hands (rank, key) of the `top` first of n candidates to `out`.
-template <typename Out>
+template <int kThreads, typename Out>
 __device__ __forceinline__ void rank(const unsigned long long* candidates, int n, int top, const Out& out) {
   for (int c = threadIdx.x; c < n; c += kThreads) {
     const unsigned long long key = candidates[c];
@@ -367,33 +483,67 @@ __device__ __forceinline__ void write_top(const LogprobArgs& a, int row, int pla
   a.top_logprobs[at] = logprob;
 }
 
+// A row's likeliest ids.
+template <int kThreads, typename Source>
+__device__ __forceinline__ void choose(ChoiceLds<kThreads>& lds, const LogprobArgs& a, const RowTiles& p, int row,
+                                       float thread_largest, const Source& source, const RowResult& result) {
+  const float reach = largest_reached(lds, thread_largest, a.top);
+  int n = gather<false>(lds, p, reach, source);
+  if (n > kMostCandidates) {
+    // Many equal ones (a mask of the type's lowest value), or many in few lanes.
+    n = gather<true>(lds, p, reach, source);
+    if (n <= kMostCandidates - kMostTop) {
+      const int want = max(a.top - n, 0);
+      gather_equal(lds, p, reach, n, want);
+      n += want;
+    } else {
+      n = gather_slowly(lds, p, a.top);
+    }
+  }
+  rank<kThreads>(lds.candidates, n, a.top, [&](int place, unsigned long long key) {
+    write_top(a, row, place, result.logprob(value_of(key), id_of(key)), id_of(key));
+  });
+  for (int place = min(n, a.top) + static_cast<int>(threadIdx.x); place < a.top; place += kThreads) {
+    write_top(a, row, place, -infinity(), -1);
+  }
+}
+
+struct Nothing {};
+
 // A row (kPart: a part of one) a block.
-template <bool kTop, bool kPart>
+template <bool kTop, bool kPart, int kThreads>
 __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
-  __shared__ Lds lds;
+  constexpr int kWaves = kThreads / 64;
+  __shared__ SumsLds<kWaves> lds;
+  __shared__ std::conditional_t<kTop && !kPart, ChoiceLds<kThreads>, Nothing> choice;
+  __shared__ std::conditional_t<kTop && !kPart, uint16_t[kMostSlots][kThreads], Nothing> slot_most;
   const int row = kPart ? blockIdx.y : blockIdx.x;
   const int part = kPart ? blockIdx.x : 0;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int token = a.token_ids != nullptr ? a.token_ids[row] : -1;
   if (a.token_ids != nullptr && token < 0) return;  // the row is left out
-  RowPart p;
-  p.row = a.logits + static_cast<size_t>(row) * static_cast<size_t>(a.logits_stride);
-  p.shift = static_cast<int>(reinterpret_cast<uintptr_t>(p.row) >> 2 & 3u);
-  p.places = p.shift + a.vocab;
-  const int tiles = (p.places + kTile - 1) / kTile;
-  p.tile0 = kPart ? static_cast<int>(static_cast<long long>(tiles) * part / a.parts) : 0;
-  p.tile1 = kPart ? static_cast<int>(static_cast<long long>(tiles) * (part + 1) / a.parts) : tiles;
+  const RowTiles p(a, row);
+  const int tile0 = kPart ? p.first_tile(part) : 0;
+  const int tile1 = kPart ? p.first_tile(part + 1) : p.tiles;
 
   Tile next;
-  int tile = p.tile0 + wave;
-  if (tile < p.tile1) next.load(p, tile);
+  int tile = tile0 + wave;
+  if (tile < tile1) next.load(p, tile);
   const float given = token >= 0 && token < a.vocab ? clean(p.row[token]) : infinity();
   float largest = -infinity();
   double sum = 0.0, weighted = 0.0;
   int above = 0;
-  for (; tile < p.tile1; tile += kWaves) {
+  const int steps = (p.tiles + kWaves - 1) / kWaves;  // of a whole row
+  const int group = (steps + kMostSlots - 1) / kMostSlots;
+  float group_most = -infinity();
+  int slot = 0, in_group = 0;
+  if constexpr (kTop && !kPart) {
+#pragma unroll
+    for (int n = 0; n < kMostSlots; ++n) slot_most[n][threadIdx.x] = 0;
+  }
+  for (; tile < tile1; tile += kWaves) {
     Tile now = next;
-    if (tile + kWaves < p.tile1) next.load(p, tile + kWaves);
+    if (tile + kWaves < tile1) next.load(p, tile + kWaves);
     float most = max3(now.l[0], now.l[1], now.l[2]);
 #pragma unroll
     for (int i = 3; i < 15; i += 2) most = max3(most, now.l[i], now.l[i + 1]);
@@ -411,6 +561,14 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) above += __popcll(__ballot(now.l[i] > given));
     }
+    if constexpr (kTop && !kPart) {
+      group_most = in_group == 0 ? most : fmaxf(group_most, most);
+      slot_most[slot][threadIdx.x] = static_cast<uint16_t>(order16(group_most));
+      if (++in_group == group) {
+        in_group = 0;
+        ++slot;
+      }
+    }
     const float raised = fmaxf(largest, most);
     const float fall = below(largest, raised);
     const double keep = weight(fall);
@@ -426,6 +584,9 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
     sum = __builtin_fma(sum, keep, static_cast<double>(s[0] + s[1]));
     largest = raised;
   }
+  if constexpr (kTop && kPart) {
+    a.largest[(static_cast<size_t>(row) * a.parts + part) * kThreads + threadIdx.x] = largest;
+  }
 
   // The lanes' sums against the block's largest logit, in a fixed order.
   const float wave_most = wave_max(largest);
@@ -440,7 +601,7 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
   sum = wave_sum_f64(sum * keep);
   int hot = INT_MAX;
   if (!finite(most)) {
-    for (int i = p.tile0 * kTile + static_cast<int>(threadIdx.x); i < min(p.tile1 * kTile, p.places); i += kThreads) {
+    for (int i = tile0 * kTile + static_cast<int>(threadIdx.x); i < min(tile1 * kTile, p.places); i += kThreads) {
       if (i >= p.shift && clean(p.row[i - p.shift]) == most) {
         hot = i - p.shift;
         break;
@@ -456,7 +617,7 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
     lds.hot[wave] = hot;
   }
   __syncthreads();
-  PartSums all{0.0, 0.0, most, 0, INT_MAX, 0};
+  PartSums all{0.0, 0.0, most, 0, INT_MAX};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     all.sum += lds.sums[w][0];
@@ -464,63 +625,38 @@ __global__ __launch_bounds__(kThreads, 4) void logprobs_kernel(LogprobArgs a) {
     all.above += lds.above[w];
     all.hot = min(all.hot, lds.hot[w]);
   }
-  const RowResult result = kPart ? RowResult{} : result_of(all);
-  if constexpr (!kPart) {
+  if constexpr (kPart) {
+    if (threadIdx.x == 0) a.sums[static_cast<size_t>(row) * a.parts + part] = all;
+  } else {
+    const RowResult result = result_of(all);
     if (threadIdx.x == 0) write_row(a, row, token, given, all, result);
+    if constexpr (kTop) choose(choice, a, p, row, largest, RowSource<kThreads>{slot_most, largest, steps, group}, result);
   }
-  PartSums* sums = kPart ? a.sums + static_cast<size_t>(row) * a.parts + part : nullptr;
-  if constexpr (kTop) {
-    const float reach = largest_reached(lds, largest, a.top);
-    int n = gather<false>(lds, p, reach, largest);
-    if (n > kMostCandidates) {
-      // Many equal ones (a mask of the type's lowest value), or many in few lanes.
-      n = gather<true>(lds, p, reach, largest);
-      if (n <= kMostCandidates - kMostTop) {
-        const int want = max(a.top - n, 0);
-        gather_equal(lds, p, reach, n, want);
-        n += want;
-      } else {
-        n = gather_slowly(lds, p, a.top);
-      }
-    }
-    const int top = min(n, a.top);
-    if constexpr (kPart) {
-      unsigned long long* keys = a.keys + (static_cast<size_t>(row) * a.parts + part) * a.top;
-      rank(lds.candidates, n, a.top, [&](int place, unsigned long long key) { keys[place] = key; });
-      all.count = top;
-    } else {
-      rank(lds.candidates, n, a.top, [&](int place, unsigned long long key) {
-        write_top(a, row, place, result.logprob(value_of(key), id_of(key)), id_of(key));
-      });
-      for (int place = top + static_cast<int>(threadIdx.x); place < a.top; place += kThreads) {
-        write_top(a, row, place, -infinity(), -1);
-      }
-    }
-  }
-  if (kPart && threadIdx.x == 0) *sums = all;
 }
-
-constexpr int kMostParts = 32;
 
 // Joins the parts of a row, a block each.
 template <bool kTop>
-__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) {
-  __shared__ unsigned long long keys[kMostParts * kMostTop];
-  __shared__ unsigned long long candidates[kMostParts * kMostTop];
-  __shared__ int lds_count;
+__global__ __launch_bounds__(kManyThreads) void logprobs_join_kernel(LogprobArgs a) {
+  constexpr int kThreads = kManyThreads;
+  constexpr int kWaves = kThreads / 64;
+  __shared__ std::conditional_t<kTop, ChoiceLds<kThreads>, Nothing> choice;
   const int row = blockIdx.x;
   const int token = a.token_ids != nullptr ? a.token_ids[row] : -1;
   if (a.token_ids != nullptr && token < 0) return;
-  const float* logits = a.logits + static_cast<size_t>(row) * static_cast<size_t>(a.logits_stride);
-  const float given = token >= 0 && token < a.vocab ? clean(logits[token]) : infinity();
+  const RowTiles p(a, row);
   const int lane = lane_id();
   // Every wave joins the sums for itself, a part a lane.
-  PartSums mine{0.0, 0.0, -infinity(), 0, INT_MAX, 0};
+  PartSums mine{0.0, 0.0, -infinity(), 0, INT_MAX};
   if (lane < a.parts) mine = a.sums[static_cast<size_t>(row) * a.parts + lane];
+  const float given = token >= 0 && token < a.vocab ? clean(p.row[token]) : infinity();
+  float each[kMostParts];
+  float largest = -infinity();
   if constexpr (kTop) {
-    const unsigned long long* from = a.keys + static_cast<size_t>(row) * a.parts * a.top;
-    for (int i = threadIdx.x; i < a.parts * a.top; i += kThreads) keys[i] = from[i];
-    if (threadIdx.x == 0) lds_count = 0;
+    const float* from = a.largest + static_cast<size_t>(row) * a.parts * kThreads + threadIdx.x;
+#pragma unroll
+    for (int part = 0; part < kMostParts; ++part) each[part] = part < a.parts ? from[part * kThreads] : -infinity();
+#pragma unroll
+    for (int part = 0; part < kMostParts; ++part) largest = fmaxf(largest, each[part]);
   }
   PartSums all;
   all.max = wave_max(mine.max);
@@ -538,45 +674,43 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobArgs a) 
   const RowResult result = result_of(all);
   if (threadIdx.x == 0) write_row(a, row, token, given, all, result);
   if constexpr (kTop) {
-    __syncthreads();
-    // What some part has as many of is a bound for the others.
-    unsigned long long reach = lane < a.parts && mine.count == a.top ? keys[lane * a.top + a.top - 1] : 0;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned long long other = __shfl_xor(reach, o, 64);
-      reach = other > reach ? other : reach;
-    }
-    for (int base = 0; base < a.parts * a.top; base += kThreads) {
-      const int i = base + static_cast<int>(threadIdx.x);
-      const int part = min(i / a.top, a.parts - 1);
-      const int count = __shfl(mine.count, part, 64);
-      if (i < a.parts * a.top && i - part * a.top < count && keys[i] >= reach) {
-        candidates[atomicAdd(&lds_count, 1)] = keys[i];
-      }
-    }
-    __syncthreads();
-    const int n = lds_count;
-    rank(candidates, n, a.top, [&](int place, unsigned long long key) {
-      write_top(a, row, place, result.logprob(value_of(key), id_of(key)), id_of(key));
-    });
-    for (int place = min(n, a.top) + static_cast<int>(threadIdx.x); place < a.top; place += kThreads) {
-      write_top(a, row, place, -infinity(), -1);
-    }
+    const int part_tiles = (p.tiles + p.parts - 1) / p.parts;  // at most
+    choose(choice, a, p, row, largest, PartsSource<kThreads>{each, p.parts, (part_tiles + kWaves - 1) / kWaves}, result);
   }
 }
 
 // Parts that a row is cut into: as many as give each compute unit two, of no less
-// than a step of each wave.
+// than a step of each wave. With a row for every second compute unit the second
+// launch and the reads of its own cost as much as they save: 64 rows of 128256 in
+// parts 17.7 us, 128 as long either way, 200 in parts 28.5, whole 23.3.
 int parts_for(int rows, int vocab) {
   const int compute_units = device_compute_units();
-  if (rows >= compute_units) return 1;
-  const int steps = (vocab + kTile * kWaves - 1) / (kTile * kWaves);
+  if (2 * rows > compute_units) return 1;
+  constexpr int kStep = kTile * kManyThreads / 64;
+  const int steps = (vocab + kStep - 1) / kStep;
   return std::max(1, std::min({kMostParts, (2 * compute_units + rows - 1) / rows, steps}));
 }
 
 size_t workspace_for(int rows, int parts, int top) {
   return static_cast<size_t>(rows) * static_cast<size_t>(parts) *
-         (sizeof(PartSums) + static_cast<size_t>(top) * sizeof(unsigned long long));
+         (sizeof(PartSums) + (top > 0 ? kManyThreads * sizeof(float) : 0));
+}
+
+template <bool kTop>
+void launch_parts(const LogprobArgs& a, int rows, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(a.parts), static_cast<unsigned>(rows));
+  logprobs_kernel<kTop, true, kManyThreads><<<grid, kManyThreads, 0, s>>>(a);
+  logprobs_join_kernel<kTop><<<static_cast<unsigned>(rows), kManyThreads, 0, s>>>(a);
+}
+
+template <int kThreads>
+void launch_rows(const LogprobArgs& a, int rows, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(rows);
+  if (a.top > 0) {
+    logprobs_kernel<true, false, kThreads><<<blocks, kThreads, 0, s>>>(a);
+  } else {
+    logprobs_kernel<false, false, kThreads><<<blocks, kThreads, 0, s>>>(a);
+  }
 }
 
 }  // namespace
@@ -609,7 +743,7 @@ extern "C" int lcr_batch_logprobs(float* logprobs, int32_t* ranks, float* entrop
   CAPI_CHECK(workspace != nullptr || workspace_bytes == 0,
              "batch_logprobs workspace of " << workspace_bytes << " bytes has no pointer");
   CAPI_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0, "batch_logprobs workspace must be 16-byte aligned");
-  CAPI_CHECK(static_cast<long long>(rows) * kThreads <= UINT32_MAX,
+  CAPI_CHECK(static_cast<long long>(rows) * kManyThreads <= UINT32_MAX,
              "batch_logprobs of " << rows << " rows needs more than 2^32 threads");
   LogprobArgs a{logprobs, ranks, entropies, top_ids, top_logprobs, logits, token_ids, top, vocab, logits_stride,
                 1, nullptr, nullptr};
@@ -618,21 +752,16 @@ extern "C" int lcr_batch_logprobs(float* logprobs, int32_t* ranks, float* entrop
   if (parts > 1 && workspace != nullptr && workspace_bytes >= workspace_for(rows, parts, top)) {
     a.parts = parts;
     a.sums = static_cast<PartSums*>(workspace);
-    a.keys = reinterpret_cast<unsigned long long*>(a.sums + static_cast<size_t>(rows) * parts);
-    const dim3 grid(static_cast<unsigned>(parts), static_cast<unsigned>(rows));
+    a.largest = reinterpret_cast<float*>(a.sums + static_cast<size_t>(rows) * parts);
     if (top > 0) {
-      logprobs_kernel<true, true><<<grid, kThreads, 0, s>>>(a);
-      CAPI_LAUNCHED();
-      logprobs_join_kernel<true><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+      launch_parts<true>(a, rows, s);
     } else {
-      logprobs_kernel<false, true><<<grid, kThreads, 0, s>>>(a);
-      CAPI_LAUNCHED();
-      logprobs_join_kernel<false><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+      launch_parts<false>(a, rows, s);
     }
-  } else if (top > 0) {
-    logprobs_kernel<true, false><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+  } else if (vocab <= kFewThreadTiles * kTile) {
+    launch_rows<kFewThreads>(a, rows, s);
   } else {
-    logprobs_kernel<false, false><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+    launch_rows<kManyThreads>(a, rows, s);
   }
   CAPI_LAUNCHED();
   return LCR_OK;
