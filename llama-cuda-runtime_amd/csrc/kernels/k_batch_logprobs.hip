@@ -7,10 +7,10 @@
 //   log p = l - m - log s,  entropy = log s - t / s.
 // Sixteen logits at a time are summed in fp32, and those sums in fp64.
 //
-// The likeliest ids need no order of all logits: the k-th largest of the lanes'
-// largest logits is one that at least k logits reach, and few others do. What the
-// lanes that hold one had is read again, and logits at least as large (about k) are
-// ranked by counting. The streaming pass does nothing for it but keep the largest.
+// The likeliest ids need no order of all logits: the k-th largest of 64 columns'
+// largest logits is one that at least k logits reach, and few others do. The tiles in
+// which a lane reaches it are read again, and logits at least as large (few more than
+// k) are ranked by counting. The streaming pass does nothing for it but keep the largest.
 //
 // Bound by memory: 11 operations a logit, the exponential four times as long as the
 // others, are half of the vector units' time at the rate that logits arrive.
@@ -181,13 +181,12 @@ constexpr int kMostReads = 1024;
 template <int kThreads>
 struct ChoiceLds {
   static constexpr int kWaves = kThreads / 64;
-  float lists[kWaves][64];
+  float largest[kWaves][64];
   unsigned long long candidates[kMostCandidates];
   uint16_t reads[kMostReads];   // what is read again, as the Source names it
   int found[kWaves];
   int read_count;
   int count;   // of candidates
-  float reach;
 };
 
 template <int kWaves>
@@ -216,16 +215,6 @@ __device__ __forceinline__ float exchange(float v, bool down) {
   return lower == down ? fmaxf(v, other) : fminf(v, other);
 }
 
-// 64 values that rise and then fall, or the reverse, in descending order.
-__device__ __forceinline__ float sort_bitonic(float v) {
-  v = exchange<32>(v, true);
-  v = exchange<16>(v, true);
-  v = exchange<8>(v, true);
-  v = exchange<4>(v, true);
-  v = exchange<2>(v, true);
-  return exchange<1>(v, true);
-}
-
 // A wave's 64 values in descending order.
 __device__ __forceinline__ float sort_wave(float v) {
   const int lane = lane_id();
@@ -244,25 +233,26 @@ __device__ __forceinline__ float sort_wave(float v) {
   v = exchange<4>(v, (lane & 32) == 0);
   v = exchange<2>(v, (lane & 32) == 0);
   v = exchange<1>(v, (lane & 32) == 0);
-  return sort_bitonic(v);
+  v = exchange<32>(v, true);
+  v = exchange<16>(v, true);
+  v = exchange<8>(v, true);
+  v = exchange<4>(v, true);
+  v = exchange<2>(v, true);
+  return exchange<1>(v, true);
 }
 
-// The top-th largest of the block's 64 kWaves values, for all of it.
+// The top-th largest of 64 values, each the largest that one lane of all waves has: a
+// bound that at least `top` logits of the block reach, and not many more. (With 20 of
+// 64, some 24. The exact one of all the lanes' takes three more merges and barriers.)
 template <int kThreads>
 __device__ __forceinline__ float largest_reached(ChoiceLds<kThreads>& lds, float v, int top) {
   constexpr int kWaves = kThreads / 64;
-  const int wave = static_cast<int>(threadIdx.x) >> 6;
-  v = sort_wave(v);
-#pragma unroll
-  for (int step = 1; step < kWaves; step <<= 1) {
-    if ((wave & (2 * step - 1)) == step) lds.lists[wave][lane_id()] = v;
-    __syncthreads();
-    // the larger of two lists' 64 values, one read backwards: they rise and fall
-    if ((wave & (2 * step - 1)) == 0) v = sort_bitonic(fmaxf(v, lds.lists[wave + step][63 - lane_id()]));
-  }
-  if (threadIdx.x == static_cast<unsigned>(top - 1)) lds.reach = v;
+  lds.largest[threadIdx.x >> 6][lane_id()] = v;
   __syncthreads();
-  return lds.reach;
+  v = lds.largest[0][lane_id()];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) v = fmaxf(v, lds.largest[w][lane_id()]);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sort_wave(v)), top - 1));
 }
 
 // Upper bits of a value's place in the order of values.
