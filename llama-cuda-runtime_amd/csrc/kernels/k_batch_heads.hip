@@ -15,7 +15,7 @@
 #include "../../../include/lcr_batch.h"
 #include "../capi_util.h"
 #include "../kv_cache.h"
-#include "device_common.h"
+#include "head_rotation.h"
 
 namespace lcr {
 namespace {
@@ -69,15 +69,6 @@ __device__ __forceinline__ HeadPlace place_head(const HeadsArgs& a, int row, int
                    (is_key ? a.view.keys : a.view.values) + at, is_key ? a.k_norm : nullptr, is_key};
 }
 
-// Sum over the kLanes lanes (a power of two) that share a head.
-template <int kLanes>
-__device__ __forceinline__ float head_sum(float v) {
-  if constexpr (kLanes >= 16) v += xor_lane<8>(v);
-  if constexpr (kLanes >= 8) v += xor_lane<4>(v);
-  if constexpr (kLanes >= 4) v += xor_lane<2>(v);
-  return v + xor_lane<1>(v);
-}
-
 template <int kHeadDim>
 __global__ __launch_bounds__(kHeadsThreads) void batch_heads_kernel(HeadsArgs a) {
   constexpr int kLanes = kHeadDim / 16;
@@ -94,34 +85,7 @@ __global__ __launch_bounds__(kHeadsThreads) void batch_heads_kernel(HeadsArgs a)
   const HeadPlace h = place_head(a, row, head, cache_slot, kHeadDim);
   vec16 lo = load16(h.src + i), hi = load16(h.src + kHalf + i);
   if (h.rotate) {
-    const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<size_t>(position) * kHalf + i);
-    float4 angle[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) angle[j] = cs[j];
-    float x[8], y[8];
-    unpack8(lo, x);
-    unpack8(hi, y);
-    if (h.weight != nullptr) {
-      float wx[8], wy[8];
-      unpack8(load16(h.weight + i), wx);
-      unpack8(load16(h.weight + kHalf + i), wy);
-      float square = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) square = __builtin_fmaf(x[j], x[j], __builtin_fmaf(y[j], y[j], square));
-      const float scale = 1.0f / sqrtf(head_sum<kLanes>(square) * (1.0f / kHeadDim) + a.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = x[j] * scale * wx[j];
-        y[j] = y[j] * scale * wy[j];
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 r0 = rope_rotate(x[2 * j], y[2 * j], make_float2(angle[j].x, angle[j].y));
-      const float2 r1 = rope_rotate(x[2 * j + 1], y[2 * j + 1], make_float2(angle[j].z, angle[j].w));
-      lo.w[j] = pack_elems(r0.x, r1.x);
-      hi.w[j] = pack_elems(r0.y, r1.y);
-    }
+    norm_rotate<kHeadDim>(lo, hi, h.weight, a.eps, a.table + static_cast<size_t>(position) * kHalf, i);
   }
   store16(h.dst + i, lo);
   store16(h.dst + kHalf + i, hi);

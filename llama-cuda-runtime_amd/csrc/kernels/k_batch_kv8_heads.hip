@@ -11,6 +11,7 @@
 #include <cstdint>
 
 #include "../capi_util.h"
+#include "head_rotation.h"
 #include "kv8.h"
 
 namespace lcr {
@@ -19,6 +20,7 @@ namespace {
 constexpr int kHeadsThreads = 256;
 constexpr int kHeadsWaves = kHeadsThreads / 64;
 constexpr int kMaxHeadDim = 256;
+constexpr int kMostWaves = 16384;  // that a call's keys and values are spread over, more or less
 
 struct Heads8Args {
   elem_t* q_out;
@@ -58,6 +60,12 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   v += xor_lane_f64<4>(v);
   v += xor_lane_f64<2>(v);
   return v + xor_lane_f64<1>(v);
+}
+
+__device__ __forceinline__ void wave_settled() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // Which rows of a call write to a block: lanes 0 .. 30 look at rows row - 15 ..
@@ -244,6 +252,337 @@ __global__ __launch_bounds__(kHeadsThreads) void batch_kv8_heads_any_kernel(Head
   }
 }
 
+// ---------------------------------------------------------------------------
+// Heads of 64 and 128, rows on 16 bytes
+// ---------------------------------------------------------------------------
+
+// Rows of a window, whose blocks are some waves' work, and the rows about them that
+// may lie in the same blocks: lane n looks at row first - 15 + n.
+constexpr int kWindowRows = 16;
+constexpr int kWindowLanes = kWindowRows + 2 * 15;
+
+struct Window {
+  int first;      // row
+  int slot;       // this lane's row's, -1: none that counts
+  int position;
+  int leader;     // the lane of its block's first row
+  unsigned long long leaders;  // lanes of the window that are first of their blocks
+
+  __device__ __forceinline__ Window(const Heads8Args& a, int first_row) : first(first_row), slot(-1), position(0) {
+    const int lane = lane_id();
+    const int row = first - 15 + lane;
+    if (lane < kWindowLanes && row >= 0 && row < a.tokens) {
+      const int s = a.slots[row];
+      position = a.positions[row];
+      if (row_is_live(a, s, position)) slot = s;
+    }
+    // Each lane looks back: a wave shift for each of the 15 lanes before it.
+    const int block = slot >> 4;
+    int before = block;
+    leader = lane;
+#pragma unroll
+    for (int o = 1; o <= 15; ++o) {
+      before = __builtin_amdgcn_update_dpp(-1, before, 0x138, 0xF, 0xF, false);  // wave_shr:1
+      if (before == block) leader = lane - o;
+    }
+    leaders = __ballot(slot >= 0 && leader == lane && lane >= 15 && lane < 15 + kWindowRows);
+  }
+};
+static_assert(kKv8Block == 16, "a slot's block is slot >> 4");
+
+// Up to 16 rows that follow each other, with blocks that lie among them whole: four
+// lanes a row. One new token each of 16 sequences, or 16 of one, is one such set.
+struct RowSet {
+  int row;         // this lane's, -1: none that counts
+  int position;
+  int t;           // its position in its block
+  int first;       // which of the set's rows is the first of its block
+  size_t block;    // first byte of the block of the first kv head, and its scale
+  size_t scale;
+  uint32_t written;  // the block's positions that this call writes
+
+  // Takes a set's leaders out of `left`.
+  __device__ __forceinline__ RowSet(const Heads8Args& a, const Window& win, unsigned long long& left,
+                                    uint32_t* lds_written) {
+    const int start = __builtin_ctzll(left);
+    // leaders with rows behind the set wait for one of their own
+    unsigned long long cut = __ballot(win.slot >= 0 && lane_id() >= start + 16 && win.leader >= start &&
+                                      win.leader < start + 16);
+    unsigned long long whole = left & (0xffffull << start);
+    for (; cut != 0; cut &= cut - 1) whole &= ~(1ull << __builtin_amdgcn_readlane(win.leader, __builtin_ctzll(cut)));
+    left &= ~whole;
+    const int group = lane_id() >> 2;
+    const int from = start + group;  // at most 30 + 15
+    const int slot = __shfl(win.slot, from, 64);
+    const int leader = __shfl(win.leader, from, 64);
+    position = __shfl(win.position, from, 64);
+    row = slot >= 0 && (whole >> leader & 1ull) != 0 ? win.first - 15 + from : -1;
+    t = slot & (kKv8Block - 1);
+    first = row >= 0 ? leader - start : group;
+    const int counted = row >= 0 ? slot : 0;
+    const int page = counted / a.view.page_size;
+    const int n = (counted - page * a.view.page_size) / kKv8Block;
+    block = a.view.block_at(page, 0, n);
+    scale = a.view.scale_at(page, 0, n);
+    if (lane_id() < 16) lds_written[lane_id()] = 0;
+    wave_settled();
+    if (row >= 0 && (lane_id() & 3) == 0) atomicOr(&lds_written[first], 1u << t);
+    wave_settled();
+    written = lds_written[first];
+    wave_settled();
+  }
+  __device__ __forceinline__ bool leads() const { return row >= 0 && first == lane_id() >> 2; }
+};
+
+// The scale of a row's block, from the largest of this row's values (of four lanes):
+// the larger of what the block's new values need and, unless the block begins, of what
+// it has. `move`: what the numbers held are multiplied by, 1 where they stay.
+__device__ __forceinline__ float block_scale(const RowSet& set, float held, float largest, uint32_t* lds_largest,
+                                             float& move) {
+  largest = fmaxf(largest, xor_lane<1>(largest));
+  largest = fmaxf(largest, xor_lane<2>(largest));
+  if (lane_id() < 16) lds_largest[lane_id()] = 0;
+  wave_settled();
+  // no less than 0, so that they compare as their bits do
+  if (set.row >= 0 && (lane_id() & 3) == 0) atomicMax(&lds_largest[set.first], __builtin_bit_cast(uint32_t, largest));
+  wave_settled();
+  largest = __builtin_bit_cast(float, lds_largest[set.first]);
+  wave_settled();
+  const float need = power_of_two(kv8_exponent_for(largest));
+  move = 1.0f;
+  if (set.written & 1u) return need;
+  const float after = fmaxf(need, held);
+  if (after > held) move = held / after;
+  return after;
+}
+
+__device__ __forceinline__ uint32_t moved_numbers(uint32_t w, float move) {
+  float x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = kv8_number(static_cast<uint8_t>(w >> (8 * i))) * move;
+  return kv8_pair(x[0], x[1]) | kv8_pair(x[2], x[3]) << 16;
+}
+
+// Rounds what blocks hold to their larger scales, but for the positions written: block
+// after block, by the whole wave. Stores touch only bytes that no others do, so that
+// they need no order among the new numbers'.
+template <int kHeadDim, bool kKeys>
+__device__ __forceinline__ void move_blocks(const RowSet& set, uint8_t* numbers, float move) {
+  for (unsigned long long m = __ballot(set.leads() && (lane_id() & 3) == 0 && move != 1.0f); m != 0; m &= m - 1) {
+    const int lane = __builtin_ctzll(m);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(set.block), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(set.block >> 32), lane);
+    const uint32_t written = __builtin_amdgcn_readlane(set.written, lane);
+    const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, move), lane));
+    uint8_t* bytes = numbers + (static_cast<size_t>(hi) << 32 | lo);
+    for (int n = lane_id(); n < kKv8Block * kHeadDim / 4; n += 64) {
+      uint32_t* const at = reinterpret_cast<uint32_t*>(bytes) + n;
+      // four dims of one position, or one dim of four
+      const uint32_t skip = kKeys ? (written >> (4 * n / kHeadDim) & 1u ? 15u : 0u) : written >> (n / kHeadDim * 4) & 15u;
+      if (skip == 15u) continue;
+      const uint32_t w = moved_numbers(*at, by);
+      if (skip == 0u) {
+        *at = w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((skip >> i & 1u) == 0) reinterpret_cast<uint8_t*>(at)[i] = static_cast<uint8_t>(w >> (8 * i));
+        }
+      }
+    }
+  }
+}
+
+// What the largest of `n` values is, for their block's scale. Values past the largest
+// that is held are clamped and infinities made NaN, where there are any.
+template <int n>
+__device__ __forceinline__ float largest_of(float* v) {
+  float most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < n; j += 2) {
+    most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, fabsf(v[j])), fabsf(v[j + 1]));
+  }
+  if (__any(!(most <= kKv8Largest))) {
+    most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      v[j] = fabsf(v[j]) < __builtin_huge_valf() ? kv8_clamped(v[j]) : __builtin_nanf("");
+      most = fmaxf(most, kv8_size(v[j]));
+    }
+  }
+  return most;
+}
+
+// Four values over their scale as numbers: none is infinite.
+__device__ __forceinline__ uint32_t four_numbers(const float* v, float inverse) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, w, true);
+  return static_cast<uint32_t>(w);
+}
+
+// Keys of a set: a lane has a quarter of both halves of a head, so that pairs stay in
+// their lanes and the norm is two exchanges.
+template <int kHeadDim>
+__device__ __forceinline__ void append_keys(const Heads8Args& a, const RowSet& set, int head, uint32_t* lds_largest) {
+  constexpr int kHalf = kHeadDim / 2;
+  constexpr int kPairs = kHeadDim / 8;  // of a lane
+  const int i0 = kPairs * (lane_id() & 3);
+  const size_t scale_at = set.scale + static_cast<size_t>(head) * static_cast<size_t>(a.view.scale_head_stride);
+  const float held = a.view.key_scales[scale_at];
+  const int row = max(set.row, 0);
+  const elem_t* src = a.k + static_cast<size_t>(row) * static_cast<size_t>(a.src_row_stride) +
+                      static_cast<size_t>(head) * kHeadDim + i0;
+  const float4* cs = reinterpret_cast<const float4*>(a.table + static_cast<size_t>(set.row >= 0 ? set.position : 0) * kHalf + i0);
+  float v[2 * kPairs];  // lower halves' elements, then the upper's
+  if (set.row >= 0) {
+#pragma unroll
+    for (int j = 0; j < kPairs; j += 8) {
+      unpack8(load16(src + j), v + j);
+      unpack8(load16(src + kHalf + j), v + kPairs + j);
+    }
+    double scale = 1.0;
+    if (a.k_norm != nullptr) {
+      double square = 0.0;
+#pragma unroll
+      for (int j = 0; j < 2 * kPairs; ++j) square = __builtin_fma(static_cast<double>(v[j]), static_cast<double>(v[j]), square);
+      square += xor_lane_f64<1>(square);
+      square += xor_lane_f64<2>(square);
+      scale = 1.0 / sqrt(square * (1.0 / kHeadDim) + static_cast<double>(a.eps));
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; j += 8) {
+      float4 angle[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) angle[n] = cs[j / 2 + n];
+      float wx[8], wy[8];
+      if (a.k_norm != nullptr) {
+        unpack8(load16(a.k_norm + i0 + j), wx);
+        unpack8(load16(a.k_norm + kHalf + i0 + j), wy);
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        double x = v[j + n], y = v[kPairs + j + n];
+        if (a.k_norm != nullptr) {
+          x = x * scale * static_cast<double>(wx[n]);
+          y = y * scale * static_cast<double>(wy[n]);
+        }
+        const double c = n & 1 ? angle[n / 2].z : angle[n / 2].x;
+        const double s = n & 1 ? angle[n / 2].w : angle[n / 2].y;
+        v[j + n] = static_cast<float>(x * c - y * s);
+        v[kPairs + j + n] = static_cast<float>(y * c + x * s);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2 * kPairs; ++j) v[j] = 0.0f;
+  }
+  float move;
+  const float scale = block_scale(set, held, largest_of<2 * kPairs>(v), lds_largest, move);
+  uint8_t* const numbers = a.view.keys + static_cast<size_t>(head) * static_cast<size_t>(a.view.head_stride);
+  if (set.row >= 0) {
+    if (set.leads() && (lane_id() & 3) == 0) a.view.key_scales[scale_at] = scale;
+    uint8_t* const to = numbers + set.block + kv8_key_byte(kHeadDim, set.t, i0);
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int j = 0; j < kPairs; j += 8) {
+      *reinterpret_cast<uint2*>(to + j) = make_uint2(four_numbers(v + j, inverse), four_numbers(v + j + 4, inverse));
+      *reinterpret_cast<uint2*>(to + kHalf + j) =
+          make_uint2(four_numbers(v + kPairs + j, inverse), four_numbers(v + kPairs + j + 4, inverse));
+    }
+  }
+  move_blocks<kHeadDim, true>(set, numbers, move);
+}
+
+// Values of a set: a lane has a quarter of a head's dims.
+template <int kHeadDim>
+__device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet& set, int head, uint32_t* lds_largest) {
+  constexpr int kDims = kHeadDim / 4;
+  const int i0 = kDims * (lane_id() & 3);
+  const size_t scale_at = set.scale + static_cast<size_t>(head) * static_cast<size_t>(a.view.scale_head_stride);
+  const float held = a.view.value_scales[scale_at];
+  const elem_t* src = a.v + static_cast<size_t>(max(set.row, 0)) * static_cast<size_t>(a.src_row_stride) +
+                      static_cast<size_t>(head) * kHeadDim + i0;
+  float v[kDims];
+#pragma unroll
+  for (int j = 0; j < kDims; j += 8) {
+    vec16 w{{0u, 0u, 0u, 0u}};
+    if (set.row >= 0) w = load16(src + j);
+    unpack8(w, v + j);
+  }
+  float move;
+  const float scale = block_scale(set, held, largest_of<kDims>(v), lds_largest, move);
+  uint8_t* const numbers = a.view.values + static_cast<size_t>(head) * static_cast<size_t>(a.view.head_stride);
+  if (set.row >= 0) {
+    if (set.leads() && (lane_id() & 3) == 0) a.view.value_scales[scale_at] = scale;
+    uint8_t* const to = numbers + set.block + kv8_value_byte(kHeadDim, set.t, i0);
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int j = 0; j < kDims; j += 4) {
+      const uint32_t w = four_numbers(v + j, inverse);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[4 * (j + i)] = static_cast<uint8_t>(w >> (8 * i));
+    }
+  }
+  move_blocks<kHeadDim, false>(set, numbers, move);
+}
+
+// The first q_blocks blocks have the queries, kHeadDim / 16 lanes a head; behind them
+// `waves` waves share a window's kv heads, keys and values.
+template <int kHeadDim>
+__global__ __launch_bounds__(kHeadsThreads) void batch_kv8_heads_kernel(Heads8Args a, unsigned q_blocks, int waves) {
+  __shared__ uint32_t lds_words[kHeadsWaves][16];
+  if (blockIdx.x < q_blocks) {
+    constexpr int kLanes = kHeadDim / 16;
+    constexpr int kHalf = kHeadDim / 2;
+    const long long unit = (static_cast<long long>(blockIdx.x) * kHeadsThreads + threadIdx.x) / kLanes;
+    const int row = static_cast<int>(unit / a.num_heads);
+    const int head = static_cast<int>(unit - static_cast<long long>(row) * a.num_heads);
+    const int i = 8 * (static_cast<int>(threadIdx.x) % kLanes);
+    if (row >= a.tokens) return;  // whole heads leave together
+    const int position = a.positions[row];
+    if (!row_is_live(a, a.slots[row], position)) return;
+    const elem_t* src = a.q + static_cast<size_t>(row) * static_cast<size_t>(a.src_row_stride) +
+                        static_cast<size_t>(head) * kHeadDim + i;
+    elem_t* dst = a.q_out + (static_cast<size_t>(row) * a.num_heads + head) * kHeadDim + i;
+    vec16 lo = load16(src), hi = load16(src + kHalf);
+    norm_rotate<kHeadDim>(lo, hi, a.q_norm, a.eps, a.table + static_cast<size_t>(position) * kHalf, i);
+    store16(dst, lo);
+    store16(dst + kHalf, hi);
+    return;
+  }
+  const int in_block = static_cast<int>(threadIdx.x) >> 6;
+  const long long wave = static_cast<long long>(blockIdx.x - q_blocks) * kHeadsWaves + in_block;
+  const int window = __builtin_amdgcn_readfirstlane(static_cast<int>(wave / waves));
+  const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(wave % waves));
+  if (window * kWindowRows >= a.tokens) return;
+  const Window win(a, window * kWindowRows);
+  const int kv = a.view.num_kv_heads;
+  unsigned long long left = win.leaders;
+  while (left != 0) {
+    const RowSet set(a, win, left, lds_words[in_block]);
+    for (int n = share; n < 2 * kv; n += waves) {
+      if (n < kv) {
+        append_keys<kHeadDim>(a, set, n, lds_words[in_block]);
+      } else {
+        append_values<kHeadDim>(a, set, n - kv, lds_words[in_block]);
+      }
+    }
+  }
+}
+
+template <int kHeadDim>
+void launch_heads(const Heads8Args& a, hipStream_t s) {
+  const long long q_lanes = static_cast<long long>(a.tokens) * a.num_heads * (kHeadDim / 16);
+  const unsigned q_blocks = static_cast<unsigned>((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
+  const int windows = (a.tokens + kWindowRows - 1) / kWindowRows;
+  const int waves = std::min(2 * a.view.num_kv_heads, (kMostWaves + windows - 1) / windows);
+  const long long kv_waves = waves > 0 ? static_cast<long long>(windows) * waves : 0;
+  const unsigned blocks = q_blocks + static_cast<unsigned>((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
+  batch_kv8_heads_kernel<kHeadDim><<<blocks, kHeadsThreads, 0, s>>>(a, q_blocks, std::max(waves, 1));
+}
+
+bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 }  // namespace
 }  // namespace lcr
 
@@ -302,8 +641,16 @@ extern "C" int lcr_batch_norm_rope_write_kv8(void* q_out, const lcr_kv8_view* vi
   a.pool_slots = pool_pages * view->page_size;
   a.src_row_stride = src_row_stride;
   auto s = static_cast<hipStream_t>(stream);
-  const unsigned blocks = static_cast<unsigned>((tokens * heads + kHeadsWaves - 1) / kHeadsWaves);
-  batch_kv8_heads_any_kernel<<<blocks, kHeadsThreads, 0, s>>>(a);
+  const bool aligned = on_16_bytes(q_out) && on_16_bytes(q) && on_16_bytes(k) && on_16_bytes(v) &&
+                       on_16_bytes(q_norm) && on_16_bytes(k_norm) && on_16_bytes(rope_table) && src_row_stride % 8 == 0;
+  if (aligned && view->head_dim == 64) {
+    launch_heads<64>(a, s);
+  } else if (aligned && view->head_dim == 128) {
+    launch_heads<128>(a, s);
+  } else {
+    const unsigned blocks = static_cast<unsigned>((tokens * heads + kHeadsWaves - 1) / kHeadsWaves);
+    batch_kv8_heads_any_kernel<<<blocks, kHeadsThreads, 0, s>>>(a);
+  }
   CAPI_LAUNCHED();
   return LCR_OK;
 }
