@@ -375,18 +375,24 @@ __device__ __forceinline__ void move_blocks(const RowSet& set, uint8_t* numbers,
     const uint32_t written = __builtin_amdgcn_readlane(set.written, lane);
     const float by = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, move), lane));
     uint8_t* bytes = numbers + (static_cast<size_t>(hi) << 32 | lo);
-    for (int n = lane_id(); n < kKv8Block * kHeadDim / 4; n += 64) {
-      uint32_t* const at = reinterpret_cast<uint32_t*>(bytes) + n;
-      // four dims of one position, or one dim of four
-      const uint32_t skip = kKeys ? (written >> (4 * n / kHeadDim) & 1u ? 15u : 0u) : written >> (n / kHeadDim * 4) & 15u;
-      if (skip == 15u) continue;
-      const uint32_t w = moved_numbers(*at, by);
-      if (skip == 0u) {
-        *at = w;
-      } else {
+    constexpr int kChunks = kHeadDim / 64;  // 16 bytes a lane
+    vec16 old[kChunks];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((skip >> i & 1u) == 0) reinterpret_cast<uint8_t*>(at)[i] = static_cast<uint8_t>(w >> (8 * i));
+    for (int h = 0; h < kChunks; ++h) old[h] = load16(bytes + 16 * (lane_id() + 64 * h));
+#pragma unroll
+    for (int h = 0; h < kChunks; ++h) {
+      // 16 dims of one position, or four of four
+      const int at = 16 * (lane_id() + 64 * h);
+      const uint32_t skip = kKeys ? (written >> (at / kHeadDim) & 1u ? 15u : 0u) : written >> (at / (4 * kHeadDim) * 4) & 15u;
+      vec16 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w.w[i] = moved_numbers(old[h].w[i], by);
+      if (skip == 0u) {
+        store16(bytes + at, w);
+      } else if (skip != 15u) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          if ((skip >> (n & 3) & 1u) == 0) bytes[at + n] = static_cast<uint8_t>(w.w[n / 4] >> (8 * (n & 3)));
         }
       }
     }
@@ -411,6 +417,13 @@ __device__ __forceinline__ float largest_of(float* v) {
     }
   }
   return most;
+}
+
+__device__ __forceinline__ void unpack4(const uint2& w, float* out) {
+  out[0] = elem_lo(w.x);
+  out[1] = elem_hi(w.x);
+  out[2] = elem_lo(w.y);
+  out[3] = elem_hi(w.y);
 }
 
 // Four values over their scale as numbers: none is infinite.
@@ -440,37 +453,39 @@ __device__ __forceinline__ void append_keys(const Heads8Args& a, const RowSet& s
       unpack8(load16(src + j), v + j);
       unpack8(load16(src + kHalf + j), v + kPairs + j);
     }
+    // Without a norm everything is multiplied with ones, as two forms of the loop below
+    // cost the registers of both.
+    const bool normed = a.k_norm != nullptr;
+    const elem_t* weights = normed ? a.k_norm + i0 : src;
     double scale = 1.0;
-    if (a.k_norm != nullptr) {
+    if (normed) {
       double square = 0.0;
 #pragma unroll
       for (int j = 0; j < 2 * kPairs; ++j) square = __builtin_fma(static_cast<double>(v[j]), static_cast<double>(v[j]), square);
       square += xor_lane_f64<1>(square);
       square += xor_lane_f64<2>(square);
       scale = 1.0 / sqrt(square * (1.0 / kHeadDim) + static_cast<double>(a.eps));
+      // widened again below: kept in fp64, they cost twice their registers
+#pragma unroll
+      for (int j = 0; j < 2 * kPairs; ++j) asm volatile("" : "+v"(v[j]));
     }
 #pragma unroll
-    for (int j = 0; j < kPairs; j += 8) {
-      float4 angle[4];
+    for (int j = 0; j < kPairs; j += 4) {
+      const float4 angle[2] = {cs[j / 2], cs[j / 2 + 1]};
+      float wx[4], wy[4];
+      unpack4(*reinterpret_cast<const uint2*>(weights + j), wx);
+      unpack4(*reinterpret_cast<const uint2*>(weights + kHalf + j), wy);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) angle[n] = cs[j / 2 + n];
-      float wx[8], wy[8];
-      if (a.k_norm != nullptr) {
-        unpack8(load16(a.k_norm + i0 + j), wx);
-        unpack8(load16(a.k_norm + kHalf + i0 + j), wy);
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        double x = v[j + n], y = v[kPairs + j + n];
-        if (a.k_norm != nullptr) {
-          x = x * scale * static_cast<double>(wx[n]);
-          y = y * scale * static_cast<double>(wy[n]);
-        }
+      for (int n = 0; n < 4; ++n) {
+        const double x = static_cast<double>(v[j + n]) * scale * static_cast<double>(normed ? wx[n] : 1.0f);
+        const double y = static_cast<double>(v[kPairs + j + n]) * scale * static_cast<double>(normed ? wy[n] : 1.0f);
         const double c = n & 1 ? angle[n / 2].z : angle[n / 2].x;
         const double s = n & 1 ? angle[n / 2].w : angle[n / 2].y;
         v[j + n] = static_cast<float>(x * c - y * s);
         v[kPairs + j + n] = static_cast<float>(y * c + x * s);
       }
+      // heads of 128: what the next four need is loaded behind these, for registers
+      if constexpr (kHeadDim > 64) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
 #pragma unroll
@@ -526,15 +541,23 @@ __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet&
   move_blocks<kHeadDim, false>(set, numbers, move);
 }
 
-// The first q_blocks blocks have the queries, kHeadDim / 16 lanes a head; behind them
-// `waves` waves share a window's kv heads, keys and values.
+// Blocks with queries, kHeadDim / 16 lanes a head, and blocks whose waves share the
+// windows' kv heads, keys and values, `waves` a window. The first move bytes and the
+// others compute, so they lie between each other, eight blocks at a time for the eight
+// XCDs: each `period`-th group is one of the kv_groups. 6779 rows of 32 on 8 heads of
+// 64, queries and then the others 23 us; either alone 11 and 15.
 template <int kHeadDim>
-__global__ __launch_bounds__(kHeadsThreads) void batch_kv8_heads_kernel(Heads8Args a, unsigned q_blocks, int waves) {
+__global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(
+    Heads8Args a, unsigned kv_groups, unsigned period, int waves) {
   __shared__ uint32_t lds_words[kHeadsWaves][16];
-  if (blockIdx.x < q_blocks) {
+  const unsigned group = blockIdx.x / 8u, in_group = blockIdx.x % 8u;
+  const unsigned nth = group / period;
+  const bool is_kv = nth * period == group && nth < kv_groups;
+  if (!is_kv) {
+    const unsigned q_block = 8u * (group - min(nth + (nth * period == group ? 0u : 1u), kv_groups)) + in_group;
     constexpr int kLanes = kHeadDim / 16;
     constexpr int kHalf = kHeadDim / 2;
-    const long long unit = (static_cast<long long>(blockIdx.x) * kHeadsThreads + threadIdx.x) / kLanes;
+    const long long unit = (static_cast<long long>(q_block) * kHeadsThreads + threadIdx.x) / kLanes;
     const int row = static_cast<int>(unit / a.num_heads);
     const int head = static_cast<int>(unit - static_cast<long long>(row) * a.num_heads);
     const int i = 8 * (static_cast<int>(threadIdx.x) % kLanes);
@@ -551,7 +574,7 @@ __global__ __launch_bounds__(kHeadsThreads) void batch_kv8_heads_kernel(Heads8Ar
     return;
   }
   const int in_block = static_cast<int>(threadIdx.x) >> 6;
-  const long long wave = static_cast<long long>(blockIdx.x - q_blocks) * kHeadsWaves + in_block;
+  const long long wave = static_cast<long long>(8u * nth + in_group) * kHeadsWaves + in_block;
   const int window = __builtin_amdgcn_readfirstlane(static_cast<int>(wave / waves));
   const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(wave % waves));
   if (window * kWindowRows >= a.tokens) return;
@@ -572,13 +595,15 @@ __global__ __launch_bounds__(kHeadsThreads) void batch_kv8_heads_kernel(Heads8Ar
 
 template <int kHeadDim>
 void launch_heads(const Heads8Args& a, hipStream_t s) {
+  auto groups_of = [](long long blocks) { return static_cast<unsigned>((blocks + 7) / 8); };
   const long long q_lanes = static_cast<long long>(a.tokens) * a.num_heads * (kHeadDim / 16);
-  const unsigned q_blocks = static_cast<unsigned>((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
   const int windows = (a.tokens + kWindowRows - 1) / kWindowRows;
   const int waves = std::min(2 * a.view.num_kv_heads, (kMostWaves + windows - 1) / windows);
-  const long long kv_waves = waves > 0 ? static_cast<long long>(windows) * waves : 0;
-  const unsigned blocks = q_blocks + static_cast<unsigned>((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
-  batch_kv8_heads_kernel<kHeadDim><<<blocks, kHeadsThreads, 0, s>>>(a, q_blocks, std::max(waves, 1));
+  const long long kv_waves = static_cast<long long>(windows) * waves;
+  const unsigned kv_groups = groups_of((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
+  const unsigned groups = kv_groups + groups_of((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
+  const unsigned period = kv_groups > 0 ? groups / kv_groups : 1;
+  batch_kv8_heads_kernel<kHeadDim><<<8 * groups, kHeadsThreads, 0, s>>>(a, kv_groups, period, std::max(waves, 1));
 }
 
 bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
