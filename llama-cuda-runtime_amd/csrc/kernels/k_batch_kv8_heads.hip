@@ -508,53 +508,64 @@ __device__ __forceinline__ void append_keys(const Heads8Args& a, const RowSet& s
   move_blocks<kHeadDim, true>(set, numbers, move);
 }
 
-// Values of a set: a lane has a quarter of a head's dims.
+// Values of a set: a lane has four neighbouring dims of each 16. A position's bytes
+// lie four apart, those of the three beside it between them. A row alone among its
+// four reads them and writes all, unless they change their scale; rows together write
+// their bytes. (4000 rows of sequences of their own, 16 on 8 heads of 128, 54 us with
+// bytes alone.)
 template <int kHeadDim>
 __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet& set, int head, uint32_t* lds_largest) {
-  constexpr int kDims = kHeadDim / 4;
-  const int i0 = kDims * (lane_id() & 3);
+  constexpr int kFours = kHeadDim / 16;
+  const int i0 = 4 * (lane_id() & 3);
   const size_t scale_at = set.scale + static_cast<size_t>(head) * static_cast<size_t>(a.view.scale_head_stride);
   const float held = a.view.value_scales[scale_at];
   const elem_t* src = a.v + static_cast<size_t>(max(set.row, 0)) * static_cast<size_t>(a.src_row_stride) +
                       static_cast<size_t>(head) * kHeadDim + i0;
-  float v[kDims];
+  uint8_t* const numbers = a.view.values + static_cast<size_t>(head) * static_cast<size_t>(a.view.head_stride);
+  uint8_t* const four = numbers + set.block + kv8_value_byte(kHeadDim, set.t & ~3, i0);
+  const bool single = set.row >= 0 && __popc(set.written >> (set.t & ~3) & 15u) == 1;
+  float v[4 * kFours];
+  vec16 beside[kFours];
 #pragma unroll
-  for (int j = 0; j < kDims; j += 8) {
-    vec16 w{{0u, 0u, 0u, 0u}};
-    if (set.row >= 0) w = load16(src + j);
-    unpack8(w, v + j);
+  for (int j = 0; j < kFours; ++j) {
+    uint2 w = make_uint2(0u, 0u);
+    if (set.row >= 0) w = *reinterpret_cast<const uint2*>(src + 16 * j);
+    unpack4(w, v + 4 * j);
+    if (single) beside[j] = load16(four + 64 * j);
   }
   float move;
-  const float scale = block_scale(set, held, largest_of<kDims>(v), lds_largest, move);
-  uint8_t* const numbers = a.view.values + static_cast<size_t>(head) * static_cast<size_t>(a.view.head_stride);
+  const float scale = block_scale(set, held, largest_of<4 * kFours>(v), lds_largest, move);
   if (set.row >= 0) {
     if (set.leads() && (lane_id() & 3) == 0) a.view.value_scales[scale_at] = scale;
-    uint8_t* const to = numbers + set.block + kv8_value_byte(kHeadDim, set.t, i0);
     const float inverse = 1.0f / scale;
+    const int byte = set.t & 3;
 #pragma unroll
-    for (int j = 0; j < kDims; j += 4) {
-      const uint32_t w = four_numbers(v + j, inverse);
+    for (int j = 0; j < kFours; ++j) {
+      const uint32_t w = four_numbers(v + 4 * j, inverse);
+      if (single && move == 1.0f) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) to[4 * (j + i)] = static_cast<uint8_t>(w >> (8 * i));
+        for (int i = 0; i < 4; ++i) {
+          beside[j].w[i] = (beside[j].w[i] & ~(0xffu << (8 * byte))) | (w >> (8 * i) & 0xffu) << (8 * byte);
+        }
+        store16(four + 64 * j, beside[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) four[64 * j + 4 * i + byte] = static_cast<uint8_t>(w >> (8 * i));
+      }
     }
   }
   move_blocks<kHeadDim, false>(set, numbers, move);
 }
 
-// Blocks with queries, kHeadDim / 16 lanes a head, and blocks whose waves share the
-// windows' kv heads, keys and values, `waves` a window. The first move bytes and the
-// others compute, so they lie between each other, eight blocks at a time for the eight
-// XCDs: each `period`-th group is one of the kv_groups. 6779 rows of 32 on 8 heads of
-// 64, queries and then the others 23 us; either alone 11 and 15.
+// The first kv_blocks blocks' waves share the windows' kv heads, keys and values,
+// `waves` a window; behind them come the queries, kHeadDim / 16 lanes a head. The first
+// compute, the others move bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64,
+// queries first 23 us, then 19; either alone 11 and 13.
 template <int kHeadDim>
-__global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(
-    Heads8Args a, unsigned kv_groups, unsigned period, int waves) {
+__global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(Heads8Args a, unsigned kv_blocks, int waves) {
   __shared__ uint32_t lds_words[kHeadsWaves][16];
-  const unsigned group = blockIdx.x / 8u, in_group = blockIdx.x % 8u;
-  const unsigned nth = group / period;
-  const bool is_kv = nth * period == group && nth < kv_groups;
-  if (!is_kv) {
-    const unsigned q_block = 8u * (group - min(nth + (nth * period == group ? 0u : 1u), kv_groups)) + in_group;
+  if (blockIdx.x >= kv_blocks) {
+    const unsigned q_block = blockIdx.x - kv_blocks;
     constexpr int kLanes = kHeadDim / 16;
     constexpr int kHalf = kHeadDim / 2;
     const long long unit = (static_cast<long long>(q_block) * kHeadsThreads + threadIdx.x) / kLanes;
@@ -574,7 +585,7 @@ __global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(
     return;
   }
   const int in_block = static_cast<int>(threadIdx.x) >> 6;
-  const long long wave = static_cast<long long>(8u * nth + in_group) * kHeadsWaves + in_block;
+  const long long wave = static_cast<long long>(blockIdx.x) * kHeadsWaves + in_block;
   const int window = __builtin_amdgcn_readfirstlane(static_cast<int>(wave / waves));
   const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(wave % waves));
   if (window * kWindowRows >= a.tokens) return;
@@ -595,15 +606,13 @@ __global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(
 
 template <int kHeadDim>
 void launch_heads(const Heads8Args& a, hipStream_t s) {
-  auto groups_of = [](long long blocks) { return static_cast<unsigned>((blocks + 7) / 8); };
   const long long q_lanes = static_cast<long long>(a.tokens) * a.num_heads * (kHeadDim / 16);
+  const unsigned q_blocks = static_cast<unsigned>((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
   const int windows = (a.tokens + kWindowRows - 1) / kWindowRows;
   const int waves = std::min(2 * a.view.num_kv_heads, (kMostWaves + windows - 1) / windows);
   const long long kv_waves = static_cast<long long>(windows) * waves;
-  const unsigned kv_groups = groups_of((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
-  const unsigned groups = kv_groups + groups_of((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
-  const unsigned period = kv_groups > 0 ? groups / kv_groups : 1;
-  batch_kv8_heads_kernel<kHeadDim><<<8 * groups, kHeadsThreads, 0, s>>>(a, kv_groups, period, std::max(waves, 1));
+  const unsigned kv_blocks = static_cast<unsigned>((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
+  batch_kv8_heads_kernel<kHeadDim><<<kv_blocks + q_blocks, kHeadsThreads, 0, s>>>(a, kv_blocks, std::max(waves, 1));
 }
 
 bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
