@@ -2,11 +2,18 @@
 // queries to a buffer, keys and values appended to a cache of 8-bit numbers.
 //
 // A block of 16 positions of a head shares a scale, so the rows of a call that lie
-// in one block are a wave's work together: the largest of their values decides
-// whether the scale holds, and where it does not, the numbers held are rounded to
-// the new one. The wave of the first of those rows does it; rows that are not the
-// first of their block have none. A row knows by the 15 rows before it, and its
-// block's others are among the 15 behind it.
+// in one block have to know each other's largest value: it decides whether the scale
+// holds, and where it does not, the numbers held are rounded to the new one. A row is
+// its block's first if none of the 15 rows before it lies there, and the block's others
+// are among the 15 behind it.
+//
+// Heads of 64 and 128: a wave takes 16 rows that hold whole blocks, four lanes a row,
+// whether they are one sequence's or 16 sequences'; the blocks' largest values meet in
+// LDS. Bound by memory and, at many rows, by what it takes to norm and rotate in fp64
+// (which the vector units run as fast as fp32): 6779 rows of 32 + 8 + 8 heads of 64
+// 18.2 us for 78 MB, 4.3 TB/s of a copy's 5.2; of 16 + 8 + 8 heads of 128 33 us for
+// 100 MB, 24 of them without the keys; 8 rows 4.2 us, a chain of three reads; 320 by
+// fives, of heads of 128, 7.1.
 #include <algorithm>
 #include <cstdint>
 
@@ -21,6 +28,10 @@ constexpr int kHeadsThreads = 256;
 constexpr int kHeadsWaves = kHeadsThreads / 64;
 constexpr int kMaxHeadDim = 256;
 constexpr int kMostWaves = 16384;  // that a call's keys and values are spread over, more or less
+// Rows that do not fill a window leave a second set in most: every second one goes to
+// waves of its own while that gives no SIMD two. 320 rows by fives, 16 on 8 heads of
+// 128, 9.7 us in turn, 7.1 so; 700 rows by fives 10.8 and 10.6, one by one 5.2 and 6.3.
+constexpr int kHalvedWaves = 512;
 
 struct Heads8Args {
   elem_t* q_out;
@@ -558,7 +569,7 @@ __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet&
 }
 
 // The first kv_blocks blocks' waves share the windows' kv heads, keys and values,
-// `waves` a window; behind them come the queries, kHeadDim / 16 lanes a head. The first
+// `waves` a window (with twice as many as those, each half has every second set); behind them come the queries, kHeadDim / 16 lanes a head. The first
 // compute, the others move bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64,
 // queries first 23 us, then 19; either alone 11 and 13.
 template <int kHeadDim>
@@ -587,13 +598,17 @@ __global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(Heads
   const int in_block = static_cast<int>(threadIdx.x) >> 6;
   const long long wave = static_cast<long long>(blockIdx.x) * kHeadsWaves + in_block;
   const int window = __builtin_amdgcn_readfirstlane(static_cast<int>(wave / waves));
-  const int share = __builtin_amdgcn_readfirstlane(static_cast<int>(wave % waves));
+  const int in_window = __builtin_amdgcn_readfirstlane(static_cast<int>(wave % waves));
   if (window * kWindowRows >= a.tokens) return;
   const Window win(a, window * kWindowRows);
   const int kv = a.view.num_kv_heads;
+  const bool halved = waves > 2 * kv;  // then 4 kv
+  const int half = halved && in_window >= 2 * kv ? 1 : 0;
+  const int share = in_window - half * 2 * kv;
   unsigned long long left = win.leaders;
-  while (left != 0) {
+  for (int at = 0; left != 0; ++at) {
     const RowSet set(a, win, left, lds_words[in_block]);
+    if (halved && (at & 1) != half) continue;
     for (int n = share; n < 2 * kv; n += waves) {
       if (n < kv) {
         append_keys<kHeadDim>(a, set, n, lds_words[in_block]);
@@ -609,7 +624,10 @@ void launch_heads(const Heads8Args& a, hipStream_t s) {
   const long long q_lanes = static_cast<long long>(a.tokens) * a.num_heads * (kHeadDim / 16);
   const unsigned q_blocks = static_cast<unsigned>((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
   const int windows = (a.tokens + kWindowRows - 1) / kWindowRows;
-  const int waves = std::min(2 * a.view.num_kv_heads, (kMostWaves + windows - 1) / windows);
+  const int shares = 2 * a.view.num_kv_heads;
+  const int waves = static_cast<long long>(windows) * shares <= kHalvedWaves
+                        ? 2 * shares
+                        : std::min(shares, (kMostWaves + windows - 1) / windows);
   const long long kv_waves = static_cast<long long>(windows) * waves;
   const unsigned kv_blocks = static_cast<unsigned>((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
   batch_kv8_heads_kernel<kHeadDim><<<kv_blocks + q_blocks, kHeadsThreads, 0, s>>>(a, kv_blocks, std::max(waves, 1));
