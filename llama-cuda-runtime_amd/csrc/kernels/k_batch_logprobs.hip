@@ -13,7 +13,10 @@
 // k) are ranked by counting. The streaming pass does nothing for it but keep the largest.
 //
 // Bound by memory: 11 operations a logit, the exponential four times as long as the
-// others, are half of the vector units' time at the rate that logits arrive.
+// others, are half of the vector units' time at the rate that logits arrive. 1500 rows
+// of 50001 logits 49 us, 6.1 TB/s of a streaming read's 7.0; 700 of 128256 with 8 ids
+// 62 us, 5.8, without ids 56. One row, in 16 parts: 5 us for the parts, 7.5 to join them
+// and choose, chains of some ten reads and exchanges.
 #include <algorithm>
 #include <climits>
 #include <cstdint>
@@ -313,7 +316,7 @@ struct PartsSource {
 // The row's logits at or above (kAbove: above) `reach` as candidates; -inf is none.
 // What the lanes that reach it had is read again, four logits at a time, by the whole
 // block. 256 rows of 128256, 20 ids: with those lanes reading theirs, one step behind
-// the other, 60 us; all that they had by the block 30; the tiles that reach it 26; no
+// the other, 60 us; all that they had by the block 30; the tiles that reach it 28; no
 // ids at all 22.
 template <bool kAbove, int kThreads, typename Source>
 __device__ __forceinline__ int gather(ChoiceLds<kThreads>& lds, const RowTiles& p, float reach, const Source& source) {

@@ -365,3 +365,54 @@ def test_row_starts_that_do_not_ascend(lcr, gpu):
             c = Case("bf16", [40, 90, 20], [4, 4, 4], heads=4, kv=2, d=d, seed=24)
             c.starts = np.array(starts, np.int32)
             c.run(lcr, max_new=12)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+def test_scales(lcr, gpu, scale):
+    for d in (64, 128, 80):
+        c = Case("bf16", [1300, 5], [2, 7], heads=4, kv=2, d=d, seed=38)
+        c.scale = scale
+        c.check(lcr)
+
+
+@pytest.mark.parametrize("variant", ["bf16", "fp16"])
+@pytest.mark.parametrize("columns", [1, 90])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_in_many_tiles_of_a_unit(lcr, gpu, variant, columns, d):
+    """Values that only a unit's later rows see, in neighbouring tiles and in every
+    second one, in one launch and (wide tables) cut: each reaches its element of the
+    rows from its position on, and nothing else changes."""
+    for past, new in (([0], [600]), ([330, 0], [290, 410])):
+        c = Case(variant, past, new, heads=1, kv=1, d=d, seed=39)
+        wide = np.full((len(past), max(columns, c.tables.shape[1])), -1, np.int32)
+        wide[:, : c.tables.shape[1]] = c.tables
+        c.tables = wide
+        clean = c.run(lcr)
+        expected = to_f32(clean, c.kind).copy()
+        r = rng(40)
+        for b, (first, n) in enumerate(zip(c.starts, new)):
+            at = sorted(r.choice(n - 2, 9, replace=False).tolist()) + [n - 2]
+            for dim, i in enumerate(at):
+                page, slot = c.place(b, past[b] + i)
+                c.cache.set_position("values", page, 0, slot, slice(dim, dim + 1), (ref.NAN, 0xFF)[dim % 2])
+                expected[first + i:first + n, 0, dim] = np.nan
+        got = to_f32(c.run(lcr), c.kind)
+        assert (np.isnan(got) == np.isnan(expected)).all()
+        assert ((got == expected) | np.isnan(expected)).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_workspace_keeps_what_lies_behind_it(lcr, gpu, d):
+    lib = lcr.load_library("bf16")
+    for past, new in (([2500, 40], [1, 1]), ([1800, 1100], [8, 3]), ([1500, 20], [60, 3])):
+        c = Case("bf16", past, new, heads=4, kv=2, d=d, seed=52)
+        size = lib.lcr_batch_attention_kv8_workspace_bytes(2, c.tokens, max(new), 4, 2, d)
+        guard = np.full(size + 4096, 0x5A, np.uint8)
+        ws, out = dev(guard), dev(np.zeros(c.tokens * 4 * d, np.uint16))
+        c.cache.upload(dev)
+        view = c.cache.view(lcr, p, p(dev(c.tables)))
+        status = lib.lcr_batch_attention_kv8(
+            p(out), p(dev(c.q)), ctypes.byref(view), p(dev(c.starts)), p(dev(c.lengths)), 2, c.tokens, max(new), 4, 2,
+            c.tables.shape[1], c.pool, c.q_stride, c.scale, p(ws), size, None)
+        assert status == 0, lib.lcr_last_error_message()
+        expect_bits_equal(host(ws, np.uint8)[size:], guard[size:], "behind the workspace")

@@ -304,3 +304,23 @@ def test_same_bits_again(lcr, gpu):
     w.call(qkv, slots, positions)
     for a, b in zip(first, (w.cache.keys, w.cache.values, w.cache.key_scales, w.cache.value_scales)):
         expect_bits_equal(a.view(np.uint8), b.view(np.uint8), "again")
+
+
+@pytest.mark.parametrize("d", [64, 128, 48])
+def test_slots_that_break_the_rules(lcr, gpu, d):
+    """The same slot for many rows, a block's rows far apart: of those blocks nothing is
+    said, the others keep what they held and the queries are as ever."""
+    w = Writer(lcr, "bf16", heads=3, kv=2, d=d, norm=False, pool=8, seed=14)
+    c = w.cache
+    for slots in (np.full(40, 33), np.tile([16, 70, 17, 71, 40], 20), np.arange(100) % 32, np.arange(64)[::-1] % 48):
+        was = [x.copy() for x in (c.keys, c.values, c.key_scales, c.value_scales)]
+        w.call(w.rows(len(slots)), slots, np.zeros(len(slots)), check=False)
+        touched, touched_scales = np.zeros(c.keys.size, bool), np.zeros(c.key_scales.size, bool)
+        for slot in set(slots.tolist()):
+            page, n = slot // 16, 0
+            touched[c.at[page, :, n]] = True
+            touched_scales[c.scales_at[page, :, n]] = True
+        for got, old in zip((c.keys, c.values), was[:2]):
+            expect_bits_equal(got[~touched], old[~touched], "other blocks")
+        for got, old in zip((c.key_scales, c.value_scales), was[2:]):
+            expect_bits_equal(got[~touched_scales], old[~touched_scales], "other blocks' scales")

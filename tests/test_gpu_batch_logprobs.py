@@ -302,3 +302,14 @@ def test_a_smaller_workspace(lcr, gpu):
     call.ws = (ws, max(need - 16, 0)) if need else (None, 0)
     call.run().check()
     sync()
+
+
+@pytest.mark.parametrize("rows,vocab,top", [(1, 128256, 32), (100, 30000, 5), (128, 9000, 20)])
+def test_a_workspace_keeps_what_lies_behind_it(lcr, gpu, rows, vocab, top):
+    call = Call(lcr, normal(rng(rows), rows, vocab), rng(1).integers(0, vocab, rows), top)
+    size = call.ws[1]
+    assert size > 0
+    guard = np.full(size + 4096, 0x5A, np.uint8)
+    call.ws = (dev(guard), size)
+    call.run().check()
+    expect_bits_equal(host(call.ws[0], np.uint8)[size:], guard[size:], "behind the workspace")
