@@ -11,9 +11,9 @@
 // whether they are one sequence's or 16 sequences'; the blocks' largest values meet in
 // LDS. Bound by memory and, at many rows, by what it takes to norm and rotate in fp64
 // (which the vector units run as fast as fp32): 6779 rows of 32 + 8 + 8 heads of 64
-// 18.2 us for 78 MB, 4.3 TB/s of a copy's 5.2; of 16 + 8 + 8 heads of 128 33 us for
+// 18.2 us for 78 MB, 4.3 TB/s of a copy's 5.2; of 16 + 8 + 8 heads of 128 34 us for
 // 100 MB, 24 of them without the keys; 8 rows 4.2 us, a chain of three reads; 320 by
-// fives, of heads of 128, 7.1.
+// fives, of heads of 128, 6.8.
 #include <algorithm>
 #include <cstdint>
 
@@ -495,8 +495,6 @@ __device__ __forceinline__ void append_keys(const Heads8Args& a, const RowSet& s
         v[j + n] = static_cast<float>(x * c - y * s);
         v[kPairs + j + n] = static_cast<float>(y * c + x * s);
       }
-      // heads of 128: what the next four need is loaded behind these, for registers
-      if constexpr (kHeadDim > 64) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
 #pragma unroll
@@ -571,9 +569,11 @@ __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet&
 // The first kv_blocks blocks' waves share the windows' kv heads, keys and values,
 // `waves` a window (with twice as many as those, each half has every second set); behind them come the queries, kHeadDim / 16 lanes a head. The first
 // compute, the others move bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64,
-// queries first 23 us, then 19; either alone 11 and 13.
+// queries first 23 us, then 19; either alone 11 and 13. Heads of 128 take 154 registers,
+// three waves a SIMD: held to 128 by loads one behind the other, 1000 rows by fives
+// 13.0 us instead of 11.6, prompts of 6779 33.7 instead of 34.8.
 template <int kHeadDim>
-__global__ __launch_bounds__(kHeadsThreads, 4) void batch_kv8_heads_kernel(Heads8Args a, unsigned kv_blocks, int waves) {
+__global__ __launch_bounds__(kHeadsThreads, 2) void batch_kv8_heads_kernel(Heads8Args a, unsigned kv_blocks, int waves) {
   __shared__ uint32_t lds_words[kHeadsWaves][16];
   if (blockIdx.x >= kv_blocks) {
     const unsigned q_block = blockIdx.x - kv_blocks;
