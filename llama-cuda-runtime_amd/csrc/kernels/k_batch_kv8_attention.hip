@@ -197,6 +197,12 @@ __device__ __forceinline__ BlockScales load_scales(const Args& a, const KvPiece&
                      ((constant_floats)(reinterpret_cast<uintptr_t>(a.view.value_scales)))[at]};
 }
 
+// A block's first byte in its page: in 64 bits, as a page may have more than 2^32.
+template <typename Shape>
+__device__ __forceinline__ size_t block_in_page(int block) {
+  return static_cast<size_t>(static_cast<uint32_t>(block)) * Shape::kBlockBytes;
+}
+
 template <typename Shape>
 __device__ __forceinline__ uint32_t key_chunk_at(int h) {
   return static_cast<uint32_t>((lane_id() & 15) * Shape::kHeadDim + 64 * h + 16 * (lane_id() >> 4));
@@ -287,8 +293,7 @@ __device__ __forceinline__ void few_rows(Lds8<Shape>& lds, const Args& a, const 
     for (int n = 0; n < kBlocks; ++n) {
       const int page = pool_page(a, places.of[n].page, bad);
       const int block = places.of[n].block;
-      at.of[n] = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                 static_cast<size_t>(static_cast<uint32_t>(block * Shape::kBlockBytes));
+      at.of[n] = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) + block_in_page<Shape>(block);
 #pragma unroll
       for (int h = 0; h < Shape::kChunks; ++h) {
         tile.keys[n][h] = load_numbers<true>(p.keys + at.of[n], key_chunk_at<Shape>(h));
@@ -423,8 +428,8 @@ __device__ __forceinline__ void many_rows(Lds8<Shape>& lds, const Args& a, const
   auto place_of = [&](int t) { return find_block(a, plan, p, (p.key0 + 64 * t) / kKv8Block + my_block); };
   auto load = [&](const BlockPlace& place) {
     const int page = pool_page(a, place.page, bad);
-    const size_t at = static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) +
-                      static_cast<size_t>(place.block * Shape::kBlockBytes);
+    const size_t at =
+        static_cast<size_t>(page) * static_cast<size_t>(a.view.page_stride) + block_in_page<Shape>(place.block);
     Raw raw;
     raw.keys = load_numbers<false>(p.keys + at, key_chunk_at<Shape>(my_chunk));
     raw.values = load_numbers<false>(p.values + at, value_chunk_at<Shape>(my_chunk));
