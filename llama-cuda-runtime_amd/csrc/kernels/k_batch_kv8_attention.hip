@@ -107,8 +107,8 @@ struct Lds8 {
 // chunks take 147 us for 158, and two of them beside 16 single tokens 66 for 72;
 // falling by quarters 150 and 68.
 struct Pace {
-  int left;       // steps of the share
-  int next;       // steps done at which the priority falls
+  int left = 0;   // steps of the share
+  int next = 0;   // steps done at which the priority falls
   int level = 0;  // the priority; at 0 it stays
 
   __device__ __forceinline__ void begin(int steps) {
@@ -118,7 +118,7 @@ struct Pace {
     __builtin_amdgcn_s_setprio(3);
   }
   __device__ __forceinline__ void reached(int steps) {
-    while (steps >= next && level > 0) {
+    while (level > 0 && steps >= next) {
       next += left - (left >> 1);
       left >>= 1;
       --level;
@@ -132,6 +132,9 @@ struct Pace {
     }
   }
 };
+// Of a call whose units are not cut, which begins none: a constant, so that it does
+// not compile with a member left without a value.
+constexpr Pace kUnpaced;
 
 // Two neighbouring numbers of a word as elements.
 template <bool kHigh>
@@ -545,7 +548,7 @@ __global__ __launch_bounds__(Shape::kThreads, Shape::kSimdWaves) void batch_atte
   // seen by every wave behind the barriers of the search for the share
   if (threadIdx.x == 0) lds.special[0] = lds.special[1] = -1;
   int tiles_done = 0;
-  Pace pace;
+  Pace pace = kUnpaced;
   walk_share<Shape, kMany, uint8_t>(
       a, plan, lds.sums, &lds.found, [&](int steps) { if (Shape::kPaced && plan.split) pace.begin(steps); },
       [&](const KvPiece& p) { few_rows<Shape, kTileRows>(lds, a, plan, p, pace); },
