@@ -664,31 +664,37 @@ __global__ __launch_bounds__(kGenericThreads) void batch_attention_kv8_generic_k
   }
 }
 
+// A launch has fewer than 2^32 threads in all.
+int check_threads(const Args& a, long long blocks, int threads) {
+  CAPI_CHECK(blocks * threads <= UINT32_MAX, "batch attention of " << a.tokens << " rows of " << a.num_heads
+                                                                   << " heads needs more than 2^32 threads");
+  return LCR_OK;
+}
+
 template <int kHeadDim, int kMaxRows>
-void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+int launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
   using Shape = Shape8<kHeadDim, kMaxRows>;
   constexpr int kTileRows = kMaxRows == 0 ? Shape::kTileRows : kFewRows;
   const TiledPlan plan = plan_tiled<Shape>(a, workspace, workspace_bytes);
+  const int status = check_threads(a, static_cast<long long>(plan.shares) * a.view.num_kv_heads, Shape::kThreads);
+  if (status != LCR_OK) return status;
   const unsigned blocks = static_cast<unsigned>(plan.shares) * static_cast<unsigned>(a.view.num_kv_heads);
   batch_attention_kv8_kernel<Shape><<<blocks, Shape::kThreads, 0, s>>>(a, plan);
-  if (!plan.split) return;
+  if (!plan.split) return LCR_OK;
   // A row is a chain of loads, so none follows another.
   constexpr bool kRowEach = kMaxRows == 0;
   const int few_rows = static_cast<int>(std::min<long long>(static_cast<long long>(a.max_new) * a.group, kFewRows));
   const dim3 join(blocks, kRowEach ? kTileRows / (4 * 256 / kHeadDim) : (few_rows + 3) / 4);
   batch_attention_join_kernel<kHeadDim, kRowEach, Args><<<join, kJoinThreads, 0, s>>>(a, plan, kTileRows);
+  return LCR_OK;
 }
 
 template <int kHeadDim>
-void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
+int launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStream_t s) {
   const long long most = static_cast<long long>(a.max_new) * a.group;
-  if (most <= 16) {
-    launch_tiled<kHeadDim, 16>(a, workspace, workspace_bytes, s);
-  } else if (most <= kFewRows) {
-    launch_tiled<kHeadDim, 32>(a, workspace, workspace_bytes, s);
-  } else {
-    launch_tiled<kHeadDim, 0>(a, workspace, workspace_bytes, s);
-  }
+  if (most <= 16) return launch_tiled<kHeadDim, 16>(a, workspace, workspace_bytes, s);
+  if (most <= kFewRows) return launch_tiled<kHeadDim, 32>(a, workspace, workspace_bytes, s);
+  return launch_tiled<kHeadDim, 0>(a, workspace, workspace_bytes, s);
 }
 
 bool on_bytes(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -764,26 +770,17 @@ extern "C" int lcr_batch_attention_kv8(void* out, const void* q, const lcr_kv8_v
                    lengths, batch, tokens, max_new, num_heads, heads_per_kv, table_stride, pool_pages, q_row_stride,
                    table_stride * view->page_size, scale};
   auto s = static_cast<hipStream_t>(stream);
-  const bool tiled = tiled_takes(a);
-  // A launch has fewer than 2^32 threads in all.
-  const long long units = static_cast<long long>(tokens) * num_heads;
-  const long long blocks =
-      !tiled ? (units + kGenericWaves - 1) / kGenericWaves
-             : view->num_kv_heads * (view->head_dim == 64 ? most_tiled_units<Shape8<64, 32>>(a)
-                                                          : most_tiled_units<Shape8<128, 32>>(a));
-  const int threads = !tiled ? kGenericThreads : view->head_dim == 64 ? Shape8<64, 0>::kThreads : Shape8<128, 0>::kThreads;
-  CAPI_CHECK(blocks * threads <= UINT32_MAX, "batch attention of " << tokens << " rows of " << num_heads
-                                                                   << " heads needs more than 2^32 threads");
-  if (tiled) {
-    if (view->head_dim == 64) {
-      launch_tiled<64>(a, workspace, workspace_bytes, s);
-    } else {
-      launch_tiled<128>(a, workspace, workspace_bytes, s);
-    }
-    CAPI_LAUNCHED();
-    return LCR_OK;
+  if (tiled_takes(a)) {
+    const int status = view->head_dim == 64 ? launch_tiled<64>(a, workspace, workspace_bytes, s)
+                                            : launch_tiled<128>(a, workspace, workspace_bytes, s);
+    if (status != LCR_OK) return status;
+  } else {
+    const long long units = static_cast<long long>(tokens) * num_heads;
+    const long long blocks = (units + kGenericWaves - 1) / kGenericWaves;
+    const int status = check_threads(a, blocks, kGenericThreads);
+    if (status != LCR_OK) return status;
+    batch_attention_kv8_generic_kernel<<<static_cast<unsigned>(blocks), kGenericThreads, 0, s>>>(a);
   }
-  batch_attention_kv8_generic_kernel<<<static_cast<unsigned>(blocks), kGenericThreads, 0, s>>>(a);
   CAPI_LAUNCHED();
   return LCR_OK;
 }
