@@ -27,11 +27,17 @@ namespace {
 constexpr int kHeadsThreads = 256;
 constexpr int kHeadsWaves = kHeadsThreads / 64;
 constexpr int kMaxHeadDim = 256;
-constexpr int kMostWaves = 16384;  // that a call's keys and values are spread over, more or less
+// Waves a compute unit that a call's keys and values are spread over, more or less:
+// with more rows a wave takes several heads of its own, having looked for their blocks
+// once. With 64, 32 and a wave a head: 28783 rows of 32 on 8 heads of 64 91, 89 and 98
+// us, of 16 on 8 of 128 127, 129 and 133, 10049 of 32 on 32 of 64 62, 62 and 76, 20000
+// of sequences of their own 81, 83 and 87.
+constexpr int kMostWaves = 64;
 // Rows that do not fill a window leave a second set in most: every second one goes to
-// waves of its own while that gives no SIMD two. 320 rows by fives, 16 on 8 heads of
-// 128, 9.7 us in turn, 7.1 so; 700 rows by fives 10.8 and 10.6, one by one 5.2 and 6.3.
-constexpr int kHalvedWaves = 512;
+// waves of its own while that gives no SIMD two (by the waves a compute unit there are
+// without). 320 rows by fives, 16 on 8 heads of 128, 9.7 us in turn, 7.1 so; 700 rows by
+// fives 10.8 and 10.6, one by one 5.2 and 6.3.
+constexpr int kHalvedWaves = 2;
 
 struct Heads8Args {
   elem_t* q_out;
@@ -571,7 +577,8 @@ __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet&
 // compute, the others move bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64,
 // queries first 23 us, then 19; either alone 11 and 13. Heads of 128 take 154 registers,
 // three waves a SIMD: held to 128 by loads one behind the other, 1000 rows by fives
-// 13.0 us instead of 11.6, prompts of 6779 33.7 instead of 34.8.
+// take 13.0 us for 11.6, 2500 18.2 for 16.1, prompts of 6779 33.2 for 32.8 without a norm
+// and 34.1 for 35.1 with one.
 template <int kHeadDim>
 __global__ __launch_bounds__(kHeadsThreads, 2) void batch_kv8_heads_kernel(Heads8Args a, unsigned kv_blocks, int waves) {
   __shared__ uint32_t lds_words[kHeadsWaves][16];
@@ -625,9 +632,10 @@ void launch_heads(const Heads8Args& a, hipStream_t s) {
   const unsigned q_blocks = static_cast<unsigned>((q_lanes + kHeadsThreads - 1) / kHeadsThreads);
   const int windows = (a.tokens + kWindowRows - 1) / kWindowRows;
   const int shares = 2 * a.view.num_kv_heads;
-  const int waves = static_cast<long long>(windows) * shares <= kHalvedWaves
+  const int units = device_compute_units();
+  const int waves = static_cast<long long>(windows) * shares <= kHalvedWaves * units
                         ? 2 * shares
-                        : std::min(shares, (kMostWaves + windows - 1) / windows);
+                        : std::min(shares, (kMostWaves * units + windows - 1) / windows);
   const long long kv_waves = static_cast<long long>(windows) * waves;
   const unsigned kv_blocks = static_cast<unsigned>((kv_waves + kHeadsWaves - 1) / kHeadsWaves);
   batch_kv8_heads_kernel<kHeadDim><<<kv_blocks + q_blocks, kHeadsThreads, 0, s>>>(a, kv_blocks, std::max(waves, 1));
