@@ -118,7 +118,7 @@ struct Pace {
     __builtin_amdgcn_s_setprio(3);
   }
   __device__ __forceinline__ void reached(int steps) {
-    while (level > 0 && steps >= next) {
+    while (steps >= next && level > 0) {
       next += left - (left >> 1);
       left >>= 1;
       --level;
