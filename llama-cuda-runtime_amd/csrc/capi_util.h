@@ -6,6 +6,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <sstream>
 #include <string>
 
@@ -30,6 +31,10 @@ int guarded(F&& body) {
 }
 
 }  // namespace capi
+
+// Whether a pointer is a multiple of n, a power of two.
+inline bool on_bytes(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
 }  // namespace lcr
 
 #define CAPI_CHECK(cond, msg)                       \

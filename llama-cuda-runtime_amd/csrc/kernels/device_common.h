@@ -115,6 +115,13 @@ __device__ __forceinline__ void plain_barrier() {
   asm volatile("" : : : "memory");
 }
 
+// What a wave alone writes to LDS is there for its other lanes behind this.
+__device__ __forceinline__ void wave_settled() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // LDS byte address of a __shared__ object.
 __device__ __forceinline__ uint32_t lds_address_of(const void* p) {
   typedef const __attribute__((address_space(3))) char* lds_char_ptr;
@@ -274,6 +281,14 @@ __device__ __forceinline__ float xor_lane(float v) {
   return __builtin_bit_cast(float, xor_lane_bits<kMask>(__builtin_bit_cast(int, v)));
 }
 
+template <int kMask>
+__device__ __forceinline__ double xor_lane_f64(double v) {
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits))));
+  const uint32_t hi = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits >> 32))));
+  return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
+}
+
 // Butterfly over the 64 lanes of a wavefront, offsets 32, 16, 8, 4, 2, 1.
 // Lane i adds lane i^o at each step; addition commutes, so every lane ends
 // with the same bits.
@@ -285,6 +300,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   v += xor_lane<2>(v);
   v += xor_lane<1>(v);
   return v;
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+  v += xor_lane_f64<32>(v);
+  v += xor_lane_f64<16>(v);
+  v += xor_lane_f64<8>(v);
+  v += xor_lane_f64<4>(v);
+  v += xor_lane_f64<2>(v);
+  return v + xor_lane_f64<1>(v);
 }
 __device__ __forceinline__ float wave_max(float v) {
   v = fmaxf(v, xor_lane<32>(v));

@@ -549,8 +549,6 @@ void launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStr
   }
 }
 
-bool on_bytes(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
 // The matrix-core kernels take a positive scale (the running maximum is the
 // scores') and a group that fits a tile.
 bool tiled_takes(const Args& a) {

@@ -152,8 +152,6 @@ void launch_heads(const HeadsArgs& a, hipStream_t s) {
   batch_heads_kernel<kHeadDim><<<blocks, kHeadsThreads, 0, s>>>(a);
 }
 
-bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace lcr
 
@@ -206,9 +204,9 @@ extern "C" int lcr_batch_norm_rope_write_kv(void* q_out, const lcr_kv_view* view
   a.pool_slots = pool_pages * view->page_size;
   a.src_row_stride = src_row_stride;
   auto s = static_cast<hipStream_t>(stream);
-  const bool aligned = on_16_bytes(q_out) && on_16_bytes(q) && on_16_bytes(k) && on_16_bytes(v) &&
-                       on_16_bytes(q_norm) && on_16_bytes(k_norm) && on_16_bytes(rope_table) &&
-                       on_16_bytes(view->keys) && on_16_bytes(view->values) && src_row_stride % 8 == 0 &&
+  const bool aligned = on_bytes(q_out, 16) && on_bytes(q, 16) && on_bytes(k, 16) && on_bytes(v, 16) &&
+                       on_bytes(q_norm, 16) && on_bytes(k_norm, 16) && on_bytes(rope_table, 16) &&
+                       on_bytes(view->keys, 16) && on_bytes(view->values, 16) && src_row_stride % 8 == 0 &&
                        view->page_stride % 8 == 0 && view->head_stride % 8 == 0;
   // A launch has fewer than 2^32 threads in all.
   CAPI_CHECK(tokens * heads * head_lanes(a, aligned) <= UINT32_MAX - kHeadsThreads,

@@ -565,12 +565,6 @@ constexpr int kGenericWaves = 4;
 constexpr int kGenericThreads = 64 * kGenericWaves;
 constexpr int kGenericMaxDim = 256;
 
-__device__ __forceinline__ void wave_settled() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Lane L of a 64-key tile takes key L's whole dot product; the tile's weights, with
 // their scales, go through LDS, and lane L then holds elements L, L + 64, ... of
 // the output. Nothing is shared between heads or rows and nothing split: the way
@@ -696,8 +690,6 @@ int launch_tiled(const Args& a, void* workspace, size_t workspace_bytes, hipStre
   if (most <= kFewRows) return launch_tiled<kHeadDim, 32>(a, workspace, workspace_bytes, s);
   return launch_tiled<kHeadDim, 0>(a, workspace, workspace_bytes, s);
 }
-
-bool on_bytes(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 // The matrix-core kernels take a positive scale (the running maximum is the
 // scores') and a group that fits a tile.

@@ -62,29 +62,6 @@ __device__ __forceinline__ bool row_is_live(const Heads8Args& a, int slot, int p
   return slot >= 0 && slot < a.pool_slots && position >= 0 && position < a.table_positions;
 }
 
-template <int kMask>
-__device__ __forceinline__ double xor_lane_f64(double v) {
-  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t lo = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits))));
-  const uint32_t hi = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits >> 32))));
-  return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
-}
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  v += xor_lane_f64<32>(v);
-  v += xor_lane_f64<16>(v);
-  v += xor_lane_f64<8>(v);
-  v += xor_lane_f64<4>(v);
-  v += xor_lane_f64<2>(v);
-  return v + xor_lane_f64<1>(v);
-}
-
-__device__ __forceinline__ void wave_settled() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Which rows of a call write to a block: lanes 0 .. 30 look at rows row - 15 ..
 // row + 15.
 struct BlockRows {
@@ -641,8 +618,6 @@ void launch_heads(const Heads8Args& a, hipStream_t s) {
   batch_kv8_heads_kernel<kHeadDim><<<kv_blocks + q_blocks, kHeadsThreads, 0, s>>>(a, kv_blocks, std::max(waves, 1));
 }
 
-bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace lcr
 
@@ -701,8 +676,8 @@ extern "C" int lcr_batch_norm_rope_write_kv8(void* q_out, const lcr_kv8_view* vi
   a.pool_slots = pool_pages * view->page_size;
   a.src_row_stride = src_row_stride;
   auto s = static_cast<hipStream_t>(stream);
-  const bool aligned = on_16_bytes(q_out) && on_16_bytes(q) && on_16_bytes(k) && on_16_bytes(v) &&
-                       on_16_bytes(q_norm) && on_16_bytes(k_norm) && on_16_bytes(rope_table) && src_row_stride % 8 == 0;
+  const bool aligned = on_bytes(q_out, 16) && on_bytes(q, 16) && on_bytes(k, 16) && on_bytes(v, 16) &&
+                       on_bytes(q_norm, 16) && on_bytes(k_norm, 16) && on_bytes(rope_table, 16) && src_row_stride % 8 == 0;
   if (aligned && view->head_dim == 64) {
     launch_heads<64>(a, s);
   } else if (aligned && view->head_dim == 128) {

@@ -96,23 +96,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ float below(float l, float max) { return fmaxf(l - max, -3.0e38f); }
 __device__ __forceinline__ float weight(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-template <int kMask>
-__device__ __forceinline__ double xor_lane_f64(double v) {
-  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t lo = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits))));
-  const uint32_t hi = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits >> 32))));
-  return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
-}
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  v += xor_lane_f64<32>(v);
-  v += xor_lane_f64<16>(v);
-  v += xor_lane_f64<8>(v);
-  v += xor_lane_f64<4>(v);
-  v += xor_lane_f64<2>(v);
-  return v + xor_lane_f64<1>(v);
-}
-
 // A row in tiles of kTile places, cut into parts. Loads are 16-byte aligned, so that
 // index i of the row is place i + shift of them; places outside the row hold -inf.
 struct RowTiles {

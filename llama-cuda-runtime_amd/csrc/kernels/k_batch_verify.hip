@@ -178,23 +178,6 @@ struct Exp2 {
   }
 };
 
-template <int kMask>
-__device__ __forceinline__ double xor_lane_f64(double v) {
-  const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
-  const uint32_t lo = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits))));
-  const uint32_t hi = static_cast<uint32_t>(xor_lane_bits<kMask>(static_cast<int>(static_cast<uint32_t>(bits >> 32))));
-  return __builtin_bit_cast(double, (static_cast<unsigned long long>(hi) << 32) | lo);
-}
-
-__device__ __forceinline__ double wave_sum_f64(double v) {
-  v += xor_lane_f64<32>(v);
-  v += xor_lane_f64<16>(v);
-  v += xor_lane_f64<8>(v);
-  v += xor_lane_f64<4>(v);
-  v += xor_lane_f64<2>(v);
-  return v + xor_lane_f64<1>(v);
-}
-
 // v of another lane by DPP, 0 in lanes that get none.
 template <int kControl, int kRowMask, bool kBoundZero>
 __device__ __forceinline__ double dpp_f64(double v) {
