@@ -264,7 +264,8 @@ typedef struct lcr_kv8_view {
  * All rows of a call whose slots lie in one block have to be among 16 rows that
  * follow each other, as those of a sequence are; slots differ from row to row. Of
  * blocks for which that is not so, nothing is said but that nothing out of bounds
- * is touched. */
+ * is touched. A call takes up to 2^26 - 4 heads, of queries, keys and values of all
+ * rows together. */
 int lcr_batch_norm_rope_write_kv8(void* q_out, const lcr_kv8_view* view, const void* q, const void* k,
                                   const void* v, const void* q_norm, const void* k_norm, float eps,
                                   const float* rope_table, int table_positions, const int32_t* positions,
@@ -274,7 +275,10 @@ int lcr_batch_norm_rope_write_kv8(void* q_out, const lcr_kv8_view* view, const v
 /* lcr_batch_attention over an 8-bit cache: of the values that the cache stands for,
  * the same results, to the rounding of sums, with the same arguments, limits and
  * workspace rules (head_dim a multiple of 16 up to 256; 64 and 128 run on the matrix
- * cores). Positions that no row of a sequence sees may hold anything, scales
+ * cores). There too the weights exp(s - max) are rounded to the element type on the
+ * matrix cores, for the value product and for their sum alike: by half a step each,
+ * and in fp16 by 2^-32 of the row's largest where that is more. Statistics and sums are
+ * fp32. Pages may be of any size that a table holds, also past 2^32 bytes. Positions that no row of a sequence sees may hold anything, scales
  * included, and numbers that a row does not see leave it as it is; a NaN that it sees
  * makes its element NaN, also where the weight rounds to 0. */
 int lcr_batch_attention_kv8(void* out, const void* q, const lcr_kv8_view* view, const int32_t* row_starts,

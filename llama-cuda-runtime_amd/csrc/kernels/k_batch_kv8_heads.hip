@@ -11,9 +11,9 @@
 // whether they are one sequence's or 16 sequences'; the blocks' largest values meet in
 // LDS. Bound by memory and, at many rows, by what it takes to norm and rotate in fp64
 // (which the vector units run as fast as fp32): 6779 rows of 32 + 8 + 8 heads of 64
-// 18.2 us for 78 MB, 4.3 TB/s of a copy's 5.2; of 16 + 8 + 8 heads of 128 34 us for
-// 100 MB, 24 of them without the keys; 8 rows 4.2 us, a chain of three reads; 320 by
-// fives, of heads of 128, 6.8.
+// 18.2 us for 78 MB, 4.3 TB/s of a copy's 5.2; of 16 + 8 + 8 heads of 128 33 us for
+// 100 MB (35 with norms, 24 without the keys); 8 rows 4.2 us, a chain of three reads; 64
+// sequences of up to five rows, of heads of 128, 6.8.
 #include <algorithm>
 #include <cstdint>
 
@@ -35,8 +35,8 @@ constexpr int kMaxHeadDim = 256;
 constexpr int kMostWaves = 64;
 // Rows that do not fill a window leave a second set in most: every second one goes to
 // waves of its own while that gives no SIMD two (by the waves a compute unit there are
-// without). 320 rows by fives, 16 on 8 heads of 128, 9.7 us in turn, 7.1 so; 700 rows by
-// fives 10.8 and 10.6, one by one 5.2 and 6.3.
+// without). 64 sequences of up to five rows, 16 on 8 heads of 128, 9.7 us in turn, 7.1
+// so; 140 of them 10.8 and 10.6, 700 of one row 5.2 and 6.3.
 constexpr int kHalvedWaves = 2;
 
 struct Heads8Args {
@@ -550,12 +550,13 @@ __device__ __forceinline__ void append_values(const Heads8Args& a, const RowSet&
 }
 
 // The first kv_blocks blocks' waves share the windows' kv heads, keys and values,
-// `waves` a window (with twice as many as those, each half has every second set); behind them come the queries, kHeadDim / 16 lanes a head. The first
-// compute, the others move bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64,
-// queries first 23 us, then 19; either alone 11 and 13. Heads of 128 take 154 registers,
-// three waves a SIMD: held to 128 by loads one behind the other, 1000 rows by fives
-// take 13.0 us for 11.6, 2500 18.2 for 16.1, prompts of 6779 33.2 for 32.8 without a norm
-// and 34.1 for 35.1 with one.
+// `waves` a window (with twice as many as those, each half has every second set); behind
+// them come the queries, kHeadDim / 16 lanes a head. The first compute, the others move
+// bytes, and so they overlap: 6779 rows of 32 on 8 heads of 64, queries first 23 us, then
+// 19; either alone 11 and 13. Heads of 128 take 154 registers, three waves a SIMD: held
+// to 128 by loads one behind the other, 200 sequences of up to five rows take 13.0 us for
+// 11.6, 500 18.2 for 16.1, prompts of 6779 33.2 for 32.8 without a norm and 34.1 for 35.1
+// with one.
 template <int kHeadDim>
 __global__ __launch_bounds__(kHeadsThreads, 2) void batch_kv8_heads_kernel(Heads8Args a, unsigned kv_blocks, int waves) {
   __shared__ uint32_t lds_words[kHeadsWaves][16];
